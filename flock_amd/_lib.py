@@ -71,6 +71,17 @@ SIGNATURES: dict[str, tuple] = {
         _i32,
         [_p, _p, _p, _p, _p, _p, _f32, _i32, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32,
          _u32, _p, _u64]),
+    "flk_kv4_page_bytes": (_u64, [_u32, _u32, _u32]),
+    "flk_kv4_plan_ws_bytes": (_u64, [_u32]),
+    "flk_kv4_plan": (_i32, [_p] * 10 + [_u32] * 7 + [_p, _u64]),
+    "flk_kv4_prologue": (
+        _i32,
+        [_p, _p, _p, _u32, _p, _p, _p, _f32, _i32, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32,
+         _u32]),
+    "flk_kv4_append": (_i32, [_p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32]),
+    "flk_kv4_read": (_i32, [_p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32]),
+    "flk_kv4_attn_ws_bytes": (_u64, [_u32] * 8),
+    "flk_kv4_attn": (_i32, [_p] * 6 + [_u32] * 12 + [_p, _u64]),
     # include/flock_q8.h
     "flk_q8_matvec": (_i32, [_p, _p, _p, _p, _u32, _u32, _u32]),
     "flk_q8_split": (_i32, [_p, _u32, _u32, _p, _p]),

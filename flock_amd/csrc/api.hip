@@ -11,6 +11,7 @@
 #include <mutex>
 
 #include "common.hpp"
+#include "kv4.hpp"
 
 namespace flk {
 
@@ -866,4 +867,205 @@ int32_t flk_graph_launch(void* graph) {
 int32_t flk_graph_destroy(void* graph) {
   if (graph == nullptr) return FLK_OK;
   return hip_status(hipGraphExecDestroy(static_cast<hipGraphExec_t>(graph)), "hipGraphExecDestroy");
+}
+
+// ------------------------------------------------- paged cache in 4 bits ---
+static bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
+
+static int32_t check_words(const void* p, const char* name) {
+  if (reinterpret_cast<uintptr_t>(p) % 4 != 0)
+    return fail(FLK_ERR_ARG, "%s must be 4-byte aligned", name);
+  return FLK_OK;
+}
+
+// A non-null device array of 32-bit words.
+#define FLK_WORDS(p)                          \
+  do {                                        \
+    FLK_NONNULL(p);                           \
+    if (int32_t rc_ = check_words((p), #p)) return rc_; \
+  } while (0)
+
+static int32_t check_pages(uint32_t n_pages, uint32_t page) {
+  if (page != 32 && page != 64 && page != 128 && page != 256)
+    return fail(FLK_ERR_UNSUPPORTED, "pages of %u tokens not supported (32, 64, 128 or 256)", page);
+  if (n_pages == 0) return fail(FLK_ERR_ARG, "n_pages must be >= 1");
+  if ((uint64_t)n_pages * page > 0xFFFFFFFFull)
+    return fail(FLK_ERR_UNSUPPORTED, "%u pages of %u tokens: slots are 32-bit numbers", n_pages,
+                page);
+  return FLK_OK;
+}
+
+static int32_t check_kv4(const void* pool, uint32_t n_heads, uint32_t n_kv_heads,
+                         uint32_t head_dim, uint32_t n_pages, uint32_t page) {
+  FLK_NONNULL(pool);
+  FLK_ALIGNED(pool);
+  if (int32_t rc = check_heads(n_heads, n_kv_heads, head_dim)) return rc;
+  return check_pages(n_pages, page);
+}
+
+uint64_t flk_kv4_page_bytes(uint32_t n_kv_heads, uint32_t head_dim, uint32_t page) {
+  if (n_kv_heads == 0 || (head_dim != 64 && head_dim != 128) ||
+      (page != 32 && page != 64 && page != 128 && page != 256))
+    return 0;
+  return (uint64_t)n_kv_heads * (page / kKv4Tile) * 36 * head_dim;
+}
+
+uint64_t flk_kv4_plan_ws_bytes(uint32_t n_seqs) {
+  return n_seqs == 0 || n_seqs > 65535 ? 0 : kv4_plan_ws_bytes(n_seqs);
+}
+
+int32_t flk_kv4_plan(const uint32_t* n_keys, const uint32_t* n_new, const uint32_t* table_in,
+                     uint32_t* table_out, const uint32_t* free_in, uint32_t* free_out,
+                     uint32_t* q_off, uint32_t* positions, uint32_t* slots, uint32_t* lost,
+                     uint32_t n_seqs, uint32_t max_blocks, uint32_t n_pages, uint32_t max_tokens,
+                     uint32_t page, uint32_t window, uint32_t n_sinks, void* ws,
+                     uint64_t ws_bytes) {
+  FLK_WORDS(n_keys);
+  FLK_WORDS(n_new);
+  FLK_WORDS(table_in);
+  FLK_WORDS(table_out);
+  FLK_WORDS(free_in);
+  FLK_WORDS(free_out);
+  FLK_WORDS(q_off);
+  FLK_WORDS(positions);
+  FLK_WORDS(slots);
+  FLK_WORDS(lost);
+  if (int32_t rc = check_pages(n_pages, page)) return rc;
+  if (n_seqs == 0 || max_blocks == 0 || max_tokens == 0)
+    return fail(FLK_ERR_ARG, "kv4_plan n_seqs=%u max_blocks=%u max_tokens=%u", n_seqs, max_blocks,
+                max_tokens);
+  if (n_seqs > 65535) return fail(FLK_ERR_UNSUPPORTED, "kv4_plan n_seqs %u exceeds 65535", n_seqs);
+  if (overlap(free_in, 4 * (1 + (uint64_t)n_pages), free_out, 4 * (1 + (uint64_t)n_pages)))
+    return fail(FLK_ERR_ARG, "kv4_plan: free_out lies over free_in");
+  const uint64_t table_bytes = 4ull * n_seqs * max_blocks;
+  if (table_in != table_out && overlap(table_in, table_bytes, table_out, table_bytes))
+    return fail(FLK_ERR_ARG, "kv4_plan: table_out lies partly over table_in");
+  if (int32_t rc = check_ws(ws, ws_bytes, kv4_plan_ws_bytes(n_seqs))) return rc;
+  const Kv4PlanArgs a{n_keys, n_new,      table_in, free_in,    table_out, free_out, q_off, positions,
+                      slots,  lost,       n_seqs,   max_blocks, n_pages,   max_tokens, page, window,
+                      n_sinks};
+  return hip_status(launch_kv4_plan(a, ws, g_stream), "flk_kv4_plan");
+}
+
+int32_t flk_kv4_prologue(const float* q_raw, const float* k_raw, const float* v_raw,
+                         uint32_t in_stride, const float* gq, const float* gk,
+                         const float* inv_freq, float eps, int32_t pairing,
+                         const uint32_t* positions, const uint32_t* slots, float* qn_out,
+                         void* pool, uint32_t n_tokens, uint32_t n_heads, uint32_t n_kv_heads,
+                         uint32_t head_dim, uint32_t n_pages, uint32_t page) {
+  FLK_NONNULL(q_raw);
+  FLK_NONNULL(k_raw);
+  FLK_NONNULL(v_raw);
+  FLK_NONNULL(gq);
+  FLK_NONNULL(gk);
+  FLK_NONNULL(inv_freq);
+  FLK_WORDS(positions);
+  FLK_WORDS(slots);
+  FLK_NONNULL(qn_out);
+  if (int32_t rc = check_kv4(pool, n_heads, n_kv_heads, head_dim, n_pages, page)) return rc;
+  if (n_tokens == 0) return fail(FLK_ERR_ARG, "n_tokens must be >= 1, got 0");
+  if (pairing != FLK_ROPE_NEOX && pairing != FLK_ROPE_NORM)
+    return fail(FLK_ERR_ARG, "rope pairing %d (0 = neox, 1 = norm)", pairing);
+  if (in_stride != 0 && in_stride < n_heads * head_dim)
+    return fail(FLK_ERR_ARG, "in_stride %u is shorter than a q row (%u floats)", in_stride,
+                n_heads * head_dim);
+  Kv4AppendArgs a{};
+  a.q = q_raw, a.k = k_raw, a.v = v_raw;
+  a.q_stride = in_stride ? in_stride : n_heads * head_dim;
+  a.kv_stride = in_stride ? in_stride : n_kv_heads * head_dim;
+  a.gq = gq, a.gk = gk, a.inv_freq = inv_freq;
+  a.eps = eps, a.pairing = pairing;
+  a.positions = positions, a.slots = slots;
+  a.qn_out = qn_out;
+  a.pool = static_cast<uint8_t*>(pool);
+  a.n_tokens = n_tokens, a.n_heads = n_heads;
+  a.s = Kv4Shape{n_kv_heads, head_dim, n_pages, page};
+  return hip_status(launch_kv4_append(a, g_stream), "flk_kv4_prologue");
+}
+
+int32_t flk_kv4_append(const float* kn, const float* v, const uint32_t* slots, void* pool,
+                       uint32_t n_tokens, uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_pages,
+                       uint32_t page) {
+  FLK_NONNULL(kn);
+  FLK_NONNULL(v);
+  FLK_WORDS(slots);
+  if (int32_t rc = check_kv4(pool, n_kv_heads, n_kv_heads, head_dim, n_pages, page)) return rc;
+  if (n_tokens == 0) return fail(FLK_ERR_ARG, "n_tokens must be >= 1, got 0");
+  Kv4AppendArgs a{};
+  a.k = kn, a.v = v;
+  a.kv_stride = n_kv_heads * head_dim;
+  a.slots = slots;
+  a.pool = static_cast<uint8_t*>(pool);
+  a.n_tokens = n_tokens;
+  a.s = Kv4Shape{n_kv_heads, head_dim, n_pages, page};
+  return hip_status(launch_kv4_append(a, g_stream), "flk_kv4_append");
+}
+
+int32_t flk_kv4_read(const void* pool, const uint32_t* slots, float* k, float* v,
+                     uint32_t n_tokens, uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_pages,
+                     uint32_t page) {
+  FLK_WORDS(slots);
+  FLK_NONNULL(k);
+  FLK_NONNULL(v);
+  FLK_ALIGNED(k);
+  FLK_ALIGNED(v);
+  if (int32_t rc = check_kv4(pool, n_kv_heads, n_kv_heads, head_dim, n_pages, page)) return rc;
+  if (n_tokens == 0) return fail(FLK_ERR_ARG, "n_tokens must be >= 1, got 0");
+  if ((uint64_t)n_tokens * n_kv_heads * (head_dim / 4) > 0xFFFFFFFFull * 64)
+    return fail(FLK_ERR_UNSUPPORTED, "kv4_read of %u tokens exceeds the grid", n_tokens);
+  return hip_status(launch_kv4_read(static_cast<const uint8_t*>(pool), slots, k, v, n_tokens,
+                                    Kv4Shape{n_kv_heads, head_dim, n_pages, page}, g_stream),
+                    "flk_kv4_read");
+}
+
+uint64_t flk_kv4_attn_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
+                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                               uint32_t window, uint32_t n_sinks) {
+  if (n_seqs == 0 || n_seqs > 65535 || max_q == 0 || max_n_keys == 0 || n_kv_heads == 0 ||
+      n_heads == 0 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 8 ||
+      (head_dim != 64 && head_dim != 128))
+    return 0;
+  return kv4_attn_ws_bytes(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, head_dim, window,
+                           n_sinks);
+}
+
+int32_t flk_kv4_attn(const float* q, const void* pool, const uint32_t* table,
+                     const uint32_t* n_keys, const uint32_t* q_off, float* o, uint32_t n_seqs,
+                     uint32_t n_tokens, uint32_t max_q, uint32_t max_n_keys, uint32_t max_blocks,
+                     uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_pages,
+                     uint32_t page, uint32_t window, uint32_t n_sinks, void* ws,
+                     uint64_t ws_bytes) {
+  FLK_NONNULL(q);
+  FLK_WORDS(table);
+  FLK_WORDS(n_keys);
+  FLK_WORDS(q_off);
+  FLK_NONNULL(o);
+  FLK_ALIGNED(q);
+  FLK_ALIGNED(o);
+  if (int32_t rc = check_kv4(pool, n_heads, n_kv_heads, head_dim, n_pages, page)) return rc;
+  if (n_seqs == 0 || n_tokens == 0 || max_q == 0 || max_n_keys == 0 || max_blocks == 0)
+    return fail(FLK_ERR_ARG, "kv4_attn n_seqs=%u n_tokens=%u max_q=%u max_n_keys=%u max_blocks=%u",
+                n_seqs, n_tokens, max_q, max_n_keys, max_blocks);
+  if (n_seqs > 65535) return fail(FLK_ERR_UNSUPPORTED, "kv4_attn n_seqs %u exceeds 65535", n_seqs);
+  if (max_n_keys > (uint64_t)max_blocks * page)
+    return fail(FLK_ERR_ARG, "kv4_attn: %u keys do not fit %u blocks of %u tokens", max_n_keys,
+                max_blocks, page);
+  const uint64_t bytes = 4ull * n_tokens * n_heads * head_dim;
+  if (q != o && overlap(q, bytes, o, bytes))
+    return fail(FLK_ERR_ARG, "kv4_attn: o lies partly over q");
+  const uint64_t need = kv4_attn_ws_bytes(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, head_dim,
+                                          window, n_sinks);
+  if (int32_t rc = check_ws(ws, ws_bytes, need)) return rc;
+  Kv4AttnArgs a{};
+  a.q = q;
+  a.pool = static_cast<const uint8_t*>(pool);
+  a.table = table, a.n_keys = n_keys, a.q_off = q_off;
+  a.o = o;
+  a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.max_q = max_q, a.max_n_keys = max_n_keys;
+  a.max_blocks = max_blocks, a.n_heads = n_heads, a.window = window, a.n_sinks = n_sinks;
+  a.s = Kv4Shape{n_kv_heads, head_dim, n_pages, page};
+  return hip_status(launch_kv4_attn(a, ws, g_stream), "flk_kv4_attn");
 }

@@ -54,6 +54,23 @@ export const hip = Deno.dlopen(Deno.env.get("FLOCK_ATTN_LIB") ?? "libflock_attn.
     parameters: [P, P, P, P, P, P, F32, I32, P, P, P, P, P, P, U32, U32, U32, U32, U32, P, U64],
     result: I32,
   },
+  flk_kv4_page_bytes: { parameters: [U32, U32, U32], result: U64 },
+  flk_kv4_plan_ws_bytes: { parameters: [U32], result: U64 },
+  flk_kv4_plan: {
+    parameters: [P, P, P, P, P, P, P, P, P, P, U32, U32, U32, U32, U32, U32, U32, P, U64],
+    result: I32,
+  },
+  flk_kv4_prologue: {
+    parameters: [P, P, P, U32, P, P, P, F32, I32, P, P, P, P, U32, U32, U32, U32, U32, U32],
+    result: I32,
+  },
+  flk_kv4_append: { parameters: [P, P, P, P, U32, U32, U32, U32, U32], result: I32 },
+  flk_kv4_read: { parameters: [P, P, P, P, U32, U32, U32, U32, U32], result: I32 },
+  flk_kv4_attn_ws_bytes: { parameters: [U32, U32, U32, U32, U32, U32, U32, U32], result: U64 },
+  flk_kv4_attn: {
+    parameters: [P, P, P, P, P, P, U32, U32, U32, U32, U32, U32, U32, U32, U32, U32, U32, U32, P, U64],
+    result: I32,
+  },
   // include/flock_q8.h
   flk_q8_matvec: { parameters: [P, P, P, P, U32, U32, U32], result: I32 },
   flk_q8_split: { parameters: ["buffer", U32, U32, "buffer", "buffer"], result: I32 },

@@ -277,6 +277,71 @@ def decode_layer_ragged(q_raw, k_raw, v_raw, gq, gk, inv_freq, eps: float, pairi
                                         head_dim, w, nb), "flk_decode_layer_ragged")
 
 
+# ------------------------------------------------------ paged cache in 4 bits
+def kv4_page_bytes(n_kv_heads: int, head_dim: int, page: int) -> int:
+    """Bytes of a page of ``page`` tokens of a 4-bit pool."""
+    n = int(lib().flk_kv4_page_bytes(n_kv_heads, head_dim, page))
+    if n == 0:
+        raise FlockError(-1, "invalid shape for flk_kv4_page_bytes")
+    return n
+
+
+def kv4_plan_ws_bytes(n_seqs: int) -> int:
+    return int(lib().flk_kv4_plan_ws_bytes(n_seqs))
+
+
+def kv4_plan(n_keys, n_new, table_in, table_out, free_in, free_out, q_off, positions, slots, lost,
+             n_seqs: int, max_blocks: int, n_pages: int, max_tokens: int, page: int, window: int,
+             n_sinks: int, ws) -> None:
+    """Block table, free list, row offsets, positions and slots of a step, from
+    the lengths after it and the new tokens of each sequence (flk_kv4_plan)."""
+    w, nb = _ws(ws)
+    check(lib().flk_kv4_plan(ptr(n_keys), ptr(n_new), ptr(table_in), ptr(table_out), ptr(free_in),
+                             ptr(free_out), ptr(q_off), ptr(positions), ptr(slots), ptr(lost),
+                             n_seqs, max_blocks, n_pages, max_tokens, page, window, n_sinks, w,
+                             nb), "flk_kv4_plan")
+
+
+def kv4_prologue(q_raw, k_raw, v_raw, gq, gk, inv_freq, eps: float, pairing, positions, slots,
+                 qn_out, pool, n_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                 n_pages: int, page: int, in_stride: int = 0) -> None:
+    """qk_prologue with positions[t] and the pool's slots[t] for token t."""
+    check(lib().flk_kv4_prologue(ptr(q_raw), ptr(k_raw), ptr(v_raw), in_stride, ptr(gq), ptr(gk),
+                                 ptr(inv_freq), eps, _pairing(pairing), ptr(positions), ptr(slots),
+                                 ptr(qn_out), ptr(pool), n_tokens, n_heads, n_kv_heads, head_dim,
+                                 n_pages, page), "flk_kv4_prologue")
+
+
+def kv4_append(kn, v, slots, pool, n_tokens: int, n_kv_heads: int, head_dim: int, n_pages: int,
+               page: int) -> None:
+    check(lib().flk_kv4_append(ptr(kn), ptr(v), ptr(slots), ptr(pool), n_tokens, n_kv_heads,
+                               head_dim, n_pages, page), "flk_kv4_append")
+
+
+def kv4_read(pool, slots, k, v, n_tokens: int, n_kv_heads: int, head_dim: int, n_pages: int,
+             page: int) -> None:
+    """The pool's values at slots[t] as f32 rows."""
+    check(lib().flk_kv4_read(ptr(pool), ptr(slots), ptr(k), ptr(v), n_tokens, n_kv_heads,
+                             head_dim, n_pages, page), "flk_kv4_read")
+
+
+def kv4_attn_ws_bytes(n_seqs: int, max_q: int, max_n_keys: int, n_heads: int, n_kv_heads: int,
+                      head_dim: int, window: int = 0, n_sinks: int = 0) -> int:
+    return int(lib().flk_kv4_attn_ws_bytes(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads,
+                                           head_dim, window, n_sinks))
+
+
+def kv4_attn(q, pool, table, n_keys, q_off, o, n_seqs: int, n_tokens: int, max_q: int,
+             max_n_keys: int, max_blocks: int, n_heads: int, n_kv_heads: int, head_dim: int,
+             n_pages: int, page: int, window: int, n_sinks: int, ws) -> None:
+    """Attention of rows q_off[b] .. of q over sequence b's keys in the pool
+    (flk_kv4_attn): its last row is at position n_keys[b] - 1."""
+    w, nb = _ws(ws)
+    check(lib().flk_kv4_attn(ptr(q), ptr(pool), ptr(table), ptr(n_keys), ptr(q_off), ptr(o),
+                             n_seqs, n_tokens, max_q, max_n_keys, max_blocks, n_heads, n_kv_heads,
+                             head_dim, n_pages, page, window, n_sinks, w, nb), "flk_kv4_attn")
+
+
 # ------------------------------------------------------------ Q8_0 projections
 def q8_split(packed, n_rows: int, n_cols: int):
     """splitQ8 (kernels/lib.ts:141-156) on the host: GGUF Q8_0 bytes -> (qs int8, scales f16 bits)."""

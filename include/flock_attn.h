@@ -252,6 +252,116 @@ int32_t flk_decode_layer_ragged(const float* q_raw, const float* k_raw, const fl
                                 uint32_t max_n_keys, uint32_t n_heads, uint32_t n_kv_heads,
                                 uint32_t head_dim, void* ws, uint64_t ws_bytes);
 
+/* ------------------------------------------------- paged cache in 4 bits -- */
+
+/* Extension, no reference counterpart (the reference keeps one contiguous f32
+ * cache per Layer, layer.ts:394-397): a batch's keys and values in 4 bits, in
+ * pages that sequences take from a common pool. One step of a layer is
+ *
+ *   flk_kv4_plan      (once per step, for all layers: tables, positions, slots)
+ *   flk_kv4_prologue  (q/k norm + RoPE, k and v into the pool)
+ *   flk_kv4_attn      (attention of the step's queries over the pool)
+ *
+ * all of them from DEVICE arrays of lengths, so that a step can be captured into
+ * a graph and replayed.
+ *
+ *   pool       n_pages * flk_kv4_page_bytes bytes, 16-byte aligned; needs no
+ *              initialisation. `page`, the tokens of a page, is 32, 64, 128 or
+ *              256; n_pages * page must be below 2^32. Pages hold every kv head.
+ *   slot       of a token: page id * page + its place in the page; a value of
+ *              n_pages * page or more (0xffffffff) means none
+ *   table      [n_seqs][max_blocks] page ids: entry i holds the sequence's
+ *              tokens i * page .. i * page + page - 1; n_pages or more
+ *              (0xffffffff): no page
+ *   n_keys[b]  keys of sequence b AFTER the step (as flk_decode_layer_ragged)
+ *   q_off      [n_seqs + 1]: sequence b's new tokens are rows q_off[b] ..
+ *              q_off[b + 1] - 1 of q and o, its last ones: the row before
+ *              q_off[b + 1] is at position n_keys[b] - 1
+ *   window     0: a token sees every key up to its own. w > 0: it sees the last w
+ *              keys (its own among them) and the sequence's first n_sinks.
+ *
+ * Values are kept per 32 neighbouring dims as codes c (0 .. 15) and one scale d:
+ * with m the block's value of largest magnitude (the positive one in a tie), d =
+ * m / -8 rounded to bf16 and that to f16, c = 8 + x * (1 / d) rounded to the
+ * nearest (half to even) and limited to 0 .. 15; the value is (c - 8) * d. Larger
+ * magnitudes than 65280 saturate; a block with an infinity or NaN is NaN as a
+ * whole. That is 0.5625 bytes a value. */
+
+/* Bytes of a page (0 for an unsupported shape). */
+uint64_t flk_kv4_page_bytes(uint32_t n_kv_heads, uint32_t head_dim, uint32_t page);
+
+/* Block tables and slot maps of a step from request lengths. Sequence b has
+ * n_keys[b] keys after the step, the last n_new[b] of them new (at most all).
+ * It holds block i after the step if i * page < n_keys[b] and, where window > 0,
+ * the block has a token that its first new token sees or n_sinks covers. Blocks to
+ * hold that table_in has no page for take one; pages of other blocks go back (all
+ * of them for n_keys[b] = 0: a finished sequence; those past the end after tokens
+ * were taken back; those that left the window).
+ *   free_in, free_out  [1 + n_pages]: a count, then that many free page ids. The
+ *     k-th block that takes a page, in order of (sequence, block), takes the k-th
+ *     from the end of free_in's list. free_out's list is what is left of it, then
+ *     the pages that went back, in the same order: they can be taken in the next
+ *     step. The two may not overlap (a caller keeps two and swaps them).
+ *   table_out  may be table_in. Entries without a page are 0xffffffff.
+ *   q_off      [n_seqs + 1] as above
+ *   positions, slots  [max_tokens], by row of q: the token's position, and its
+ *     slot. Entries behind the last token: position 0, no slot.
+ *   lost       [1]: new tokens without a slot: no page was free (a later call with
+ *     the same lengths takes what is free then), a position behind the table's
+ *     last block, or a row past max_tokens. 0 when all is well.
+ * ws: flk_kv4_plan_ws_bytes, 256-byte aligned. */
+uint64_t flk_kv4_plan_ws_bytes(uint32_t n_seqs);
+int32_t flk_kv4_plan(const uint32_t* n_keys, const uint32_t* n_new, const uint32_t* table_in,
+                     uint32_t* table_out, const uint32_t* free_in, uint32_t* free_out,
+                     uint32_t* q_off, uint32_t* positions, uint32_t* slots, uint32_t* lost,
+                     uint32_t n_seqs, uint32_t max_blocks, uint32_t n_pages,
+                     uint32_t max_tokens, uint32_t page, uint32_t window, uint32_t n_sinks,
+                     void* ws, uint64_t ws_bytes);
+
+/* flk_qk_prologue(_strided) onto the pool: q and k of token t normed and rotated
+ * at positions[t], q to qn_out, k (in 4 bits, from the same f32 values) and v to
+ * slots[t]. A token without a slot is not stored. No slot may come twice.
+ * in_stride as in flk_qk_prologue_strided. */
+int32_t flk_kv4_prologue(const float* q_raw, const float* k_raw, const float* v_raw,
+                         uint32_t in_stride, const float* gq, const float* gk,
+                         const float* inv_freq, float eps, int32_t pairing,
+                         const uint32_t* positions, const uint32_t* slots, float* qn_out,
+                         void* pool, uint32_t n_tokens, uint32_t n_heads, uint32_t n_kv_heads,
+                         uint32_t head_dim, uint32_t n_pages, uint32_t page);
+
+/* flk_kv_append onto the pool: rows kn, v [n_tokens][n_kv_heads][head_dim] in 4
+ * bits to slots[t]. */
+int32_t flk_kv4_append(const float* kn, const float* v, const uint32_t* slots, void* pool,
+                       uint32_t n_tokens, uint32_t n_kv_heads, uint32_t head_dim,
+                       uint32_t n_pages, uint32_t page);
+
+/* The values at slots[t] as rows k, v [n_tokens][n_kv_heads][head_dim] (16-byte
+ * aligned); zeros for a token without a slot. */
+int32_t flk_kv4_read(const void* pool, const uint32_t* slots, float* k, float* v,
+                     uint32_t n_tokens, uint32_t n_kv_heads, uint32_t head_dim,
+                     uint32_t n_pages, uint32_t page);
+
+/* Attention of each sequence's new tokens over its keys in the pool (the rows of
+ * this step must be there already). q, o: [n_tokens][n_heads][head_dim] f32; rows
+ * that no sequence has are left as they were. max_q bounds every q_off[b + 1] -
+ * q_off[b], max_n_keys every n_keys[b] (at most max_blocks * page): they set the
+ * launch shape, so near bounds are faster. A sequence beyond either is refused on
+ * the device, as is one whose visible keys lack a page: its o rows are NaN. A row
+ * that sees no key (n_keys[b] below its row count) is zeros. o may be q, but not
+ * lie partly over it. Sums are f32, q and the weights enter the matrix products in
+ * two f16 parts (22 bits), the cache's values as they are.
+ * ws: flk_kv4_attn_ws_bytes of the same arguments, 256-byte aligned; calls that
+ * share one must be ordered on one stream. */
+uint64_t flk_kv4_attn_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
+                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                               uint32_t window, uint32_t n_sinks);
+int32_t flk_kv4_attn(const float* q, const void* pool, const uint32_t* table,
+                     const uint32_t* n_keys, const uint32_t* q_off, float* o, uint32_t n_seqs,
+                     uint32_t n_tokens, uint32_t max_q, uint32_t max_n_keys,
+                     uint32_t max_blocks, uint32_t n_heads, uint32_t n_kv_heads,
+                     uint32_t head_dim, uint32_t n_pages, uint32_t page, uint32_t window,
+                     uint32_t n_sinks, void* ws, uint64_t ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,5 @@
 // Attention over the paged 4-bit cache: one wave per (query, head).
-#include "kv4.hpp"
+#include "kv4_attn.hpp"
 
 namespace flk {
 
@@ -83,12 +83,25 @@ __global__ __launch_bounds__(64) void kv4_attn_kernel(Kv4AttnArgs a, float scale
   for (int c = 0; c < D / 64; c++) a.o[row + 64 * c + lane] = l == 0.f ? 0.f : acc[c] / l;
 }
 
-uint64_t kv4_attn_ws_bytes(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t,
-                           uint32_t) {
+// Up to 16 query-head rows a kv head take the decode kernel.
+static bool few_rows(uint32_t max_q, uint32_t n_heads, uint32_t n_kv_heads) {
+  return (uint64_t)max_q * (n_heads / n_kv_heads) <= 16;
+}
+
+uint64_t kv4_attn_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys, uint32_t n_heads,
+                           uint32_t n_kv_heads, uint32_t head_dim, uint32_t window,
+                           uint32_t n_sinks) {
+  if (few_rows(max_q, n_heads, n_kv_heads))
+    return kv4_decode_plan(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, head_dim, window,
+                           n_sinks).ws_bytes;
   return 0;
 }
 
-hipError_t launch_kv4_attn(const Kv4AttnArgs& a, void*, hipStream_t st) {
+hipError_t launch_kv4_attn(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
+  if (few_rows(a.max_q, a.n_heads, a.s.n_kv_heads))
+    return launch_kv4_decode(a, kv4_decode_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads,
+                                                a.s.n_kv_heads, a.s.head_dim, a.window, a.n_sinks),
+                             ws, st);
   const float scale = (float)(1.0 / sqrt((double)a.s.head_dim));
   const dim3 grid(a.n_heads, a.max_q, a.n_seqs);
   if (a.s.head_dim == 128)

@@ -13,6 +13,13 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // 16 c, a bit position higher): no shift for the second, and no rounding anywhere.
 __device__ __forceinline__ halfx2 as_half2(uint32_t v) { return __builtin_bit_cast(halfx2, v); }
 __device__ __forceinline__ uint32_t as_u32(halfx2 v) { return __builtin_bit_cast(uint32_t, v); }
+// (w & mask) | bits in one instruction: its two constants do not both fit as literals,
+// so the compiler makes two of it unless they are held in registers.
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(bits));
+  return r;
+}
 template <int J>
 __device__ __forceinline__ halfx2 kv4_pair(uint32_t w, halfx2 d) {
   const uint32_t x = J >= 2 ? w >> 8 : w;
@@ -20,10 +27,10 @@ __device__ __forceinline__ halfx2 kv4_pair(uint32_t w, halfx2 d) {
   if constexpr (J & 1) {
     const halfx2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
     const halfx2 off = {(_Float16)-72.f, (_Float16)-72.f};
-    c = __builtin_elementwise_fma(as_half2((x & 0x00f000f0u) | 0x64006400u), sixteenth, off);
+    c = __builtin_elementwise_fma(as_half2(and_or(x, 0x00f000f0u, 0x64006400u)), sixteenth, off);
   } else {
     const halfx2 off = {(_Float16)-1032.f, (_Float16)-1032.f};
-    c = as_half2((x & 0x000f000fu) | 0x64006400u) + off;
+    c = as_half2(and_or(x, 0x000f000fu, 0x64006400u)) + off;
   }
   return c * d;
 }
@@ -37,6 +44,12 @@ __device__ __forceinline__ halfx2 pack_half2(float a, float b) {
   typedef float f2 __attribute__((ext_vector_type(2)));
   const f2 v = {a, b};
   return __builtin_convertvector(v, halfx2);
+}
+
+// The second f16 parts of two values whose first are hi: x - hi is exact in f32 (one
+// mixed-precision FMA each).
+__device__ __forceinline__ halfx2 rest_half2(float a, float b, halfx2 hi) {
+  return pack_half2(fmaf((float)hi[0], -1.f, a), fmaf((float)hi[1], -1.f, b));
 }
 
 // A power of two that brings a row's largest |q| to 2^14 .. 2^15, and its inverse:
@@ -69,6 +82,45 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, uint32_t b) {
   s.refused = s.n_keys > a.max_n_keys || s.nq > a.max_q;
   return s;
 }
+
+// Which keys of a tile the rows of a row tile see, in 32 bits: a key `off` into the
+// tile and a row `delta` positions behind the row tile's first.
+struct Kv4Mask {
+  int causal, window, sinks;
+  __device__ __forceinline__ bool sees(int off, int delta) const {
+    return causal + off <= delta && (window + off > delta || off < sinks);
+  }
+};
+__device__ __forceinline__ int clamp30(int64_t x) {
+  return (int)(x < -(1 << 30) ? -(1 << 30) : x > (1 << 30) ? 1 << 30 : x);
+}
+// The keys that a row tile at positions first .. last sees: its tiles, and which of
+// them every row sees whole.
+struct Kv4Span {
+  Kv4Tiles tiles;
+  int64_t first;
+  uint32_t window, n_sinks;
+  uint32_t before, from, sinks;  // whole: below `before`, and from `from` or below `sinks`
+  __device__ __forceinline__ Kv4Span(int64_t first_, int64_t last, uint32_t window_,
+                                     uint32_t n_sinks_)
+      : tiles(kv4_tiles(first_, last, window_, n_sinks_)),
+        first(first_),
+        window(window_),
+        n_sinks(n_sinks_) {
+    before = first < 0 ? 0u : (uint32_t)((first + 1) / kKv4Tile);
+    const int64_t w = last - (int64_t)window + kKv4Tile;  // ceil((last - window + 1) / 32)
+    from = window == 0 || w < 0 ? 0u : (uint32_t)(w / kKv4Tile);
+    sinks = n_sinks / kKv4Tile;
+  }
+  __device__ __forceinline__ bool whole(uint32_t tile) const {
+    return tile < before && (tile >= from || tile < sinks);
+  }
+  __device__ __forceinline__ Kv4Mask mask(uint32_t tile) const {
+    const int64_t key0 = (int64_t)tile * kKv4Tile;
+    return {clamp30(key0 - first), window == 0 ? 1 << 30 : clamp30(key0 - first + window),
+            clamp30((int64_t)n_sinks - key0)};
+  }
+};
 
 // Pieces that a row tile's key tiles are cut into: as few as leave none more than
 // `most` tiles, then as equal as they come.

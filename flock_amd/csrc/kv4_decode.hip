@@ -24,23 +24,36 @@ struct TileRegs {
   uint32_t ks;
 };
 
-__device__ __forceinline__ uint4 load16(const uint8_t* p) {
-  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-  const u4 v = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p));
-  return make_uint4(v[0], v[1], v[2], v[3]);
-}
-
+// Every load of a tile is relative to its first byte, which is uniform: buffer loads
+// take that in scalar registers and leave one 32-bit offset a lane for each part.
+constexpr int kBufferWord3 = 0x00020000;  // untyped
+constexpr int kNonTemporal = 2;
+struct TileOffsets {
+  int k, ks, v, vs;
+};
 template <int D>
-__device__ __forceinline__ void load_tile(TileRegs<D>& t, const uint8_t* base, int lane) {
+__device__ __forceinline__ TileOffsets tile_offsets(int lane) {
   const int n = lane & 15, kg = lane >> 4;
+  return {(n * 4 + kg) * 16,
+          Kv4<D>::kKScale + (n * Kv4<D>::kBlocks + (D == 128 ? kg : kg >> 1)) * 4, lane * 16,
+          (kg * Kv4<D>::kBlocks + n * (D / 16) / 32) * 16};
+}
+template <int D>
+__device__ __forceinline__ void load_tile(TileRegs<D>& t, const uint8_t* base,
+                                          const TileOffsets& at) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0,
+                                                      Kv4<D>::kTileBytes, kBufferWord3);
+  auto load16 = [&](int lane_at, int offset) {
+    const u4 v = __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane_at, offset, kNonTemporal);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  };
 #pragma unroll
-  for (int c = 0; c < D / 64; c++) {
-    t.k[c] = load16(base + c * 1024 + (n * 4 + kg) * 16);
-    t.v[c] = load16(base + Kv4<D>::kV + c * 1024 + (kg * 16 + n) * 16);
-  }
-  t.ks = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(
-      base + Kv4<D>::kKScale + (n * Kv4<D>::kBlocks + (D == 128 ? kg : kg >> 1)) * 4));
-  t.vs = load16(base + Kv4<D>::kVScale + (kg * Kv4<D>::kBlocks + n * (D / 16) / 32) * 16);
+  for (int c = 0; c < D / 64; c++) t.k[c] = load16(at.k + c * 1024, 0);
+  t.ks = __builtin_amdgcn_raw_buffer_load_b32(rsrc, at.ks, 0, kNonTemporal);
+  t.vs = load16(at.vs, Kv4<D>::kVScale);
+#pragma unroll
+  for (int c = 0; c < D / 64; c++) t.v[c] = load16(at.v, Kv4<D>::kV + c * 1024);
 }
 
 template <int D, int NT>
@@ -76,19 +89,19 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
   const uint32_t n_rows = min((uint32_t)kRows, rows - r0);
   const int64_t pos0 = (int64_t)seq.n_keys - seq.nq;
   const int64_t first = pos0 + r0 / group, last = pos0 + (r0 + n_rows - 1) / group;
-  const Kv4Tiles tiles = kv4_tiles(first, last, a.window, a.n_sinks);
-  const Kv4Pieces pc = kv4_pieces(tiles.count(), plan.most);
+  const Kv4Span span(first, last, a.window, a.n_sinks);
+  const Kv4Pieces pc = kv4_pieces(span.tiles.count(), plan.most);
   if (split >= pc.n) return;
-  const uint32_t t0 = split * pc.per, t1 = min(t0 + pc.per, tiles.count());
+  const uint32_t t0 = split * pc.per, t1 = min(t0 + pc.per, span.tiles.count());
 
   // q: column col of column tile nt is part col & 1 of row 8 nt + col / 2.
   Half8 q[NT][kSteps];
   float c_s[NT];
-  int64_t pos[NT];
+  int delta[NT];  // the row's position behind the first
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
     const uint32_t r = min(r0 + 8 * nt + (col >> 1), rows - 1);
-    pos[nt] = pos0 + r / group;
+    delta[nt] = (int)(r / group - r0 / group);
     const float4* src = reinterpret_cast<const float4*>(
         a.q + ((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D +
         kg * (D / 4));
@@ -109,7 +122,7 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
     for (int i = 0; i < D / 8; i++) {
       const float u = x[2 * i] * rs.up, v = x[2 * i + 1] * rs.up;
       const halfx2 hi = pack_half2(u, v);
-      const halfx2 lo = pack_half2(u - (float)hi[0], v - (float)hi[1]);
+      const halfx2 lo = rest_half2(u, v, hi);
       q[nt][i >> 2].u[i & 3] = as_u32(col & 1 ? lo : hi);
     }
   }
@@ -122,28 +135,22 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
   const uint32_t log_page = 31 - __builtin_clz(a.s.page);  // 5 .. 8
   const uint32_t* row = a.table + (size_t)b * a.max_blocks;
   const size_t tile_bytes = Kv4<D>::kTileBytes;
-  uint32_t ids = 0;  // lane i: the page of this wave's i-th tile from id_at
-  uint32_t id_at = 0;
   const uint32_t n_it = t0 + wave < t1 ? (t1 - t0 - wave + kDecWaves - 1) / kDecWaves : 0;
-  auto index = [&](uint32_t it) { return tiles.tile(t0 + wave + it * kDecWaves); };
-  auto fetch_ids = [&](uint32_t it) {
-    id_at = it;
-    ids = row[index(min(it + lane, n_it - 1)) >> (log_page - 5)];
+  auto index = [&](uint32_t it) { return span.tiles.tile(t0 + wave + it * kDecWaves); };
+  // Page ids come through the scalar cache: a vector load would have the wait for it
+  // also wait for the tiles in flight.
+  auto page_of = [&](uint32_t it) {
+    typedef const __attribute__((address_space(4))) uint32_t* ConstPtr;
+    return *(ConstPtr)(uintptr_t)(row + (index(it) >> (log_page - 5)));
   };
-  bool cur_bad = false, nxt_bad = false;
-  auto base_of = [&](uint32_t it, bool& bad) {
-    uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(it - id_at));
-    bad = id >= a.s.n_pages;
-    id = bad ? 0 : id;
+  auto base_of = [&](uint32_t it, uint32_t id) {
+    id = id >= a.s.n_pages ? 0 : id;
     const uint32_t in = index(it) & ((a.s.page >> 5) - 1);
     return a.pool + ((((size_t)id * G + kvh) << (log_page - 5)) + in) * tile_bytes;
   };
 
   auto work = [&](const TileRegs<D>& t, uint32_t it, bool bad) {
-    const uint32_t key0 = index(it) * kKv4Tile;
-    const bool whole = (int64_t)key0 + 31 <= first &&
-                       (a.window == 0 || (int64_t)key0 > last - (int64_t)a.window ||
-                        (uint64_t)key0 + 31 < a.n_sinks);
+    const bool whole = span.whole(index(it));
     // S^T of the two halves.
     const halfx2 ks = bad ? as_half2(0x7e007e00u) : as_half2(t.ks);
     const halfx2 d0 = {ks[0], ks[0]}, d1 = {ks[1], ks[1]};
@@ -177,10 +184,10 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
         x[i] += dpp<kDppXor1>(x[i]);
       }
       if (!whole) {
+        const Kv4Mask mask = span.mask(index(it));
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          const int64_t key = (int64_t)key0 + 16 * (i >> 2) + 4 * kg + (i & 3);
-          x[i] = kv4_sees(pos[nt], key, a.window, a.n_sinks) ? x[i] : -INFINITY;
+          x[i] = mask.sees(16 * (i >> 2) + 4 * kg + (i & 3), delta[nt]) ? x[i] : -INFINITY;
         }
       }
 #pragma unroll
@@ -205,7 +212,7 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const halfx2 hi = pack_half2(x[2 * i], x[2 * i + 1]);
-        const halfx2 lo = pack_half2(x[2 * i] - (float)hi[0], x[2 * i + 1] - (float)hi[1]);
+        const halfx2 lo = rest_half2(x[2 * i], x[2 * i + 1], hi);
         p[nt].u[i] = as_u32(col & 1 ? lo : hi);
       }
     }
@@ -224,6 +231,7 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
         any |= lo || hi;
       }
       if (__ballot(any)) {
+        const Kv4Mask mask = span.mask(index(it));
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
           Half8 sees;
@@ -233,8 +241,8 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
 #pragma unroll
             for (int j = 0; j < 2; j++) {
               const int u = 2 * i + j;
-              const int64_t key = (int64_t)key0 + 16 * (u >> 2) + 4 * kg + (u & 3);
-              if (kv4_sees(pos[nt], key, a.window, a.n_sinks)) sees.u[i] |= 0x3c00u << (16 * j);
+              if (mask.sees(16 * (u >> 2) + 4 * kg + (u & 3), delta[nt]))
+                sees.u[i] |= 0x3c00u << (16 * j);
             }
           }
           floatx4v count = {};
@@ -270,19 +278,19 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
 
   if (n_it > 0) {
     TileRegs<D> x, y;
-    fetch_ids(0);
-    load_tile<D>(x, base_of(0, cur_bad), lane);
+    const TileOffsets at = tile_offsets<D>(lane);
+    uint32_t id_x = page_of(0), id_y = page_of(min(1u, n_it - 1));
+    load_tile<D>(x, base_of(0, id_x), at);
     for (uint32_t it = 0; it < n_it; it += 2) {
       // Past the end the last tile is read once more (an L2 hit) and not used.
-      uint32_t nx = min(it + 1, n_it - 1);
-      if (nx - id_at >= 64) fetch_ids(nx);
-      load_tile<D>(y, base_of(nx, nxt_bad), lane);
-      work(x, it, cur_bad);
+      const uint32_t n1 = min(it + 1, n_it - 1), n2 = min(it + 2, n_it - 1);
+      load_tile<D>(y, base_of(n1, id_y), at);
+      const uint32_t id_2 = page_of(n2), id_3 = page_of(min(it + 3, n_it - 1));
+      work(x, it, id_x >= a.s.n_pages);
       if (it + 1 >= n_it) break;
-      nx = min(it + 2, n_it - 1);
-      if (nx - id_at >= 64) fetch_ids(nx);
-      load_tile<D>(x, base_of(nx, cur_bad), lane);
-      work(y, it + 1, nxt_bad);
+      load_tile<D>(x, base_of(n2, id_2), at);
+      work(y, it + 1, id_y >= a.s.n_pages);
+      id_x = id_2, id_y = id_3;
     }
   }
 
@@ -341,18 +349,18 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
   }
 }
 
-// Joins the pieces of a row: a wave per row, lanes over dims.
+// Joins the pieces of a row: a workgroup per row, D / 4 threads over its dims and the
+// pieces dealt out to the 1024 / D groups of them (a long context has a hundred).
 template <int D>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, Kv4SplitPlan plan,
                                                         Kv4Part part) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ float4 s_acc[kGroups][kLanes];
+  __shared__ float s_sum[kGroups];
   const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
   const int lane = threadIdx.x & 63;
-  const uint64_t id = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const uint32_t r = (uint32_t)(id % plan.rows);
-  const uint64_t slot = id / plan.rows;
-  if (slot >= (uint64_t)a.n_seqs * plan.row_tiles * G) return;
-  const uint32_t kvh = (uint32_t)(slot % G), rt = (uint32_t)(slot / G % plan.row_tiles);
-  const uint32_t b = (uint32_t)(slot / G / plan.row_tiles);
+  const uint32_t r = blockIdx.x % plan.rows, slot = blockIdx.x / plan.rows;
+  const uint32_t kvh = slot % G, rt = slot / G % plan.row_tiles, b = slot / G / plan.row_tiles;
   const Kv4Seq seq = kv4_seq(a, b);
   const uint32_t rows = seq.nq * group, r0 = rt * plan.rows, rr = r0 + r;
   if (seq.refused || rr >= rows) return;
@@ -362,30 +370,43 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, Kv4SplitP
                                    a.n_sinks);
   const uint32_t n = kv4_pieces(tiles.count(), plan.most).n;
   if (n == 1) return;
-  const size_t at = slot * plan.splits * plan.rows + r;
+  const size_t at = (size_t)slot * plan.splits * plan.rows + r;
+  const float2* ml = reinterpret_cast<const float2*>(part.ml) + at;
   float top = -INFINITY;
-  for (uint32_t i = lane; i < n; i += 64) top = fmaxf(top, part.ml[2 * (at + (size_t)i * plan.rows)]);
+  for (uint32_t i = lane; i < n; i += 64) top = fmaxf(top, ml[(size_t)i * plan.rows].x);
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, shfl_xor(top, x));
-  float sum = 0.f, acc[D / 64] = {};
-  for (uint32_t i = 0; i < n; i++) {
-    const size_t p = at + (size_t)i * plan.rows;
-    const float m = part.ml[2 * p];
-    const float k = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
-    sum = fmaf(part.ml[2 * p + 1], k, sum);
-#pragma unroll
-    for (int c = 0; c < D / 64; c++) acc[c] = fmaf(part.acc[p * D + 64 * c + lane], k, acc[c]);
+  const uint32_t e = threadIdx.x % kLanes, g = threadIdx.x / kLanes;
+  float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 4
+  for (uint32_t i = g; i < n; i += kGroups) {
+    const float2 x = ml[(size_t)i * plan.rows];
+    const float4 y = reinterpret_cast<const float4*>(part.acc + (at + (size_t)i * plan.rows) * D)[e];
+    const float k = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.x - top);
+    sum = fmaf(x.y, k, sum);
+    f.x = fmaf(y.x, k, f.x), f.y = fmaf(y.y, k, f.y);
+    f.z = fmaf(y.z, k, f.z), f.w = fmaf(y.w, k, f.w);
+  }
+  s_acc[g][e] = f;
+  if (e == 0) s_sum[g] = sum;
+  __syncthreads();
+  if (g != 0) return;
+  for (int i = 1; i < kGroups; i++) {
+    const float4 y = s_acc[i][e];
+    f.x += y.x, f.y += y.y, f.z += y.z, f.w += y.w;
+    sum += s_sum[i];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  float* dst = a.o + ((size_t)(seq.q0 + rr / group) * a.n_heads + kvh * group + rr % group) * D;
-#pragma unroll
-  for (int c = 0; c < D / 64; c++) dst[64 * c + lane] = acc[c] * inv;
+  float4* dst = reinterpret_cast<float4*>(
+      a.o + ((size_t)(seq.q0 + rr / group) * a.n_heads + kvh * group + rr % group) * D);
+  dst[e] = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
 }
 
 // Key tiles of a piece: few enough that the pieces of the call's bounds fill the
 // 256 CUs with four workgroups each a few times over (sequences are shorter than
 // the bound), and two a wave at least.
-constexpr uint32_t kDecTarget = 4096, kDecFew = 2 * kDecWaves;
+constexpr uint32_t kDecTarget = 4096, kDecAlone = 1024, kDecFew = 2 * kDecWaves;
 
 Kv4SplitPlan kv4_decode_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
                              uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
@@ -397,7 +418,8 @@ Kv4SplitPlan kv4_decode_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_key
   p.row_tiles = (uint32_t)((rows + p.rows - 1) / p.rows);
   const uint32_t tiles = kv4_max_tiles(max_n_keys, (p.rows + group - 1) / group + 1, window, n_sinks);
   const uint64_t items = (uint64_t)n_seqs * n_kv_heads * p.row_tiles;
-  const uint64_t most = (items * tiles + kDecTarget - 1) / kDecTarget;
+  const uint32_t target = n_seqs == 1 ? kDecAlone : kDecTarget;
+  const uint64_t most = (items * tiles + target - 1) / target;
   p.most = (uint32_t)(most < kDecFew ? kDecFew : most > 0xffffffffu ? 0xffffffffu : most);
   p.splits = (tiles + p.most - 1) / p.most;
   p.ws_bytes = p.splits == 1 ? 0
@@ -409,7 +431,7 @@ Kv4SplitPlan kv4_decode_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_key
 template <int D>
 static hipError_t launch(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws, hipStream_t st) {
   const uint64_t items = (uint64_t)a.n_seqs * a.s.n_kv_heads * p.row_tiles;
-  if (items * p.splits > 0x7fffffffull || items * p.rows / 4 > 0x7fffffffull)
+  if (items * p.splits > 0x7fffffffull || items * p.rows > 0x7fffffffull)
     return hipErrorInvalidConfiguration;
   Kv4Part part{static_cast<float*>(ws), nullptr};
   part.acc = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) +
@@ -422,7 +444,7 @@ static hipError_t launch(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws, 
     hipLaunchKernelGGL((kv4_decode_kernel<D, 2>), grid, block, 0, st, a, p, part, scale);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
-  hipLaunchKernelGGL(kv4_merge_kernel<D>, dim3((uint32_t)((items * p.rows + 3) / 4)), dim3(256), 0,
+  hipLaunchKernelGGL(kv4_merge_kernel<D>, dim3((uint32_t)(items * p.rows)), dim3(256), 0,
                      st, a, p, part);
   return hipGetLastError();
 }

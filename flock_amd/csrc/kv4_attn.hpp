@@ -155,5 +155,24 @@ Kv4SplitPlan kv4_decode_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_key
                              uint32_t window, uint32_t n_sinks);
 hipError_t launch_kv4_decode(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws,
                              hipStream_t st);
+Kv4SplitPlan kv4_prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
+                              uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                              uint32_t window, uint32_t n_sinks);
+hipError_t launch_kv4_prefill(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws,
+                              hipStream_t st);
+
+// Partial results of pieces, in the workspace: row r of piece s of row tile x is at
+// (x * splits + s) * rows + r.
+struct Kv4Part {
+  float* ml;   // pairs (reference, sum)
+  float* acc;  // D floats
+};
+inline Kv4Part kv4_part(void* ws, const Kv4SplitPlan& p, uint64_t items) {
+  return {static_cast<float*>(ws),
+          reinterpret_cast<float*>(static_cast<uint8_t*>(ws) +
+                                   ws_align(items * p.splits * p.rows * 8))};
+}
+hipError_t launch_kv4_merge(const Kv4AttnArgs& a, const Kv4SplitPlan& p, const Kv4Part& part,
+                            hipStream_t st);
 
 }  // namespace flk

@@ -13,11 +13,6 @@ namespace flk {
 
 constexpr int kDecWaves = 4;
 
-struct Kv4Part {
-  float* ml;   // [slot][rows] pairs (m, l)
-  float* acc;  // [slot][rows][D]
-};
-
 template <int D>
 struct TileRegs {
   uint4 k[D / 64], v[D / 64], vs;
@@ -433,9 +428,7 @@ static hipError_t launch(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws, 
   const uint64_t items = (uint64_t)a.n_seqs * a.s.n_kv_heads * p.row_tiles;
   if (items * p.splits > 0x7fffffffull || items * p.rows > 0x7fffffffull)
     return hipErrorInvalidConfiguration;
-  Kv4Part part{static_cast<float*>(ws), nullptr};
-  part.acc = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) +
-                                      ws_align(items * p.splits * p.rows * 8));
+  const Kv4Part part = kv4_part(ws, p, items);
   const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
   const dim3 grid((uint32_t)(items * p.splits)), block(kDecWaves * 64);
   if (p.rows == 8)
@@ -444,8 +437,16 @@ static hipError_t launch(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws, 
     hipLaunchKernelGGL((kv4_decode_kernel<D, 2>), grid, block, 0, st, a, p, part, scale);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
-  hipLaunchKernelGGL(kv4_merge_kernel<D>, dim3((uint32_t)(items * p.rows)), dim3(256), 0,
-                     st, a, p, part);
+  return launch_kv4_merge(a, p, part, st);
+}
+
+hipError_t launch_kv4_merge(const Kv4AttnArgs& a, const Kv4SplitPlan& p, const Kv4Part& part,
+                            hipStream_t st) {
+  const uint32_t rows = a.n_seqs * a.s.n_kv_heads * p.row_tiles * p.rows;
+  if (a.s.head_dim == 128)
+    hipLaunchKernelGGL(kv4_merge_kernel<128>, dim3(rows), dim3(256), 0, st, a, p, part);
+  else
+    hipLaunchKernelGGL(kv4_merge_kernel<64>, dim3(rows), dim3(256), 0, st, a, p, part);
   return hipGetLastError();
 }
 

@@ -1,0 +1,387 @@
+// Attention of many queries a sequence over the paged 4-bit cache (prompts, chunks).
+// MFMA-bound: f16 matrix products of the cache's exact values with q and the weights
+// in two f16 parts, twice the plain products' work.
+//
+// A work item is 128 query-head rows of one kv head and a piece of their key tiles; four
+// waves of 32 rows, two workgroups a CU. Every 64 keys the workgroup turns the two tiles'
+// codes to f16 in LDS (each code once for 128 rows), into the buffer that the step before
+// has read; the next tiles' codes are loaded meanwhile. S^T = K Q^T and O^T += V^T P^T on
+// 32x32x16: a column is a row of q, and P^T is taken from the S^T accumulators as they
+// lie, because V's keys are put in the order in which a lane holds its scores.
+#include "kv4_attn.hpp"
+
+namespace flk {
+
+typedef float floatx16v __attribute__((ext_vector_type(16)));
+
+constexpr int kPreRows = 128, kPreThreads = 256, kStep = 64;
+
+// 16-byte slots of K's rows (8 dims each) and of V's (8 keys of a dim), xored so that
+// neighbouring rows of one slot lie in distinct banks.
+template <int D>
+__device__ __forceinline__ int k_slot(int key, int slot) {
+  return key * (D / 8) + (slot ^ (D == 128 ? key & 15 : (key >> 1) & 7));
+}
+__device__ __forceinline__ int v_slot(int dim, int slot) {
+  return dim * (kStep / 8) + (slot ^ ((dim >> 1) & 7) ^ ((dim >> 4) & 7));
+}
+
+template <int D>
+struct PreShared {
+  uint4 k[2][kStep * D / 8];
+  uint4 v[2][kStep * D / 8];
+  // Slots (keys) of a tile whose V scale is no number, by [block][g]; the scale counts
+  // as 0 in LDS and the rows that see such a key get their NaN here.
+  uint32_t flag[2][2][4];
+};
+
+// One thread's share of two tiles, as it lies in the pool.
+struct PreRegs {
+  uint4 k, v, vs;
+  uint32_t ks;
+};
+
+template <int D>
+__global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
+    Kv4AttnArgs a, Kv4SplitPlan plan, Kv4Part part, float scale_log2e) {
+  constexpr int kSteps = D / 16, kOT = D / 32;
+  __shared__ PreShared<D> sh;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
+  uint32_t id = blockIdx.x;
+  const uint32_t kvh = id % G;
+  id /= G;
+  const uint32_t b = id % a.n_seqs;
+  id /= a.n_seqs;
+  const uint32_t split = id % plan.splits, rt = plan.row_tiles - 1 - id / plan.splits;
+
+  const Kv4Seq seq = kv4_seq(a, b);
+  const uint32_t rows = seq.nq * group;
+  if (seq.refused) {
+    if (rt == 0 && split == 0)
+      for (uint64_t i = threadIdx.x; i < (uint64_t)rows * D; i += kPreThreads) {
+        const uint32_t r = (uint32_t)(i / D);
+        a.o[((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D + i % D] =
+            __builtin_nanf("");
+      }
+    return;
+  }
+  const uint32_t r0 = rt * kPreRows;
+  if (r0 >= rows) return;
+  const uint32_t n_rows = min((uint32_t)kPreRows, rows - r0);
+  const int64_t pos0 = (int64_t)seq.n_keys - seq.nq;
+  const Kv4Tiles tiles = kv4_tiles(pos0 + r0 / group, pos0 + (r0 + n_rows - 1) / group, a.window,
+                                   a.n_sinks);
+  const Kv4Pieces pc = kv4_pieces(tiles.count(), plan.most);
+  if (split >= pc.n) return;
+  const uint32_t t0 = split * pc.per, t1 = min(t0 + pc.per, tiles.count());
+  const uint32_t n_steps = (t1 - t0 + 1) / 2;
+
+  // This wave's rows.
+  const uint32_t w0 = r0 + wave * 32;
+  const bool idle = w0 >= rows;
+  const uint32_t wl = min(w0 + 31, rows - 1);
+  const int64_t first = pos0 + min(w0, rows - 1) / group, last = pos0 + wl / group;
+  const Kv4Span span(first, last, a.window, a.n_sinks);
+  const uint32_t my = min(w0 + col, rows - 1);  // lanes behind the last row repeat it
+  const int delta = (int)(my / group - min(w0, rows - 1) / group);
+  const size_t my_at =
+      ((size_t)(seq.q0 + my / group) * a.n_heads + kvh * group + my % group) * D;
+
+  // Two parts of q: dims 16 s + 8 h ..
+  Half8 qh[kSteps], ql[kSteps];
+  float c_s;
+  {
+    float x[D / 2], amax = 0.f;
+#pragma unroll
+    for (int s = 0; s < kSteps; s++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const float4 f = *reinterpret_cast<const float4*>(a.q + my_at + 16 * s + 8 * h + 4 * i);
+        x[8 * s + 4 * i] = f.x, x[8 * s + 4 * i + 1] = f.y;
+        x[8 * s + 4 * i + 2] = f.z, x[8 * s + 4 * i + 3] = f.w;
+      }
+#pragma unroll
+    for (int i = 0; i < D / 2; i++) amax = fmaxf(amax, fabsf(x[i]));
+    amax = max_xor<32>(amax);
+    const RowScale rs = row_scale(amax);
+    c_s = rs.down * scale_log2e;
+#pragma unroll
+    for (int i = 0; i < D / 4; i++) {
+      const float u = x[2 * i] * rs.up, v = x[2 * i + 1] * rs.up;
+      const halfx2 hi = pack_half2(u, v);
+      qh[i >> 2].u[i & 3] = as_u32(hi);
+      ql[i >> 2].u[i & 3] = as_u32(rest_half2(u, v, hi));
+    }
+  }
+
+  // Staging: a thread takes a 16-byte piece of K and one of V of tile `half` of the step
+  // (D = 128), or a piece of K or of V (D = 64).
+  const uint32_t log_page = 31 - __builtin_clz(a.s.page);
+  const uint32_t* row = a.table + (size_t)b * a.max_blocks;
+  const int st_tile = D == 128 ? wave >> 1 : wave & 1;
+  const int piece = D == 128 ? (int)(threadIdx.x & 127) : lane;
+  const bool st_k = D == 128 || wave < 2, st_v = D == 128 || wave >= 2;
+  auto tile_of = [&](uint32_t i) { return tiles.tile(min(t0 + i, t1 - 1)); };
+  auto page_of = [&](uint32_t i) {
+    typedef const __attribute__((address_space(4))) uint32_t* ConstPtr;
+    return *(ConstPtr)(uintptr_t)(row + (tile_of(i) >> (log_page - 5)));
+  };
+  PreRegs rg;
+  const int v_n = piece & 15, v_g = (piece >> 4) & 3, v_c = piece >> 6;
+  const int v_block = v_n * (D / 16) / 32;
+  const int ks_at = Kv4<D>::kKScale +
+                    4 * (D == 128 ? piece & 63 : (piece >> 2) * 2 + ((piece >> 1) & 1));
+  auto fetch = [&](uint32_t step, uint32_t page_id) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const bool bad = page_id >= a.s.n_pages;
+    const uint32_t in = tile_of(2 * step + st_tile) & ((a.s.page >> 5) - 1);
+    const uint8_t* base =
+        a.pool + ((((size_t)(bad ? 0 : page_id) * G + kvh) << (log_page - 5)) + in) *
+                     (size_t)Kv4<D>::kTileBytes;
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0,
+                                                        Kv4<D>::kTileBytes, 0x00020000);
+    if (st_k) {
+      const u4 k = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece * 16, 0, 0);
+      rg.k = make_uint4(k[0], k[1], k[2], k[3]);
+      rg.ks = __builtin_amdgcn_raw_buffer_load_b32(rsrc, ks_at, 0, 0);
+      if (bad) rg.ks = 0x7e007e00u;
+    }
+    if (st_v) {
+      const u4 v = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece * 16, Kv4<D>::kV, 0);
+      const u4 s = __builtin_amdgcn_raw_buffer_load_b128(
+          rsrc, (v_g * Kv4<D>::kBlocks + v_block) * 16, Kv4<D>::kVScale, 0);
+      rg.v = make_uint4(v[0], v[1], v[2], v[3]);
+      rg.vs = make_uint4(s[0], s[1], s[2], s[3]);
+    }
+  };
+  auto stage = [&](int buf) {
+    if (st_k) {
+      const uint32_t w[4] = {rg.k.x, rg.k.y, rg.k.z, rg.k.w};
+      const halfx2 ks = as_half2(rg.ks);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        // D = 128: piece [half][key][part], octet i of the part. D = 64: [key][part] with
+        // two octets of each half.
+        const int half = D == 128 ? piece >> 6 : i >> 1;
+        const int key = D == 128 ? (piece >> 2) & 15 : piece >> 2;
+        const int slot = D == 128 ? 4 * (piece & 3) + i : 2 * (piece & 3) + (i & 1);
+        const _Float16 d1 = half ? ks[1] : ks[0];
+        const halfx2 d = {d1, d1};
+        uint4 x;
+        x.x = as_u32(kv4_pair<0>(w[i], d)), x.y = as_u32(kv4_pair<1>(w[i], d));
+        x.z = as_u32(kv4_pair<2>(w[i], d)), x.w = as_u32(kv4_pair<3>(w[i], d));
+        sh.k[buf][k_slot<D>(32 * st_tile + 16 * half + key, slot)] = x;
+      }
+    }
+    if (st_v) {
+      uint32_t s[4] = {rg.vs.x, rg.vs.y, rg.vs.z, rg.vs.w};
+      const uint32_t w[4] = {rg.v.x, rg.v.y, rg.v.z, rg.v.w};
+      uint32_t odd = 0, mask = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) odd |= (s[i] & 0x7c007c00u) + 0x04000400u;
+      if (odd & 0x80008000u) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const bool lo = (s[i] & 0x7c00u) == 0x7c00u, hi = (s[i] & 0x7c000000u) == 0x7c000000u;
+          s[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+          mask |= (lo ? 1u : 0u) << (2 * i) | (hi ? 2u : 0u) << (2 * i);
+        }
+      }
+      if (v_c == 0 && v_n % (512 / D) == 0)
+        reinterpret_cast<uint8_t*>(sh.flag[buf][st_tile])[v_block * 4 + v_g] = (uint8_t)mask;
+      // Slots 0 .. 3 are keys 4 g .., slots 4 .. 7 keys 16 + 4 g ..: of a 16-key step, lane
+      // half g & 1 holds the scores of keys 4 (g & 1) .. (first) and 8 + 4 (g & 1) ..
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int dim = (D / 16) * v_n + 4 * v_c + j;
+        uint32_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const halfx2 d = as_half2(s[i]);
+          x[i] = as_u32(j == 0   ? kv4_pair<0>(w[i], d)
+                        : j == 1 ? kv4_pair<1>(w[i], d)
+                        : j == 2 ? kv4_pair<2>(w[i], d)
+                                 : kv4_pair<3>(w[i], d));
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+          uint2* dst = reinterpret_cast<uint2*>(
+              &sh.v[buf][v_slot(dim, 4 * st_tile + 2 * ks + (v_g & 1))]);
+          dst[v_g >> 1] = make_uint2(x[2 * ks], x[2 * ks + 1]);
+        }
+      }
+    }
+  };
+
+  floatx16v o[kOT] = {};
+  float m = -INFINITY, l = 0.f;
+
+  auto block = [&](int buf, int t2, uint32_t tile) {
+    const bool whole = span.whole(tile);
+    floatx16v s = {};
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+      const halfx8 k =
+          __builtin_bit_cast(halfx8, sh.k[buf][k_slot<D>(32 * t2 + col, 2 * i + h)]);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[i].h, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i].h, s, 0, 0, 0);
+    }
+    Kv4Mask mask{};
+    if (!whole) {
+      mask = span.mask(tile);
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        s[i] = mask.sees(8 * (i >> 2) + 4 * h + (i & 3), delta) ? s[i] : -INFINITY;
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+    top *= c_s;
+    if (__ballot(top > m + kSlack)) {
+      top = max_xor<32>(top);
+      const float nm = fmaxf(m, top);
+      const float alpha = nm == m ? 1.f : __builtin_amdgcn_exp2f(m - nm);
+      m = nm;
+      l *= alpha;
+#pragma unroll
+      for (int c = 0; c < kOT; c++) o[c] *= alpha;
+    }
+    const float mb = (m == -INFINITY ? 0.f : m) - kBias;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c_s, -mb));
+      l += s[i];
+    }
+    Half8 ph[2], pl[2];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const halfx2 hi = pack_half2(s[2 * i], s[2 * i + 1]);
+      ph[i >> 2].u[i & 3] = as_u32(hi);
+      pl[i >> 2].u[i & 3] = as_u32(rest_half2(s[2 * i], s[2 * i + 1], hi));
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+      for (int c = 0; c < kOT; c++) {
+        const halfx8 v =
+            __builtin_bit_cast(halfx8, sh.v[buf][v_slot(32 * c + col, 4 * t2 + 2 * ks + h)]);
+        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[ks].h, o[c], 0, 0, 0);
+        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[ks].h, o[c], 0, 0, 0);
+      }
+    const uint32_t* flag = sh.flag[buf][t2];
+    uint32_t any = 0;
+#pragma unroll
+    for (int c = 0; c < kOT; c++) any |= flag[c];
+    if (__builtin_amdgcn_readfirstlane(any)) {
+      for (int c = 0; c < kOT; c++) {
+        bool hit = false;
+        for (int key = 0; key < 32; key++) {
+          const uint32_t bits = flag[c] >> (8 * ((key >> 2) & 3));
+          hit |= (bits >> ((key & 3) + 4 * (key >> 4)) & 1) && (whole || mask.sees(key, delta));
+        }
+#pragma unroll
+        for (int cc = 0; cc < kOT; cc++)
+          if (cc == c && hit) o[cc] = __builtin_nanf("");
+      }
+    }
+  };
+
+  if (n_steps > 0) {
+    uint32_t id_n = page_of(st_tile);
+    fetch(0, id_n);
+    id_n = page_of(2 + st_tile);
+    stage(0);
+    fetch(1, id_n);  // past the end: the last tile again
+    __syncthreads();
+    for (uint32_t st = 0; st < n_steps; st++) {
+      const int buf = st & 1;
+      id_n = page_of(2 * (st + 2) + st_tile);
+      if (st + 1 < n_steps) {
+        stage(buf ^ 1);
+        fetch(st + 2, id_n);
+      }
+      if (!idle) {
+#pragma unroll
+        for (int t2 = 0; t2 < 2; t2++) {
+          if (t0 + 2 * st + t2 >= t1) break;
+          const uint32_t tile = tiles.tile(t0 + 2 * st + t2);
+          // Some row of the wave sees some key: not past its last, not between its first
+          // tokens and its window.
+          if (tile >= span.tiles.to || (tile >= span.tiles.sinks && tile < span.tiles.from))
+            continue;
+          block(buf, t2, tile);
+        }
+      }
+      __syncthreads();
+    }
+  }
+  if (idle || w0 + col >= rows) return;
+  float lo, hi;
+  swap_pair<32>(l, lo, hi);
+  l = lo + hi;
+  const size_t slot = ((size_t)b * plan.row_tiles + rt) * G + kvh;
+  const size_t at = (slot * plan.splits + split) * kPreRows + wave * 32 + col;
+  float* dst = pc.n == 1 ? a.o + my_at : part.acc + at * D;
+  const float inv = pc.n > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+  if (pc.n > 1 && h == 0) part.ml[2 * at] = m, part.ml[2 * at + 1] = l;
+#pragma unroll
+  for (int c = 0; c < kOT; c++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      *reinterpret_cast<float4*>(dst + 32 * c + 8 * i + 4 * h) =
+          make_float4(o[c][4 * i] * inv, o[c][4 * i + 1] * inv, o[c][4 * i + 2] * inv,
+                      o[c][4 * i + 3] * inv);
+}
+
+// Pieces: the call's work (from its bounds, causal) over two workgroups a CU, a few
+// pieces each, none below eight tiles; long prompts of many row tiles need no cuts, as
+// the heaviest row tiles come first.
+constexpr uint32_t kPreTarget = 1024, kPreFew = 8, kPreWhole = 512;
+
+Kv4SplitPlan kv4_prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
+                              uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                              uint32_t window, uint32_t n_sinks) {
+  Kv4SplitPlan p;
+  const uint32_t group = n_heads / n_kv_heads;
+  p.rows = kPreRows;
+  p.row_tiles = (uint32_t)(((uint64_t)max_q * group + kPreRows - 1) / kPreRows);
+  const uint32_t tiles = kv4_max_tiles(max_n_keys, kPreRows / group + 2, window, n_sinks);
+  const uint64_t items = (uint64_t)n_seqs * n_kv_heads * p.row_tiles;
+  // The tiles of the mean row tile.
+  const uint32_t q = max_q < max_n_keys ? max_q : max_n_keys;
+  const uint64_t mean = kv4_max_tiles(max_n_keys - q / 2, kPreRows / group + 2, window, n_sinks);
+  uint64_t most = (items * mean + kPreTarget - 1) / kPreTarget;
+  most = (most + 1) / 2 * 2;
+  if (most < kPreFew) most = kPreFew;
+  if (items >= kPreWhole) most = tiles;
+  p.most = (uint32_t)(most > 0xfffffffeu ? 0xfffffffeu : most);
+  p.splits = (uint32_t)(((uint64_t)tiles + p.most - 1) / p.most);
+  p.ws_bytes = p.splits == 1 ? 0
+                             : ws_align(items * p.splits * p.rows * 8) +
+                                   ws_align(items * p.splits * p.rows * head_dim * 4);
+  return p;
+}
+
+template <int D>
+static hipError_t launch(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws, hipStream_t st) {
+  const uint64_t items = (uint64_t)a.n_seqs * a.s.n_kv_heads * p.row_tiles;
+  if (items * p.splits > 0x7fffffffull || items * p.rows > 0x7fffffffull)
+    return hipErrorInvalidConfiguration;
+  const Kv4Part part = kv4_part(ws, p, items);
+  const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
+  hipLaunchKernelGGL(kv4_prefill_kernel<D>, dim3((uint32_t)(items * p.splits)), dim3(kPreThreads),
+                     0, st, a, p, part, scale);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return e;
+  return launch_kv4_merge(a, p, part, st);
+}
+
+hipError_t launch_kv4_prefill(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws,
+                              hipStream_t st) {
+  return a.s.head_dim == 128 ? launch<128>(a, p, ws, st) : launch<64>(a, p, ws, st);
+}
+
+}  // namespace flk

@@ -46,10 +46,23 @@ __device__ __forceinline__ halfx2 pack_half2(float a, float b) {
   return __builtin_convertvector(v, halfx2);
 }
 
-// The second f16 parts of two values whose first are hi: x - hi is exact in f32 (one
-// mixed-precision FMA each).
-__device__ __forceinline__ halfx2 rest_half2(float a, float b, halfx2 hi) {
-  return pack_half2(fmaf((float)hi[0], -1.f, a), fmaf((float)hi[1], -1.f, b));
+// x + s * (one half of a pair of f16), in one instruction.
+template <int HI>
+__device__ __forceinline__ float mix_fma(halfx2 h, float s, float x) {
+  float r;
+  if constexpr (HI)
+    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(r) : "v"(h), "v"(s), "v"(x));
+  else
+    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(s), "v"(x));
+  return r;
+}
+
+// The second f16 parts of two values whose first are hi (x - hi is exact in f32). With
+// s = 0 in place of -1 the first parts again: a lane that holds one of the two picks it
+// by s.
+__device__ __forceinline__ halfx2 rest_half2(float a, float b, halfx2 hi, float s = -1.f) {
+  return pack_half2(mix_fma<0>(hi, s, a), mix_fma<1>(hi, s, b));
 }
 
 // A power of two that brings a row's largest |q| to 2^14 .. 2^15, and its inverse:
@@ -122,16 +135,6 @@ struct Kv4Span {
   }
 };
 
-// Pieces that a row tile's key tiles are cut into: as few as leave none more than
-// `most` tiles, then as equal as they come.
-struct Kv4Pieces {
-  uint32_t n, per;
-};
-__device__ __forceinline__ Kv4Pieces kv4_pieces(uint32_t tiles, uint32_t most) {
-  const uint32_t n = max(1u, (tiles + most - 1) / most);
-  return {n, (tiles + n - 1) / n};
-}
-
 // Key tiles that a row tile of `queries` queries may have, from the call's bounds.
 inline uint32_t kv4_max_tiles(uint32_t max_n_keys, uint32_t queries, uint32_t window,
                               uint32_t n_sinks) {
@@ -142,37 +145,58 @@ inline uint32_t kv4_max_tiles(uint32_t max_n_keys, uint32_t queries, uint32_t wi
   return (uint32_t)(seen < all ? seen : all);
 }
 
-// The two kernels' plans, from the call's bounds alone (lengths are on the device).
-struct Kv4SplitPlan {
-  uint32_t rows;       // query-head rows of a row tile
-  uint32_t row_tiles;  // row tiles of a (sequence, kv head)
-  uint32_t most;       // key tiles of a piece, at most
-  uint32_t splits;     // pieces that a row tile may have
-  uint64_t ws_bytes;
-};
-Kv4SplitPlan kv4_decode_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
-                             uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
-                             uint32_t window, uint32_t n_sinks);
-hipError_t launch_kv4_decode(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws,
-                             hipStream_t st);
-Kv4SplitPlan kv4_prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
-                              uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
-                              uint32_t window, uint32_t n_sinks);
-hipError_t launch_kv4_prefill(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws,
-                              hipStream_t st);
-
-// Partial results of pieces, in the workspace: row r of piece s of row tile x is at
-// (x * splits + s) * rows + r.
+// Partial results: row r of slot x is at x * rows + r.
 struct Kv4Part {
   float* ml;   // pairs (reference, sum)
   float* acc;  // D floats
 };
-inline Kv4Part kv4_part(void* ws, const Kv4SplitPlan& p, uint64_t items) {
-  return {static_cast<float*>(ws),
-          reinterpret_cast<float*>(static_cast<uint8_t*>(ws) +
-                                   ws_align(items * p.splits * p.rows * 8))};
+
+// o of one row from n partial results, i-th at at(i): kThreads threads, D / 4 of them over
+// the row's dims and the pieces dealt out to the groups of them. A piece without a visible
+// key holds zeros (or NaN, which stay).
+template <int D, int kThreads, typename At>
+__device__ __forceinline__ void merge_pieces(const Kv4Part& part, uint32_t n, At at, float* dst) {
+  constexpr int kLanes = D / 4, kGroups = kThreads / kLanes;
+  __shared__ float4 s_acc[kGroups][kLanes];
+  __shared__ float s_sum[kGroups];
+  const float2* ml = reinterpret_cast<const float2*>(part.ml);
+  const uint32_t lane = threadIdx.x & 63, e = threadIdx.x % kLanes, g = threadIdx.x / kLanes;
+  float top = -INFINITY;
+  for (uint32_t i = lane; i < n; i += 64) top = fmaxf(top, ml[at(i)].x);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, shfl_xor(top, x));
+  float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 4
+  for (uint32_t i = g; i < n; i += kGroups) {
+    const size_t p = at(i);
+    const float2 x = ml[p];
+    const float4 y = reinterpret_cast<const float4*>(part.acc + p * D)[e];
+    const float k = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.x - top);
+    sum = fmaf(x.y, k, sum);
+    f.x = fmaf(y.x, k, f.x), f.y = fmaf(y.y, k, f.y);
+    f.z = fmaf(y.z, k, f.z), f.w = fmaf(y.w, k, f.w);
+  }
+  s_acc[g][e] = f;
+  if (e == 0) s_sum[g] = sum;
+  __syncthreads();
+  if (g != 0) return;
+  for (int i = 1; i < kGroups; i++) {
+    const float4 y = s_acc[i][e];
+    f.x += y.x, f.y += y.y, f.z += y.z, f.w += y.w;
+    sum += s_sum[i];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  reinterpret_cast<float4*>(dst)[e] = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
 }
-hipError_t launch_kv4_merge(const Kv4AttnArgs& a, const Kv4SplitPlan& p, const Kv4Part& part,
-                            hipStream_t st);
+
+uint64_t kv4_decode_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
+                             uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                             uint32_t window, uint32_t n_sinks);
+hipError_t launch_kv4_decode(const Kv4AttnArgs& a, void* ws, hipStream_t st);
+uint64_t kv4_prefill_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
+                              uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                              uint32_t window, uint32_t n_sinks);
+hipError_t launch_kv4_prefill(const Kv4AttnArgs& a, void* ws, hipStream_t st);
 
 }  // namespace flk

@@ -7,6 +7,8 @@
 // ride in columns that the few rows would leave empty. The cache's layout gives each
 // lane its operands in 16-byte pieces, and P^T is taken from the S^T accumulators as
 // they lie (a lane's scores are of the tokens whose values it holds).
+#include <algorithm>
+
 #include "kv4_attn.hpp"
 
 namespace flk {
@@ -51,81 +53,147 @@ __device__ __forceinline__ void load_tile(TileRegs<D>& t, const uint8_t* base,
   for (int c = 0; c < D / 64; c++) t.v[c] = load16(at.v, Kv4<D>::kV + c * 1024);
 }
 
+// The work: each sequence's tiles in equal pieces of at most `per` tiles, a workgroup for
+// each piece and kv head. `per` comes from the batch's total on the device, so pieces are
+// as many as the GPU wants whether the lengths are equal or far apart; every workgroup
+// sums the lengths and finds its piece. A sequence of several pieces goes through the
+// workspace and a merge launch.
+constexpr int kDecThreads = kDecWaves * 64;
+
+// Tiles of each of a sequence's kv heads; one at least where it has rows (the run that has
+// it writes them: zeros, or NaN for a refused sequence).
+__device__ __forceinline__ uint32_t dec_tiles(const Kv4AttnArgs& a, const Kv4Seq& s) {
+  if (s.nq == 0) return 0;
+  if (s.refused) return 1;
+  const int64_t pos0 = (int64_t)s.n_keys - s.nq;
+  return max(1u, kv4_tiles(pos0, (int64_t)s.n_keys - 1, a.window, a.n_sinks).count());
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {  // in a scalar register
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// Tiles of a piece at most: `pieces` pieces for the batch, none cut below `least` tiles.
+__device__ __forceinline__ uint32_t dec_per(uint32_t total, uint32_t pieces, uint32_t least) {
+  return max(total / pieces + (total % pieces != 0), least);
+}
+
+// Sum over the workgroup of v, and over the threads before this one.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_wave, uint32_t& before) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t scan = v;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    const uint32_t y = __shfl_up(scan, x, kWave);
+    if (lane >= x) scan += y;
+  }
+  if (lane == 63) s_wave[wave] = scan;
+  __syncthreads();
+  uint32_t total = 0;
+  before = scan - v;
+#pragma unroll
+  for (int w = 0; w < kDecWaves; w++) {
+    if (w < wave) before += s_wave[w];
+    total += s_wave[w];
+  }
+  return uniform(total);
+}
+
 template <int D, int NT>
-__global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
-    Kv4AttnArgs a, Kv4SplitPlan plan, Kv4Part part, float scale_log2e) {
+__global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kernel(
+    Kv4AttnArgs a, Kv4Part part, uint32_t* first_piece, uint32_t pieces, uint32_t least,
+    float scale_log2e) {
   constexpr int kRows = 8 * NT, kSteps = D / 32, kOT = D / 16;
   __shared__ float s_o[kDecWaves][kRows][D + 4];
   __shared__ float s_m[kDecWaves][kRows], s_l[kDecWaves][kRows];
+  __shared__ uint32_t s_wave[2][kDecWaves], s_found[3];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kg = lane >> 4;
   const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
-  uint32_t id = blockIdx.x;
-  const uint32_t kvh = id % G;
-  id /= G;
-  const uint32_t rt = id % plan.row_tiles;
-  id /= plan.row_tiles;
-  const uint32_t b = id % a.n_seqs, split = id / a.n_seqs;
 
-  const Kv4Seq seq = kv4_seq(a, b);
-  const uint32_t rows = seq.nq * group;  // of the (sequence, kv head)
-  if (seq.refused) {
-    if (rt == 0 && split == 0)
-      for (uint32_t i = threadIdx.x; i < rows * D; i += blockDim.x) {
-        const uint32_t r = i / D;
-        a.o[((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D + i % D] =
-            __builtin_nanf("");
+  const uint32_t kvh = blockIdx.x % G, run = blockIdx.x / G;
+  uint32_t b = 0, piece = run, n_pieces, per;
+  if (a.n_seqs == 1) {
+    const uint32_t count = uniform(dec_tiles(a, kv4_seq(a, 0)));
+    per = dec_per(count, pieces, least);
+    n_pieces = (count + per - 1) / per;
+    if (blockIdx.x == 0 && threadIdx.x == 0) first_piece[0] = 0, first_piece[1] = n_pieces;
+    if (piece >= n_pieces) return;
+  } else {
+    // A thread per `each` sequences.
+    const uint32_t each = (a.n_seqs + kDecThreads - 1) / kDecThreads;
+    const uint32_t my_b = min(threadIdx.x * each, a.n_seqs), my_end = min(my_b + each, a.n_seqs);
+    uint32_t count = 0, tiles = 0, at;
+    for (uint32_t x = my_b; x < my_end; x++) tiles += count = dec_tiles(a, kv4_seq(a, x));
+    per = dec_per(block_scan(tiles, s_wave[0], at), pieces, least);
+    uint32_t mine = (count + per - 1) / per;  // of each == 1
+    if (each > 1) {
+      mine = 0;
+      for (uint32_t x = my_b; x < my_end; x++)
+        mine += (dec_tiles(a, kv4_seq(a, x)) + per - 1) / per;
+    }
+    const uint32_t all = block_scan(mine, s_wave[1], at);
+    if (blockIdx.x == 0) {  // for the merge
+      uint32_t p = at;
+      for (uint32_t x = my_b; x < my_end; x++) {
+        first_piece[x] = p;
+        if (each > 1) p += (dec_tiles(a, kv4_seq(a, x)) + per - 1) / per;
       }
+      if (threadIdx.x == 0) first_piece[a.n_seqs] = all;
+    }
+    if (run >= all) return;
+    if (run >= at && run < at + mine) {  // one thread
+      uint32_t x = my_b, n = mine;
+      if (each > 1)
+        while (run >= at + (n = (dec_tiles(a, kv4_seq(a, x)) + per - 1) / per)) at += n, x++;
+      s_found[0] = x;
+      s_found[1] = run - at;
+      s_found[2] = n;
+    }
+    __syncthreads();
+    b = uniform(s_found[0]), piece = uniform(s_found[1]), n_pieces = uniform(s_found[2]);
+  }
+  const Kv4Seq seq = kv4_seq(a, b);
+  const uint32_t n_rows = min(seq.nq * group, (uint32_t)kRows);
+  if (seq.refused) {
+    const uint64_t rows = (uint64_t)seq.nq * group;
+    for (uint64_t i = threadIdx.x; i < rows * D; i += kDecThreads) {
+      const uint32_t r = (uint32_t)(i / D);
+      a.o[((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D + i % D] =
+          __builtin_nanf("");
+    }
     return;
   }
-  const uint32_t r0 = rt * kRows;
-  if (r0 >= rows) return;
-  const uint32_t n_rows = min((uint32_t)kRows, rows - r0);
-  const int64_t pos0 = (int64_t)seq.n_keys - seq.nq;
-  const int64_t first = pos0 + r0 / group, last = pos0 + (r0 + n_rows - 1) / group;
+  const int64_t first = (int64_t)seq.n_keys - seq.nq, last = (int64_t)seq.n_keys - 1;
   const Kv4Span span(first, last, a.window, a.n_sinks);
-  const Kv4Pieces pc = kv4_pieces(span.tiles.count(), plan.most);
-  if (split >= pc.n) return;
-  const uint32_t t0 = split * pc.per, t1 = min(t0 + pc.per, span.tiles.count());
+  // Pieces of one length, or one tile less.
+  const uint32_t n_tiles = span.tiles.count();
+  const uint32_t t0 = (uint32_t)((uint64_t)n_tiles * piece / n_pieces);
+  const uint32_t t1 = (uint32_t)((uint64_t)n_tiles * (piece + 1) / n_pieces);
 
-  // q: column col of column tile nt is part col & 1 of row 8 nt + col / 2.
-  Half8 q[NT][kSteps];
-  float c_s[NT];
+  const float second = col & 1 ? -1.f : 0.f;  // this lane's columns are second parts
+
+  // q: column col of column tile nt is part col & 1 of row 8 nt + col / 2. The rows and
+  // the first tile are on their way together.
+  float4 qf[NT][D / 16];
   int delta[NT];  // the row's position behind the first
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
-    const uint32_t r = min(r0 + 8 * nt + (col >> 1), rows - 1);
-    delta[nt] = (int)(r / group - r0 / group);
+    const uint32_t r = min((uint32_t)(8 * nt + (col >> 1)), n_rows - 1);
+    delta[nt] = (int)(r / group);
     const float4* src = reinterpret_cast<const float4*>(
         a.q + ((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D +
         kg * (D / 4));
-    float x[D / 4];
-    float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 16; i++) {
-      const float4 f = src[i];
-      x[4 * i] = f.x, x[4 * i + 1] = f.y, x[4 * i + 2] = f.z, x[4 * i + 3] = f.w;
-#pragma unroll
-      for (int j = 0; j < 4; j++) amax = fmaxf(amax, fabsf(x[4 * i + j]));
-    }
-    amax = max_xor<16>(amax);
-    amax = max_xor<32>(amax);
-    const RowScale rs = row_scale(amax);
-    c_s[nt] = rs.down * scale_log2e;
-#pragma unroll
-    for (int i = 0; i < D / 8; i++) {
-      const float u = x[2 * i] * rs.up, v = x[2 * i + 1] * rs.up;
-      const halfx2 hi = pack_half2(u, v);
-      const halfx2 lo = rest_half2(u, v, hi);
-      q[nt][i >> 2].u[i & 3] = as_u32(col & 1 ? lo : hi);
-    }
+    for (int i = 0; i < D / 16; i++) qf[nt][i] = src[i];
   }
-
+  // l: the weights' sums, from a product with ones (every element of a column the same).
   floatx4v o[NT][kOT] = {};
-  float m[NT], l[NT];
+  float l[NT] = {};
+  float m[NT];
 #pragma unroll
-  for (int nt = 0; nt < NT; nt++) m[nt] = -INFINITY, l[nt] = 0.f;
+  for (int nt = 0; nt < NT; nt++) m[nt] = -INFINITY;
 
   const uint32_t log_page = 31 - __builtin_clz(a.s.page);  // 5 .. 8
   const uint32_t* row = a.table + (size_t)b * a.max_blocks;
@@ -143,6 +211,37 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
     const uint32_t in = index(it) & ((a.s.page >> 5) - 1);
     return a.pool + ((((size_t)id * G + kvh) << (log_page - 5)) + in) * tile_bytes;
   };
+
+  TileRegs<D> x, y;
+  const TileOffsets at = tile_offsets<D>(lane);
+  uint32_t id_x = 0, id_y = 0;
+  if (n_it > 0) {
+    id_x = page_of(0);
+    id_y = page_of(min(1u, n_it - 1));
+    load_tile<D>(x, base_of(0, id_x), at);
+  }
+
+  Half8 q[NT][kSteps];
+  float c_s[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++)
+      amax = fmaxf(fmaxf(fmaxf(amax, fabsf(qf[nt][i].x)), fmaxf(fabsf(qf[nt][i].y), fabsf(qf[nt][i].z))),
+                   fabsf(qf[nt][i].w));
+    amax = max_xor<16>(amax);
+    amax = max_xor<32>(amax);
+    const RowScale rs = row_scale(amax);
+    c_s[nt] = rs.down * scale_log2e;
+#pragma unroll
+    for (int i = 0; i < D / 8; i++) {
+      const float4 f = qf[nt][i >> 1];
+      const float u = (i & 1 ? f.z : f.x) * rs.up, v = (i & 1 ? f.w : f.y) * rs.up;
+      const halfx2 hi = pack_half2(u, v);
+      q[nt][i >> 2].u[i & 3] = as_u32(rest_half2(u, v, hi, second));
+    }
+  }
 
   auto work = [&](const TileRegs<D>& t, uint32_t it, bool bad) {
     const bool whole = span.whole(index(it));
@@ -207,8 +306,7 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const halfx2 hi = pack_half2(x[2 * i], x[2 * i + 1]);
-        const halfx2 lo = rest_half2(x[2 * i], x[2 * i + 1], hi);
-        p[nt].u[i] = as_u32(col & 1 ? lo : hi);
+        p[nt].u[i] = as_u32(rest_half2(x[2 * i], x[2 * i + 1], hi, second));
       }
     }
     if (!whole) {
@@ -272,10 +370,6 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
   };
 
   if (n_it > 0) {
-    TileRegs<D> x, y;
-    const TileOffsets at = tile_offsets<D>(lane);
-    uint32_t id_x = page_of(0), id_y = page_of(min(1u, n_it - 1));
-    load_tile<D>(x, base_of(0, id_x), at);
     for (uint32_t it = 0; it < n_it; it += 2) {
       // Past the end the last tile is read once more (an L2 hit) and not used.
       const uint32_t n1 = min(it + 1, n_it - 1), n2 = min(it + 2, n_it - 1);
@@ -313,8 +407,8 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
       }
   }
   __syncthreads();
-  const size_t slot = ((size_t)b * plan.row_tiles + rt) * G + kvh;
-  for (uint32_t i = threadIdx.x; i < n_rows * (D / 4); i += blockDim.x) {
+  const size_t slot = (size_t)blockIdx.x * kRows;
+  for (uint32_t i = threadIdx.x; i < n_rows * (D / 4); i += kDecThreads) {
     const uint32_t r = i / (D / 4), e = 4 * (i % (D / 4));
     float top = s_m[0][r];
 #pragma unroll
@@ -330,129 +424,114 @@ __global__ __launch_bounds__(kDecWaves * 64, 4 / NT) void kv4_decode_kernel(
       f.z = fmaf(g.z, k, f.z), f.w = fmaf(g.w, k, f.w);
       sum = fmaf(s_l[w][r], k, sum);
     }
-    if (pc.n == 1) {
+    if (n_pieces == 1) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       f.x *= inv, f.y *= inv, f.z *= inv, f.w *= inv;
-      const uint32_t rr = r0 + r;
       *reinterpret_cast<float4*>(
-          a.o + ((size_t)(seq.q0 + rr / group) * a.n_heads + kvh * group + rr % group) * D + e) = f;
+          a.o + ((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D + e) = f;
     } else {
-      const size_t at = (slot * plan.splits + split) * kRows + r;
-      if (e == 0) part.ml[2 * at] = top, part.ml[2 * at + 1] = sum;
-      *reinterpret_cast<float4*>(part.acc + at * D + e) = f;
+      if (e == 0) part.ml[2 * (slot + r)] = top, part.ml[2 * (slot + r) + 1] = sum;
+      *reinterpret_cast<float4*>(part.acc + (slot + r) * D + e) = f;
     }
   }
 }
 
-// Joins the pieces of a row: a workgroup per row, D / 4 threads over its dims and the
-// pieces dealt out to the 1024 / D groups of them (a long context has a hundred).
-template <int D>
-__global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, Kv4SplitPlan plan,
-                                                        Kv4Part part) {
-  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
-  __shared__ float4 s_acc[kGroups][kLanes];
-  __shared__ float s_sum[kGroups];
+// Joins the pieces of a sequence's row; a workgroup per row.
+template <int D, int kThreads>
+__global__ __launch_bounds__(kThreads) void kv4_decode_merge_kernel(Kv4AttnArgs a, Kv4Part part,
+                                                                    const uint32_t* first_piece,
+                                                                    uint32_t rows,
+                                                                    uint32_t slot_rows) {
   const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
-  const int lane = threadIdx.x & 63;
-  const uint32_t r = blockIdx.x % plan.rows, slot = blockIdx.x / plan.rows;
-  const uint32_t kvh = slot % G, rt = slot / G % plan.row_tiles, b = slot / G / plan.row_tiles;
+  const uint32_t r = blockIdx.x % rows, item = blockIdx.x / rows, kvh = item % G, b = item / G;
+  const uint32_t p0 = first_piece[b], n = first_piece[b + 1] - p0;
+  if (n <= 1) return;  // written by the piece itself
   const Kv4Seq seq = kv4_seq(a, b);
-  const uint32_t rows = seq.nq * group, r0 = rt * plan.rows, rr = r0 + r;
-  if (seq.refused || rr >= rows) return;
-  const uint32_t n_rows = min(plan.rows, rows - r0);
-  const int64_t pos0 = (int64_t)seq.n_keys - seq.nq;
-  const Kv4Tiles tiles = kv4_tiles(pos0 + r0 / group, pos0 + (r0 + n_rows - 1) / group, a.window,
-                                   a.n_sinks);
-  const uint32_t n = kv4_pieces(tiles.count(), plan.most).n;
-  if (n == 1) return;
-  const size_t at = (size_t)slot * plan.splits * plan.rows + r;
-  const float2* ml = reinterpret_cast<const float2*>(part.ml) + at;
-  float top = -INFINITY;
-  for (uint32_t i = lane; i < n; i += 64) top = fmaxf(top, ml[(size_t)i * plan.rows].x);
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, shfl_xor(top, x));
-  const uint32_t e = threadIdx.x % kLanes, g = threadIdx.x / kLanes;
-  float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-#pragma unroll 4
-  for (uint32_t i = g; i < n; i += kGroups) {
-    const float2 x = ml[(size_t)i * plan.rows];
-    const float4 y = reinterpret_cast<const float4*>(part.acc + (at + (size_t)i * plan.rows) * D)[e];
-    const float k = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.x - top);
-    sum = fmaf(x.y, k, sum);
-    f.x = fmaf(y.x, k, f.x), f.y = fmaf(y.y, k, f.y);
-    f.z = fmaf(y.z, k, f.z), f.w = fmaf(y.w, k, f.w);
-  }
-  s_acc[g][e] = f;
-  if (e == 0) s_sum[g] = sum;
-  __syncthreads();
-  if (g != 0) return;
-  for (int i = 1; i < kGroups; i++) {
-    const float4 y = s_acc[i][e];
-    f.x += y.x, f.y += y.y, f.z += y.z, f.w += y.w;
-    sum += s_sum[i];
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  float4* dst = reinterpret_cast<float4*>(
-      a.o + ((size_t)(seq.q0 + rr / group) * a.n_heads + kvh * group + rr % group) * D);
-  dst[e] = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+  if (r >= seq.nq * group) return;
+  merge_pieces<D, kThreads>(
+      part, n, [&](uint32_t i) { return ((size_t)(p0 + i) * G + kvh) * slot_rows + r; },
+      a.o + ((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D);
 }
 
-// Key tiles of a piece: few enough that the pieces of the call's bounds fill the
-// 256 CUs with four workgroups each a few times over (sequences are shorter than
-// the bound), and two a wave at least.
-constexpr uint32_t kDecTarget = 4096, kDecAlone = 1024, kDecFew = 2 * kDecWaves;
-
-Kv4SplitPlan kv4_decode_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
-                             uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
-                             uint32_t window, uint32_t n_sinks) {
-  Kv4SplitPlan p;
-  const uint32_t group = n_heads / n_kv_heads;
-  const uint64_t rows = (uint64_t)max_q * group;
-  p.rows = rows <= 8 ? 8 : 16;
-  p.row_tiles = (uint32_t)((rows + p.rows - 1) / p.rows);
-  const uint32_t tiles = kv4_max_tiles(max_n_keys, (p.rows + group - 1) / group + 1, window, n_sinks);
-  const uint64_t items = (uint64_t)n_seqs * n_kv_heads * p.row_tiles;
-  const uint32_t target = n_seqs == 1 ? kDecAlone : kDecTarget;
-  const uint64_t most = (items * tiles + target - 1) / target;
-  p.most = (uint32_t)(most < kDecFew ? kDecFew : most > 0xffffffffu ? 0xffffffffu : most);
-  p.splits = (tiles + p.most - 1) / p.most;
-  p.ws_bytes = p.splits == 1 ? 0
-                             : ws_align(items * p.splits * p.rows * 8) +
-                                   ws_align(items * p.splits * p.rows * head_dim * 4);
+// Pieces that a batch is cut into (over its kv heads), beside one more a sequence at most
+// from rounding up. 768 workgroups are resident (three a CU, by the kernel's registers);
+// twice as many let the GPU even out a batch, while a single sequence's pieces are equal
+// already and two a CU stream as fast. No piece has fewer than 20 tiles: up to 640 keys
+// then need no merge launch. us, 64 sequences of up to 16385 keys / one of 131072 / 128
+// with a window of 4096: 1024 pieces 127 / 36.3 / 70.5, 1536 120 / 36.3 / 68, 2048 121 /
+// 37.3 / 72, 3000 127 / 39 / 77; 512 for the one sequence 34.4; 513 keys in pieces of 8
+// tiles 12.1, of 20 9.6.
+constexpr uint32_t kDecPieces = 1536, kDecAlone = 512, kDecLeast = 5 * kDecWaves;
+struct DecodePlan {
+  uint32_t slot_rows;  // rows of a column tile
+  uint32_t pieces, least;
+  uint32_t runs;       // workgroups of a kv head
+};
+static DecodePlan decode_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
+                              uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                              uint32_t window, uint32_t n_sinks) {
+  DecodePlan p;
+  p.slot_rows = max_q * (n_heads / n_kv_heads) <= 8 ? 8 : 16;
+  p.least = kDecLeast;
+  p.pieces = std::max(1u, (n_seqs == 1 ? kDecAlone : kDecPieces) / n_kv_heads);
+  const uint64_t tiles = kv4_max_tiles(max_n_keys, max_q, window, n_sinks);
+  const uint64_t cut = (n_seqs * tiles + p.least - 1) / p.least;  // at most, plus n_seqs
+  p.runs = (uint32_t)std::min(std::min((uint64_t)p.pieces, cut) + n_seqs - 1,
+                              n_seqs * ((tiles + p.least - 1) / p.least));
   return p;
 }
 
-template <int D>
-static hipError_t launch(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws, hipStream_t st) {
-  const uint64_t items = (uint64_t)a.n_seqs * a.s.n_kv_heads * p.row_tiles;
-  if (items * p.splits > 0x7fffffffull || items * p.rows > 0x7fffffffull)
-    return hipErrorInvalidConfiguration;
-  const Kv4Part part = kv4_part(ws, p, items);
-  const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
-  const dim3 grid((uint32_t)(items * p.splits)), block(kDecWaves * 64);
-  if (p.rows == 8)
-    hipLaunchKernelGGL((kv4_decode_kernel<D, 1>), grid, block, 0, st, a, p, part, scale);
-  else
-    hipLaunchKernelGGL((kv4_decode_kernel<D, 2>), grid, block, 0, st, a, p, part, scale);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.splits == 1) return e;
-  return launch_kv4_merge(a, p, part, st);
+static uint64_t first_bytes(uint32_t n_seqs) { return ws_align(((uint64_t)n_seqs + 1) * 4); }
+static uint64_t slots(const DecodePlan& p, uint32_t n_kv_heads) {
+  return (uint64_t)p.runs * n_kv_heads * p.slot_rows;
 }
 
-hipError_t launch_kv4_merge(const Kv4AttnArgs& a, const Kv4SplitPlan& p, const Kv4Part& part,
-                            hipStream_t st) {
-  const uint32_t rows = a.n_seqs * a.s.n_kv_heads * p.row_tiles * p.rows;
-  if (a.s.head_dim == 128)
-    hipLaunchKernelGGL(kv4_merge_kernel<128>, dim3(rows), dim3(256), 0, st, a, p, part);
+uint64_t kv4_decode_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
+                             uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                             uint32_t window, uint32_t n_sinks) {
+  const DecodePlan p =
+      decode_plan(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, head_dim, window, n_sinks);
+  return first_bytes(n_seqs) + ws_align(slots(p, n_kv_heads) * 8) +
+         ws_align(slots(p, n_kv_heads) * head_dim * 4);
+}
+
+template <int D>
+static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
+  const uint32_t G = a.s.n_kv_heads;
+  const DecodePlan p =
+      decode_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, D, a.window, a.n_sinks);
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  uint32_t* first_piece = reinterpret_cast<uint32_t*>(w);
+  Kv4Part part;
+  w += first_bytes(a.n_seqs);
+  part.ml = reinterpret_cast<float*>(w);
+  part.acc = reinterpret_cast<float*>(w + ws_align(slots(p, G) * 8));
+  const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
+  const uint32_t rows = a.max_q * (a.n_heads / G);
+  const uint64_t items = (uint64_t)a.n_seqs * G;
+  if (items * rows > 0x7fffffffull || (uint64_t)p.runs * G > 0x7fffffffull)
+    return hipErrorInvalidConfiguration;
+  const dim3 grid(p.runs * G), block(kDecThreads);
+  if (p.slot_rows == 8)
+    hipLaunchKernelGGL((kv4_decode_kernel<D, 1>), grid, block, 0, st, a, part, first_piece,
+                       p.pieces, p.least, scale);
   else
-    hipLaunchKernelGGL(kv4_merge_kernel<64>, dim3(rows), dim3(256), 0, st, a, p, part);
+    hipLaunchKernelGGL((kv4_decode_kernel<D, 2>), grid, block, 0, st, a, part, first_piece,
+                       p.pieces, p.least, scale);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.runs <= a.n_seqs) return e;  // no more pieces than sequences: none cut
+  const dim3 mgrid((uint32_t)(items * rows));
+  if (p.runs >= 8 * a.n_seqs)  // many pieces a sequence
+    hipLaunchKernelGGL((kv4_decode_merge_kernel<D, 256>), mgrid, dim3(256), 0, st, a, part,
+                       first_piece, rows, p.slot_rows);
+  else
+    hipLaunchKernelGGL((kv4_decode_merge_kernel<D, 64>), mgrid, dim3(64), 0, st, a, part,
+                       first_piece, rows, p.slot_rows);
   return hipGetLastError();
 }
 
-hipError_t launch_kv4_decode(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws,
-                             hipStream_t st) {
-  return a.s.head_dim == 128 ? launch<128>(a, p, ws, st) : launch<64>(a, p, ws, st);
+hipError_t launch_kv4_decode(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
+  return a.s.head_dim == 128 ? launch<128>(a, ws, st) : launch<64>(a, ws, st);
 }
 
 }  // namespace flk

@@ -16,6 +16,23 @@ typedef float floatx16v __attribute__((ext_vector_type(16)));
 
 constexpr int kPreRows = 128, kPreThreads = 256, kStep = 64;
 
+// Pieces that a row tile's key tiles are cut into: as few as leave none more than
+// `most` tiles, then as equal as they come.
+struct Kv4Pieces {
+  uint32_t n, per;
+};
+__device__ __forceinline__ Kv4Pieces kv4_pieces(uint32_t tiles, uint32_t most) {
+  const uint32_t n = max(1u, (tiles + most - 1) / most);
+  return {n, (tiles + n - 1) / n};
+}
+
+// The plan, from the call's bounds alone (lengths are on the device).
+struct Kv4SplitPlan {
+  uint32_t row_tiles;  // row tiles of a (sequence, kv head)
+  uint32_t most;       // key tiles of a piece, at most
+  uint32_t splits;     // pieces that a row tile may have
+};
+
 // 16-byte slots of K's rows (8 dims each) and of V's (8 keys of a dim), xored so that
 // neighbouring rows of one slot lie in distinct banks.
 template <int D>
@@ -336,17 +353,37 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
                       o[c][4 * i + 3] * inv);
 }
 
+// Joins the pieces of a row: slot (row tile's number) * splits + piece.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Kv4AttnArgs a, Kv4SplitPlan plan,
+                                                                Kv4Part part) {
+  const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
+  const uint32_t r = blockIdx.x % kPreRows, slot = blockIdx.x / kPreRows;
+  const uint32_t kvh = slot % G, rt = slot / G % plan.row_tiles, b = slot / G / plan.row_tiles;
+  const Kv4Seq seq = kv4_seq(a, b);
+  const uint32_t rows = seq.nq * group, r0 = rt * kPreRows, rr = r0 + r;
+  if (seq.refused || rr >= rows) return;
+  const uint32_t n_rows = min((uint32_t)kPreRows, rows - r0);
+  const int64_t pos0 = (int64_t)seq.n_keys - seq.nq;
+  const Kv4Tiles tiles = kv4_tiles(pos0 + r0 / group, pos0 + (r0 + n_rows - 1) / group, a.window,
+                                   a.n_sinks);
+  const uint32_t n = kv4_pieces(tiles.count(), plan.most).n;
+  if (n == 1) return;
+  merge_pieces<D, 256>(
+      part, n, [&](uint32_t i) { return ((size_t)slot * plan.splits + i) * kPreRows + r; },
+      a.o + ((size_t)(seq.q0 + rr / group) * a.n_heads + kvh * group + rr % group) * D);
+}
+
 // Pieces: the call's work (from its bounds, causal) over two workgroups a CU, a few
 // pieces each, none below eight tiles; long prompts of many row tiles need no cuts, as
 // the heaviest row tiles come first.
 constexpr uint32_t kPreTarget = 1024, kPreFew = 8, kPreWhole = 512;
 
-Kv4SplitPlan kv4_prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
-                              uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
-                              uint32_t window, uint32_t n_sinks) {
+static Kv4SplitPlan prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
+                                 uint32_t n_heads, uint32_t n_kv_heads, uint32_t window,
+                                 uint32_t n_sinks) {
   Kv4SplitPlan p;
   const uint32_t group = n_heads / n_kv_heads;
-  p.rows = kPreRows;
   p.row_tiles = (uint32_t)(((uint64_t)max_q * group + kPreRows - 1) / kPreRows);
   const uint32_t tiles = kv4_max_tiles(max_n_keys, kPreRows / group + 2, window, n_sinks);
   const uint64_t items = (uint64_t)n_seqs * n_kv_heads * p.row_tiles;
@@ -359,29 +396,41 @@ Kv4SplitPlan kv4_prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_ke
   if (items >= kPreWhole) most = tiles;
   p.most = (uint32_t)(most > 0xfffffffeu ? 0xfffffffeu : most);
   p.splits = (uint32_t)(((uint64_t)tiles + p.most - 1) / p.most);
-  p.ws_bytes = p.splits == 1 ? 0
-                             : ws_align(items * p.splits * p.rows * 8) +
-                                   ws_align(items * p.splits * p.rows * head_dim * 4);
   return p;
 }
 
+uint64_t kv4_prefill_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
+                              uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                              uint32_t window, uint32_t n_sinks) {
+  const Kv4SplitPlan p =
+      prefill_plan(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, window, n_sinks);
+  if (p.splits == 1) return 0;
+  const uint64_t rows = (uint64_t)n_seqs * n_kv_heads * p.row_tiles * p.splits * kPreRows;
+  return ws_align(rows * 8) + ws_align(rows * head_dim * 4);
+}
+
 template <int D>
-static hipError_t launch(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws, hipStream_t st) {
+static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
+  const Kv4SplitPlan p = prefill_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, a.s.n_kv_heads,
+                                      a.window, a.n_sinks);
   const uint64_t items = (uint64_t)a.n_seqs * a.s.n_kv_heads * p.row_tiles;
-  if (items * p.splits > 0x7fffffffull || items * p.rows > 0x7fffffffull)
+  if (items * p.splits > 0x7fffffffull || items * kPreRows > 0x7fffffffull)
     return hipErrorInvalidConfiguration;
-  const Kv4Part part = kv4_part(ws, p, items);
+  Kv4Part part{static_cast<float*>(ws), nullptr};
+  part.acc = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) +
+                                      ws_align(items * p.splits * kPreRows * 8));
   const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
   hipLaunchKernelGGL(kv4_prefill_kernel<D>, dim3((uint32_t)(items * p.splits)), dim3(kPreThreads),
                      0, st, a, p, part, scale);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
-  return launch_kv4_merge(a, p, part, st);
+  hipLaunchKernelGGL(kv4_prefill_merge_kernel<D>, dim3((uint32_t)(items * kPreRows)), dim3(256), 0,
+                     st, a, p, part);
+  return hipGetLastError();
 }
 
-hipError_t launch_kv4_prefill(const Kv4AttnArgs& a, const Kv4SplitPlan& p, void* ws,
-                              hipStream_t st) {
-  return a.s.head_dim == 128 ? launch<128>(a, p, ws, st) : launch<64>(a, p, ws, st);
+hipError_t launch_kv4_prefill(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
+  return a.s.head_dim == 128 ? launch<128>(a, ws, st) : launch<64>(a, ws, st);
 }
 
 }  // namespace flk

@@ -33,20 +33,22 @@ struct Kv4SplitPlan {
   uint32_t splits;     // pieces that a row tile may have
 };
 
-// 16-byte slots of K's rows (8 dims each) and of V's (8 keys of a dim), xored so that
-// neighbouring rows of one slot lie in distinct banks.
+// LDS: K's rows in 16-byte slots of 8 dims, V's (a row a dim) in slots of 8 keys, slots
+// xored with bits of the row so that neighbouring rows of one slot lie in distinct banks.
+// Byte offsets in one buffer; the xors reach bits 4 .. 7 only, so a lane's other slots are
+// its first offset xor a constant.
 template <int D>
-__device__ __forceinline__ int k_slot(int key, int slot) {
-  return key * (D / 8) + (slot ^ (D == 128 ? key & 15 : (key >> 1) & 7));
+__device__ __forceinline__ uint32_t k_at(uint32_t key, uint32_t slot) {
+  return key * (2 * D) + ((slot ^ (D == 128 ? key & 15 : (key >> 1) & 7)) << 4);
 }
-__device__ __forceinline__ int v_slot(int dim, int slot) {
-  return dim * (kStep / 8) + (slot ^ ((dim >> 1) & 7) ^ ((dim >> 4) & 7));
+__device__ __forceinline__ uint32_t v_at(uint32_t dim, uint32_t slot) {
+  return dim * (2 * kStep) + ((slot ^ ((dim >> 1) & 7) ^ ((dim >> 4) & 7)) << 4);
 }
 
 template <int D>
-struct PreShared {
-  uint4 k[2][kStep * D / 8];
-  uint4 v[2][kStep * D / 8];
+struct alignas(16) PreShared {
+  uint8_t k[2][kStep * D * 2];
+  uint8_t v[2][kStep * D * 2];
   // Slots (keys) of a tile whose V scale is no number, by [block][g]; the scale counts
   // as 0 in LDS and the rows that see such a key get their NaN here.
   uint32_t flag[2][2][4];
@@ -151,6 +153,9 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
   const int v_block = v_n * (D / 16) / 32;
   const int ks_at = Kv4<D>::kKScale +
                     4 * (D == 128 ? piece & 63 : (piece >> 2) * 2 + ((piece >> 1) & 1));
+  const int st_half = D == 128 ? piece >> 6 : 0, st_key = D == 128 ? (piece >> 2) & 15 : piece >> 2;
+  const uint32_t k_to =
+      k_at<D>(32 * st_tile + 16 * st_half + st_key, (D == 128 ? 4 : 2) * (piece & 3));
   auto fetch = [&](uint32_t step, uint32_t page_id) {
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     const bool bad = page_id >= a.s.n_pages;
@@ -177,20 +182,19 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
   auto stage = [&](int buf) {
     if (st_k) {
       const uint32_t w[4] = {rg.k.x, rg.k.y, rg.k.z, rg.k.w};
-      const halfx2 ks = as_half2(rg.ks);
+      // D = 128: piece [half][key][part], octet i of the part, one scale. D = 64: [key][part]
+      // with two octets of each half.
+      const uint32_t lo = rg.ks & 0xffffu, hi = rg.ks >> 16;
+      const uint32_t one = D == 128 && st_half ? hi : lo;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        // D = 128: piece [half][key][part], octet i of the part. D = 64: [key][part] with
-        // two octets of each half.
-        const int half = D == 128 ? piece >> 6 : i >> 1;
-        const int key = D == 128 ? (piece >> 2) & 15 : piece >> 2;
-        const int slot = D == 128 ? 4 * (piece & 3) + i : 2 * (piece & 3) + (i & 1);
-        const _Float16 d1 = half ? ks[1] : ks[0];
-        const halfx2 d = {d1, d1};
+        const halfx2 d = as_half2((D == 128 || i < 2 ? one : hi) * 0x10001u);
         uint4 x;
         x.x = as_u32(kv4_pair<0>(w[i], d)), x.y = as_u32(kv4_pair<1>(w[i], d));
         x.z = as_u32(kv4_pair<2>(w[i], d)), x.w = as_u32(kv4_pair<3>(w[i], d));
-        sh.k[buf][k_slot<D>(32 * st_tile + 16 * half + key, slot)] = x;
+        // (Slots 4 part + i, or 2 part + i % 2 of half i / 2, whose rows lie 16 keys on.)
+        const uint32_t at = D == 128 ? k_to ^ (i << 4) : (k_to ^ ((i & 1) << 4)) + (i >> 1) * 32 * D;
+        *reinterpret_cast<uint4*>(&sh.k[buf][at]) = x;
       }
     }
     if (st_v) {
@@ -225,14 +229,14 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
         }
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
-          uint2* dst = reinterpret_cast<uint2*>(
-              &sh.v[buf][v_slot(dim, 4 * st_tile + 2 * ks + (v_g & 1))]);
-          dst[v_g >> 1] = make_uint2(x[2 * ks], x[2 * ks + 1]);
+          const uint32_t at = v_at(dim, 4 * st_tile + 2 * ks + (v_g & 1)) + 8 * (v_g >> 1);
+          *reinterpret_cast<uint2*>(&sh.v[buf][at]) = make_uint2(x[2 * ks], x[2 * ks + 1]);
         }
       }
     }
   };
 
+  const uint32_t k_from = k_at<D>(col, h), v_from = v_at(col, h);
   floatx16v o[kOT] = {};
   float m = -INFINITY, l = 0.f;
 
@@ -241,8 +245,8 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
     floatx16v s = {};
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
-      const halfx8 k =
-          __builtin_bit_cast(halfx8, sh.k[buf][k_slot<D>(32 * t2 + col, 2 * i + h)]);
+      const halfx8 k = *reinterpret_cast<const halfx8*>(
+          &sh.k[0][(k_from + buf * (kStep * D * 2)) ^ (i << 5)] + t2 * (64 * D));
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[i].h, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i].h, s, 0, 0, 0);
     }
@@ -283,8 +287,9 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
     for (int ks = 0; ks < 2; ks++)
 #pragma unroll
       for (int c = 0; c < kOT; c++) {
-        const halfx8 v =
-            __builtin_bit_cast(halfx8, sh.v[buf][v_slot(32 * c + col, 4 * t2 + 2 * ks + h)]);
+        const halfx8 v = *reinterpret_cast<const halfx8*>(
+            &sh.v[0][(v_from + buf * (kStep * D * 2)) ^ ((4 * t2 + 2 * ks) ^ (2 * c)) << 4] +
+            c * (64 * kStep));
         o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[ks].h, o[c], 0, 0, 0);
         o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[ks].h, o[c], 0, 0, 0);
       }
@@ -377,7 +382,7 @@ __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Kv4AttnArgs a, K
 // Pieces: the call's work (from its bounds, causal) over two workgroups a CU, a few
 // pieces each, none below eight tiles; long prompts of many row tiles need no cuts, as
 // the heaviest row tiles come first.
-constexpr uint32_t kPreTarget = 1024, kPreFew = 8, kPreWhole = 512;
+constexpr uint32_t kPreTarget = 512, kPreFew = 4, kPreWhole = 512;
 
 static Kv4SplitPlan prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
                                  uint32_t n_heads, uint32_t n_kv_heads, uint32_t window,

@@ -1056,9 +1056,6 @@ int32_t flk_kv4_attn(const float* q, const void* pool, const uint32_t* table,
   const uint64_t bytes = 4ull * n_tokens * n_heads * head_dim;
   if (q != o && overlap(q, bytes, o, bytes))
     return fail(FLK_ERR_ARG, "kv4_attn: o lies partly over q");
-  const uint64_t need = kv4_attn_ws_bytes(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, head_dim,
-                                          window, n_sinks);
-  if (int32_t rc = check_ws(ws, ws_bytes, need)) return rc;
   Kv4AttnArgs a{};
   a.q = q;
   a.pool = static_cast<const uint8_t*>(pool);
@@ -1067,5 +1064,12 @@ int32_t flk_kv4_attn(const float* q, const void* pool, const uint32_t* table,
   a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.max_q = max_q, a.max_n_keys = max_n_keys;
   a.max_blocks = max_blocks, a.n_heads = n_heads, a.window = window, a.n_sinks = n_sinks;
   a.s = Kv4Shape{n_kv_heads, head_dim, n_pages, page};
+  if (!kv4_attn_fits(a))
+    return fail(FLK_ERR_UNSUPPORTED,
+                "kv4_attn: %u sequences of up to %u rows and %u keys exceed a launch", n_seqs, max_q,
+                max_n_keys);
+  const uint64_t need = kv4_attn_ws_bytes(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, head_dim,
+                                          window, n_sinks);
+  if (int32_t rc = check_ws(ws, ws_bytes, need)) return rc;
   return hip_status(launch_kv4_attn(a, ws, g_stream), "flk_kv4_attn");
 }

@@ -129,6 +129,7 @@ struct Kv4AttnArgs {
 uint64_t kv4_attn_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys, uint32_t n_heads,
                            uint32_t n_kv_heads, uint32_t head_dim, uint32_t window,
                            uint32_t n_sinks);
+bool kv4_attn_fits(const Kv4AttnArgs& a);
 hipError_t launch_kv4_attn(const Kv4AttnArgs& a, void* ws, hipStream_t st);
 
 }  // namespace flk

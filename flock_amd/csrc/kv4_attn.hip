@@ -15,6 +15,10 @@ uint64_t kv4_attn_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
       n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, head_dim, window, n_sinks);
 }
 
+bool kv4_attn_fits(const Kv4AttnArgs& a) {
+  return few_rows(a.max_q, a.n_heads, a.s.n_kv_heads) ? kv4_decode_fits(a) : kv4_prefill_fits(a);
+}
+
 hipError_t launch_kv4_attn(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
   return (few_rows(a.max_q, a.n_heads, a.s.n_kv_heads) ? launch_kv4_decode : launch_kv4_prefill)(
       a, ws, st);

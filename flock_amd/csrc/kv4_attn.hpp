@@ -67,13 +67,13 @@ __device__ __forceinline__ halfx2 rest_half2(float a, float b, halfx2 hi, float 
 
 // A power of two that brings a row's largest |q| to 2^14 .. 2^15, and its inverse:
 // the row's two f16 parts then hold 22 bits of every element down to 2^-39 of the
-// largest. Rows below 2^-112 keep the largest factor (their scores are 0 next to 1);
+// largest. Rows below 2^-97 keep the largest factor (their scores are 0 next to 1);
 // infinities stay infinite, and their second part is NaN.
 struct RowScale {
   float up, down;
 };
 __device__ __forceinline__ RowScale row_scale(float amax) {
-  const uint32_t e = max((__builtin_bit_cast(uint32_t, amax) >> 23) & 255u, 15u);
+  const uint32_t e = max((__builtin_bit_cast(uint32_t, amax) >> 23) & 255u, 30u);
   return {__builtin_bit_cast(float, (268u - e) << 23), __builtin_bit_cast(float, (e - 14u) << 23)};
 }
 
@@ -145,6 +145,37 @@ inline uint32_t kv4_max_tiles(uint32_t max_n_keys, uint32_t queries, uint32_t wi
   return (uint32_t)(seen < all ? seen : all);
 }
 
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {  // in a scalar register
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// Tiles of a piece at most: `pieces` pieces for the batch, none cut below `least` tiles.
+__device__ __forceinline__ uint32_t kv4_per(uint32_t total, uint32_t pieces, uint32_t least) {
+  return max(total / pieces + (total % pieces != 0), least);
+}
+
+// Sum over the workgroup of v, and over the threads before this one.
+template <int kWaves>
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_wave, uint32_t& before) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t scan = v;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    const uint32_t y = __shfl_up(scan, x, kWave);
+    if (lane >= x) scan += y;
+  }
+  if (lane == 63) s_wave[wave] = scan;
+  __syncthreads();
+  uint32_t total = 0;
+  before = scan - v;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    if (w < wave) before += s_wave[w];
+    total += s_wave[w];
+  }
+  return uniform(total);
+}
+
 // Partial results: row r of slot x is at x * rows + r.
 struct Kv4Part {
   float* ml;   // pairs (reference, sum)
@@ -190,6 +221,29 @@ __device__ __forceinline__ void merge_pieces(const Kv4Part& part, uint32_t n, At
   reinterpret_cast<float4*>(dst)[e] = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
 }
 
+// The same by D / 4 neighbouring threads alone.
+template <int D, typename At>
+__device__ __forceinline__ void merge_few(const Kv4Part& part, uint32_t n, At at, float* dst) {
+  const float2* ml = reinterpret_cast<const float2*>(part.ml);
+  const uint32_t e = threadIdx.x % (D / 4);
+  float top = -INFINITY;
+  for (uint32_t i = 0; i < n; i++) top = fmaxf(top, ml[at(i)].x);
+  float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 4
+  for (uint32_t i = 0; i < n; i++) {
+    const size_t p = at(i);
+    const float2 x = ml[p];
+    const float4 y = reinterpret_cast<const float4*>(part.acc + p * D)[e];
+    const float k = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.x - top);
+    sum = fmaf(x.y, k, sum);
+    f.x = fmaf(y.x, k, f.x), f.y = fmaf(y.y, k, f.y);
+    f.z = fmaf(y.z, k, f.z), f.w = fmaf(y.w, k, f.w);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  reinterpret_cast<float4*>(dst)[e] = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+}
+
 uint64_t kv4_decode_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
                              uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                              uint32_t window, uint32_t n_sinks);
@@ -198,5 +252,9 @@ uint64_t kv4_prefill_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_ke
                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                               uint32_t window, uint32_t n_sinks);
 hipError_t launch_kv4_prefill(const Kv4AttnArgs& a, void* ws, hipStream_t st);
+
+// Whether a call's launches and its numbers of tiles (32 bits) hold it.
+bool kv4_decode_fits(const Kv4AttnArgs& a);
+bool kv4_prefill_fits(const Kv4AttnArgs& a);
 
 }  // namespace flk

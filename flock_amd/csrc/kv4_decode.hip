@@ -69,36 +69,6 @@ __device__ __forceinline__ uint32_t dec_tiles(const Kv4AttnArgs& a, const Kv4Seq
   return max(1u, kv4_tiles(pos0, (int64_t)s.n_keys - 1, a.window, a.n_sinks).count());
 }
 
-__device__ __forceinline__ uint32_t uniform(uint32_t v) {  // in a scalar register
-  return __builtin_amdgcn_readfirstlane(v);
-}
-
-// Tiles of a piece at most: `pieces` pieces for the batch, none cut below `least` tiles.
-__device__ __forceinline__ uint32_t dec_per(uint32_t total, uint32_t pieces, uint32_t least) {
-  return max(total / pieces + (total % pieces != 0), least);
-}
-
-// Sum over the workgroup of v, and over the threads before this one.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_wave, uint32_t& before) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t scan = v;
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) {
-    const uint32_t y = __shfl_up(scan, x, kWave);
-    if (lane >= x) scan += y;
-  }
-  if (lane == 63) s_wave[wave] = scan;
-  __syncthreads();
-  uint32_t total = 0;
-  before = scan - v;
-#pragma unroll
-  for (int w = 0; w < kDecWaves; w++) {
-    if (w < wave) before += s_wave[w];
-    total += s_wave[w];
-  }
-  return uniform(total);
-}
-
 template <int D, int NT>
 __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kernel(
     Kv4AttnArgs a, Kv4Part part, uint32_t* first_piece, uint32_t pieces, uint32_t least,
@@ -116,7 +86,7 @@ __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kerne
   uint32_t b = 0, piece = run, n_pieces, per;
   if (a.n_seqs == 1) {
     const uint32_t count = uniform(dec_tiles(a, kv4_seq(a, 0)));
-    per = dec_per(count, pieces, least);
+    per = kv4_per(count, pieces, least);
     n_pieces = (count + per - 1) / per;
     if (blockIdx.x == 0 && threadIdx.x == 0) first_piece[0] = 0, first_piece[1] = n_pieces;
     if (piece >= n_pieces) return;
@@ -126,14 +96,14 @@ __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kerne
     const uint32_t my_b = min(threadIdx.x * each, a.n_seqs), my_end = min(my_b + each, a.n_seqs);
     uint32_t count = 0, tiles = 0, at;
     for (uint32_t x = my_b; x < my_end; x++) tiles += count = dec_tiles(a, kv4_seq(a, x));
-    per = dec_per(block_scan(tiles, s_wave[0], at), pieces, least);
+    per = kv4_per(block_scan<kDecWaves>(tiles, s_wave[0], at), pieces, least);
     uint32_t mine = (count + per - 1) / per;  // of each == 1
     if (each > 1) {
       mine = 0;
       for (uint32_t x = my_b; x < my_end; x++)
         mine += (dec_tiles(a, kv4_seq(a, x)) + per - 1) / per;
     }
-    const uint32_t all = block_scan(mine, s_wave[1], at);
+    const uint32_t all = block_scan<kDecWaves>(mine, s_wave[1], at);
     if (blockIdx.x == 0) {  // for the merge
       uint32_t p = at;
       for (uint32_t x = my_b; x < my_end; x++) {
@@ -495,6 +465,16 @@ uint64_t kv4_decode_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_key
          ws_align(slots(p, n_kv_heads) * head_dim * 4);
 }
 
+bool kv4_decode_fits(const Kv4AttnArgs& a) {
+  const uint32_t G = a.s.n_kv_heads;
+  const DecodePlan p =
+      decode_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.s.head_dim, a.window, a.n_sinks);
+  const uint64_t tiles =
+      (uint64_t)a.n_seqs * kv4_max_tiles(a.max_n_keys, a.max_q, a.window, a.n_sinks);
+  return tiles <= 0xffffffffull && (uint64_t)p.runs * G <= 0x7fffffffull &&
+         (uint64_t)a.n_seqs * a.max_q * a.n_heads <= 0x7fffffffull;
+}
+
 template <int D>
 static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
   const uint32_t G = a.s.n_kv_heads;
@@ -509,8 +489,6 @@ static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
   const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
   const uint32_t rows = a.max_q * (a.n_heads / G);
   const uint64_t items = (uint64_t)a.n_seqs * G;
-  if (items * rows > 0x7fffffffull || (uint64_t)p.runs * G > 0x7fffffffull)
-    return hipErrorInvalidConfiguration;
   const dim3 grid(p.runs * G), block(kDecThreads);
   if (p.slot_rows == 8)
     hipLaunchKernelGGL((kv4_decode_kernel<D, 1>), grid, block, 0, st, a, part, first_piece,

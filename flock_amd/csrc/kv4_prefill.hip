@@ -8,6 +8,8 @@
 // has read; the next tiles' codes are loaded meanwhile. S^T = K Q^T and O^T += V^T P^T on
 // 32x32x16: a column is a row of q, and P^T is taken from the S^T accumulators as they
 // lie, because V's keys are put in the order in which a lane holds its scores.
+#include <algorithm>
+
 #include "kv4_attn.hpp"
 
 namespace flk {
@@ -15,23 +17,49 @@ namespace flk {
 typedef float floatx16v __attribute__((ext_vector_type(16)));
 
 constexpr int kPreRows = 128, kPreThreads = 256, kStep = 64;
+// Pieces of a call (over its kv heads): one for each of the two workgroups a CU that are
+// resident; with as many row tiles anyway, some more, so that the heaviest are cut. None
+// has fewer than four key tiles. us, 2048 tokens / 64 at 32768 / four prompts of 500 to
+// 1500 onto up to 3000 / 8192 tokens: 512 pieces 64 / 55.6 / 166 / 545, 640 73 / 69.7 /
+// 164 / 525, 1024 74 / 73 / 179 / 559; whole row tiles cut by the call's bounds 107 / 55.7 /
+// 251 / 546.
+constexpr uint32_t kPrePieces = 512, kPreMore = 640, kPreLeast = 4;
 
-// Pieces that a row tile's key tiles are cut into: as few as leave none more than
-// `most` tiles, then as equal as they come.
-struct Kv4Pieces {
-  uint32_t n, per;
+// The work: row tiles, those of the last queries first (they see the most keys), each in
+// equal pieces of at most `per` key tiles where there are up to kMaxCut row tiles. As for
+// single tokens, `per` comes from the batch's total on the device, and every workgroup finds
+// its piece; more row tiles than that fill the GPU whole.
+constexpr uint32_t kMaxCut = kPreThreads;
+
+struct PrePlan {
+  uint32_t row_tiles;  // of a sequence, at most
+  uint32_t pieces;     // that the row tiles are cut into (for a kv head); 0: whole
+  uint32_t runs;       // workgroups of a kv head
 };
-__device__ __forceinline__ Kv4Pieces kv4_pieces(uint32_t tiles, uint32_t most) {
-  const uint32_t n = max(1u, (tiles + most - 1) / most);
-  return {n, (tiles + n - 1) / n};
+
+// Row tile e: its sequence and place, and its key tiles (none: no rows; one at least
+// otherwise, of a refused sequence the first row tile alone).
+struct PreItem {
+  uint32_t b, rt;
+};
+__device__ __forceinline__ PreItem pre_item(const Kv4AttnArgs& a, const PrePlan& p, uint32_t e) {
+  return {e % a.n_seqs, p.row_tiles - 1 - e / a.n_seqs};
 }
-
-// The plan, from the call's bounds alone (lengths are on the device).
-struct Kv4SplitPlan {
-  uint32_t row_tiles;  // row tiles of a (sequence, kv head)
-  uint32_t most;       // key tiles of a piece, at most
-  uint32_t splits;     // pieces that a row tile may have
-};
+__device__ __forceinline__ Kv4Tiles pre_tiles(const Kv4AttnArgs& a, const Kv4Seq& seq, uint32_t rt,
+                                              uint32_t group) {
+  const uint32_t r0 = rt * kPreRows, rows = seq.nq * group;
+  const int64_t pos0 = (int64_t)seq.n_keys - seq.nq;
+  return kv4_tiles(pos0 + r0 / group, pos0 + (min(r0 + (uint32_t)kPreRows, rows) - 1) / group, a.window,
+                   a.n_sinks);
+}
+__device__ __forceinline__ uint32_t pre_count(const Kv4AttnArgs& a, const PrePlan& p, uint32_t e,
+                                              uint32_t group) {
+  const PreItem i = pre_item(a, p, e);
+  const Kv4Seq seq = kv4_seq(a, i.b);
+  if (i.rt * kPreRows >= seq.nq * group) return 0;
+  if (seq.refused) return i.rt == 0;
+  return max(1u, pre_tiles(a, seq, i.rt, group).count());
+}
 
 // LDS: K's rows in 16-byte slots of 8 dims, V's (a row a dim) in slots of 8 keys, slots
 // xored with bits of the row so that neighbouring rows of one slot lie in distinct banks.
@@ -62,24 +90,52 @@ struct PreRegs {
 
 template <int D>
 __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
-    Kv4AttnArgs a, Kv4SplitPlan plan, Kv4Part part, float scale_log2e) {
+    Kv4AttnArgs a, PrePlan plan, Kv4Part part, uint32_t* first_piece, float scale_log2e) {
   constexpr int kSteps = D / 16, kOT = D / 32;
   __shared__ PreShared<D> sh;
+  __shared__ uint32_t s_wave[kPreThreads / 64], s_found[3];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
   const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
-  uint32_t id = blockIdx.x;
-  const uint32_t kvh = id % G;
-  id /= G;
-  const uint32_t b = id % a.n_seqs;
-  id /= a.n_seqs;
-  const uint32_t split = id % plan.splits, rt = plan.row_tiles - 1 - id / plan.splits;
-
+  const uint32_t kvh = blockIdx.x % G, run = blockIdx.x / G;
+  uint32_t e = run, cut = 0, n_pieces = 1;
+  if (plan.pieces > 0) {
+    // A thread per row tile.
+    const uint32_t items = a.n_seqs * plan.row_tiles;
+    uint32_t at;
+    const uint32_t count = threadIdx.x < items ? pre_count(a, plan, threadIdx.x, group) : 0;
+    uint32_t per = kv4_per(block_scan<kPreThreads / 64>(count, s_wave, at), plan.pieces, kPreLeast);
+    uint32_t mine, all;
+    // Rounding up makes more pieces than asked for: where that leaves a few for a second
+    // round of the GPU, longer ones.
+    for (int round = 0;; round++) {
+      __syncthreads();
+      mine = (count + per - 1) / per;
+      all = block_scan<kPreThreads / 64>(mine, s_wave, at);
+      if (all <= plan.pieces || items >= plan.pieces || round == 3) break;
+      per = max(per + 1, (uint32_t)((uint64_t)per * all / plan.pieces));
+    }
+    if (blockIdx.x == 0) {  // for the merge
+      if (threadIdx.x < items) first_piece[threadIdx.x] = at;
+      if (threadIdx.x == 0) first_piece[items] = all;
+    }
+    if (run >= all) return;
+    if (run >= at && run < at + mine) {  // one thread
+      s_found[0] = threadIdx.x;
+      s_found[1] = run - at;
+      s_found[2] = mine;
+    }
+    __syncthreads();
+    e = uniform(s_found[0]), cut = uniform(s_found[1]), n_pieces = uniform(s_found[2]);
+  }
+  const uint32_t b = pre_item(a, plan, e).b, rt = pre_item(a, plan, e).rt;
   const Kv4Seq seq = kv4_seq(a, b);
   const uint32_t rows = seq.nq * group;
+  const uint32_t r0 = rt * kPreRows;
+  if (r0 >= rows) return;
   if (seq.refused) {
-    if (rt == 0 && split == 0)
+    if (rt == 0)
       for (uint64_t i = threadIdx.x; i < (uint64_t)rows * D; i += kPreThreads) {
         const uint32_t r = (uint32_t)(i / D);
         a.o[((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D + i % D] =
@@ -87,15 +143,11 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
       }
     return;
   }
-  const uint32_t r0 = rt * kPreRows;
-  if (r0 >= rows) return;
-  const uint32_t n_rows = min((uint32_t)kPreRows, rows - r0);
   const int64_t pos0 = (int64_t)seq.n_keys - seq.nq;
-  const Kv4Tiles tiles = kv4_tiles(pos0 + r0 / group, pos0 + (r0 + n_rows - 1) / group, a.window,
-                                   a.n_sinks);
-  const Kv4Pieces pc = kv4_pieces(tiles.count(), plan.most);
-  if (split >= pc.n) return;
-  const uint32_t t0 = split * pc.per, t1 = min(t0 + pc.per, tiles.count());
+  const Kv4Tiles tiles = pre_tiles(a, seq, rt, group);
+  const uint32_t n_tiles = tiles.count();
+  const uint32_t t0 = (uint32_t)((uint64_t)n_tiles * cut / n_pieces);
+  const uint32_t t1 = (uint32_t)((uint64_t)n_tiles * (cut + 1) / n_pieces);
   const uint32_t n_steps = (t1 - t0 + 1) / 2;
 
   // This wave's rows.
@@ -250,6 +302,13 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[i].h, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i].h, s, 0, 0, 0);
     }
+    // (K's operands two reads ahead of the products.)
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
     Kv4Mask mask{};
     if (!whole) {
       mask = span.mask(tile);
@@ -284,22 +343,28 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
       pl[i >> 2].u[i & 3] = as_u32(rest_half2(s[2 * i], s[2 * i + 1], hi));
     }
 #pragma unroll
-    for (int ks = 0; ks < 2; ks++)
+    for (int ks = 0; ks < 2; ks++) {
+      halfx8 v[kOT];
 #pragma unroll
       for (int c = 0; c < kOT; c++) {
-        const halfx8 v = *reinterpret_cast<const halfx8*>(
+        v[c] = *reinterpret_cast<const halfx8*>(
             &sh.v[0][(v_from + buf * (kStep * D * 2)) ^ ((4 * t2 + 2 * ks) ^ (2 * c)) << 4] +
             c * (64 * kStep));
-        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[ks].h, o[c], 0, 0, 0);
-        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[ks].h, o[c], 0, 0, 0);
+        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[c], pl[ks].h, o[c], 0, 0, 0);
       }
+#pragma unroll
+      for (int c = 0; c < kOT; c++)
+        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[c], ph[ks].h, o[c], 0, 0, 0);
+    }
     const uint32_t* flag = sh.flag[buf][t2];
     uint32_t any = 0;
 #pragma unroll
     for (int c = 0; c < kOT; c++) any |= flag[c];
     if (__builtin_amdgcn_readfirstlane(any)) {
+#pragma unroll 1
       for (int c = 0; c < kOT; c++) {
         bool hit = false;
+#pragma unroll 1
         for (int key = 0; key < 32; key++) {
           const uint32_t bits = flag[c] >> (8 * ((key >> 2) & 3));
           hit |= (bits >> ((key & 3) + 4 * (key >> 4)) & 1) && (whole || mask.sees(key, delta));
@@ -344,11 +409,10 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
   float lo, hi;
   swap_pair<32>(l, lo, hi);
   l = lo + hi;
-  const size_t slot = ((size_t)b * plan.row_tiles + rt) * G + kvh;
-  const size_t at = (slot * plan.splits + split) * kPreRows + wave * 32 + col;
-  float* dst = pc.n == 1 ? a.o + my_at : part.acc + at * D;
-  const float inv = pc.n > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-  if (pc.n > 1 && h == 0) part.ml[2 * at] = m, part.ml[2 * at + 1] = l;
+  const size_t at = (size_t)blockIdx.x * kPreRows + wave * 32 + col;
+  float* dst = n_pieces == 1 ? a.o + my_at : part.acc + at * D;
+  const float inv = n_pieces > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+  if (n_pieces > 1 && h == 0) part.ml[2 * at] = m, part.ml[2 * at + 1] = l;
 #pragma unroll
   for (int c = 0; c < kOT; c++)
 #pragma unroll
@@ -358,79 +422,97 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
                       o[c][4 * i + 3] * inv);
 }
 
-// Joins the pieces of a row: slot (row tile's number) * splits + piece.
-template <int D>
-__global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Kv4AttnArgs a, Kv4SplitPlan plan,
-                                                                Kv4Part part) {
+// Joins the pieces of rows: a workgroup per row, or (FEW pieces) D / 4 threads per row, for
+// there may be many rows and nothing to join.
+template <int D, bool FEW>
+__global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Kv4AttnArgs a, PrePlan plan,
+                                                                Kv4Part part,
+                                                                const uint32_t* first_piece) {
+  constexpr uint32_t kRows = FEW ? 1024 / D : 1, kParts = kPreRows / kRows;
   const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
-  const uint32_t r = blockIdx.x % kPreRows, slot = blockIdx.x / kPreRows;
-  const uint32_t kvh = slot % G, rt = slot / G % plan.row_tiles, b = slot / G / plan.row_tiles;
-  const Kv4Seq seq = kv4_seq(a, b);
-  const uint32_t rows = seq.nq * group, r0 = rt * kPreRows, rr = r0 + r;
-  if (seq.refused || rr >= rows) return;
-  const uint32_t n_rows = min((uint32_t)kPreRows, rows - r0);
-  const int64_t pos0 = (int64_t)seq.n_keys - seq.nq;
-  const Kv4Tiles tiles = kv4_tiles(pos0 + r0 / group, pos0 + (r0 + n_rows - 1) / group, a.window,
-                                   a.n_sinks);
-  const uint32_t n = kv4_pieces(tiles.count(), plan.most).n;
-  if (n == 1) return;
-  merge_pieces<D, 256>(
-      part, n, [&](uint32_t i) { return ((size_t)slot * plan.splits + i) * kPreRows + r; },
-      a.o + ((size_t)(seq.q0 + rr / group) * a.n_heads + kvh * group + rr % group) * D);
+  const uint32_t kvh = blockIdx.x / kParts % G, e = blockIdx.x / kParts / G;
+  const uint32_t p0 = first_piece[e], n = first_piece[e + 1] - p0;
+  if (n <= 1) return;  // written by the piece itself
+  const PreItem i = pre_item(a, plan, e);
+  const Kv4Seq seq = kv4_seq(a, i.b);
+  const uint32_t r = blockIdx.x % kParts * kRows + (FEW ? threadIdx.x / (D / 4) : 0);
+  const uint32_t rr = i.rt * kPreRows + r;
+  if (rr >= seq.nq * group) return;
+  float* dst = a.o + ((size_t)(seq.q0 + rr / group) * a.n_heads + kvh * group + rr % group) * D;
+  auto at = [&](uint32_t x) { return ((size_t)(p0 + x) * G + kvh) * kPreRows + r; };
+  if constexpr (FEW)
+    merge_few<D>(part, n, at, dst);
+  else
+    merge_pieces<D, 256>(part, n, at, dst);
 }
 
-// Pieces: the call's work (from its bounds, causal) over two workgroups a CU, a few
-// pieces each, none below eight tiles; long prompts of many row tiles need no cuts, as
-// the heaviest row tiles come first.
-constexpr uint32_t kPreTarget = 512, kPreFew = 4, kPreWhole = 512;
-
-static Kv4SplitPlan prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
-                                 uint32_t n_heads, uint32_t n_kv_heads, uint32_t window,
-                                 uint32_t n_sinks) {
-  Kv4SplitPlan p;
+static PrePlan prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys, uint32_t n_heads,
+                            uint32_t n_kv_heads, uint32_t window, uint32_t n_sinks) {
+  PrePlan p;
   const uint32_t group = n_heads / n_kv_heads;
   p.row_tiles = (uint32_t)(((uint64_t)max_q * group + kPreRows - 1) / kPreRows);
-  const uint32_t tiles = kv4_max_tiles(max_n_keys, kPreRows / group + 2, window, n_sinks);
-  const uint64_t items = (uint64_t)n_seqs * n_kv_heads * p.row_tiles;
-  // The tiles of the mean row tile.
-  const uint32_t q = max_q < max_n_keys ? max_q : max_n_keys;
-  const uint64_t mean = kv4_max_tiles(max_n_keys - q / 2, kPreRows / group + 2, window, n_sinks);
-  uint64_t most = (items * mean + kPreTarget - 1) / kPreTarget;
-  most = (most + 1) / 2 * 2;
-  if (most < kPreFew) most = kPreFew;
-  if (items >= kPreWhole) most = tiles;
-  p.most = (uint32_t)(most > 0xfffffffeu ? 0xfffffffeu : most);
-  p.splits = (uint32_t)(((uint64_t)tiles + p.most - 1) / p.most);
+  const uint64_t items = (uint64_t)n_seqs * p.row_tiles;
+  const uint64_t tiles = kv4_max_tiles(max_n_keys, kPreRows / group + 2, window, n_sinks);
+  const uint64_t most = (tiles + kPreLeast - 1) / kPreLeast;  // pieces of a row tile
+  p.pieces = std::max(1u, kPrePieces / n_kv_heads);
+  if (items >= p.pieces) p.pieces = std::max(1u, kPreMore / n_kv_heads);
+  if (items > kMaxCut || most == 1) {
+    p.pieces = 0;
+    p.runs = (uint32_t)std::min(items, (uint64_t)0xffffffffu);
+  } else {
+    p.runs = (uint32_t)std::min(p.pieces + items - 1, items * most);
+  }
   return p;
 }
+
+static uint64_t first_bytes() { return ws_align((kMaxCut + 1) * 4); }
 
 uint64_t kv4_prefill_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                               uint32_t window, uint32_t n_sinks) {
-  const Kv4SplitPlan p =
-      prefill_plan(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, window, n_sinks);
-  if (p.splits == 1) return 0;
-  const uint64_t rows = (uint64_t)n_seqs * n_kv_heads * p.row_tiles * p.splits * kPreRows;
-  return ws_align(rows * 8) + ws_align(rows * head_dim * 4);
+  const PrePlan p = prefill_plan(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, window, n_sinks);
+  if (p.pieces == 0) return 0;
+  const uint64_t rows = (uint64_t)p.runs * n_kv_heads * kPreRows;
+  return first_bytes() + ws_align(rows * 8) + ws_align(rows * head_dim * 4);
+}
+
+bool kv4_prefill_fits(const Kv4AttnArgs& a) {
+  const uint32_t G = a.s.n_kv_heads;
+  const PrePlan p =
+      prefill_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.window, a.n_sinks);
+  const uint64_t items = (uint64_t)a.n_seqs * p.row_tiles;
+  const uint64_t tiles = kv4_max_tiles(a.max_n_keys, a.max_q, a.window, a.n_sinks);
+  return (uint64_t)p.runs * G <= 0x7fffffffull && items <= 0x7fffffffull / G &&
+         (p.pieces == 0 || (items * G * kPreRows <= 0x7fffffffull && items * tiles <= 0xffffffffull));
 }
 
 template <int D>
 static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
-  const Kv4SplitPlan p = prefill_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, a.s.n_kv_heads,
-                                      a.window, a.n_sinks);
-  const uint64_t items = (uint64_t)a.n_seqs * a.s.n_kv_heads * p.row_tiles;
-  if (items * p.splits > 0x7fffffffull || items * kPreRows > 0x7fffffffull)
-    return hipErrorInvalidConfiguration;
-  Kv4Part part{static_cast<float*>(ws), nullptr};
-  part.acc = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) +
-                                      ws_align(items * p.splits * kPreRows * 8));
+  const uint32_t G = a.s.n_kv_heads;
+  const PrePlan p =
+      prefill_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.window, a.n_sinks);
+  const uint64_t grid = (uint64_t)p.runs * G, items = (uint64_t)a.n_seqs * p.row_tiles * G;
+  uint32_t* first_piece = nullptr;
+  Kv4Part part{};
+  if (p.pieces > 0) {
+    uint8_t* w = static_cast<uint8_t*>(ws);
+    first_piece = reinterpret_cast<uint32_t*>(w);
+    w += first_bytes();
+    part.ml = reinterpret_cast<float*>(w);
+    part.acc = reinterpret_cast<float*>(w + ws_align(grid * kPreRows * 8));
+  }
   const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
-  hipLaunchKernelGGL(kv4_prefill_kernel<D>, dim3((uint32_t)(items * p.splits)), dim3(kPreThreads),
-                     0, st, a, p, part, scale);
+  hipLaunchKernelGGL(kv4_prefill_kernel<D>, dim3((uint32_t)grid), dim3(kPreThreads), 0, st, a, p,
+                     part, first_piece, scale);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.splits == 1) return e;
-  hipLaunchKernelGGL(kv4_prefill_merge_kernel<D>, dim3((uint32_t)(items * kPreRows)), dim3(256), 0,
-                     st, a, p, part);
+  if (e != hipSuccess || p.pieces == 0 || p.runs <= a.n_seqs * p.row_tiles) return e;
+  if (p.runs >= 8 * a.n_seqs * p.row_tiles)  // many pieces a row tile
+    hipLaunchKernelGGL((kv4_prefill_merge_kernel<D, false>), dim3((uint32_t)(items * kPreRows)),
+                       dim3(256), 0, st, a, p, part, first_piece);
+  else
+    hipLaunchKernelGGL((kv4_prefill_merge_kernel<D, true>),
+                       dim3((uint32_t)(items * (kPreRows * D / 1024))), dim3(256), 0, st, a, p,
+                       part, first_piece);
   return hipGetLastError();
 }
 

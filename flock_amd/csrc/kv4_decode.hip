@@ -280,15 +280,16 @@ __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kerne
       }
     }
     if (!whole) {
-      // Values of keys that some row does not see: scales that are no numbers (NaN
-      // blocks, memory never written) count as 0 in the products, and make NaN of the
-      // rows that do see them.
+      // Values of keys that some row does not see: scales from 8192 on, which no append
+      // writes but for NaN blocks (memory never written holds anything, and times a code
+      // it may be infinite), count as 0 in the products, and make NaN of the rows that do
+      // see them.
       Half8 flag;
       uint32_t* w = reinterpret_cast<uint32_t*>(&vs);
       bool any = false;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const bool lo = (w[i] & 0x7c00u) == 0x7c00u, hi = (w[i] & 0x7c000000u) == 0x7c000000u;
+        const bool lo = (w[i] & 0x7000u) == 0x7000u, hi = (w[i] & 0x70000000u) == 0x70000000u;
         flag.u[i] = (lo ? 0x3c00u : 0u) | (hi ? 0x3c000000u : 0u);
         w[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
         any |= lo || hi;

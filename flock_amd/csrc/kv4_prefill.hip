@@ -77,8 +77,9 @@ template <int D>
 struct alignas(16) PreShared {
   uint8_t k[2][kStep * D * 2];
   uint8_t v[2][kStep * D * 2];
-  // Slots (keys) of a tile whose V scale is no number, by [block][g]; the scale counts
-  // as 0 in LDS and the rows that see such a key get their NaN here.
+  // Slots (keys) of a tile whose V scale is 8192 or more, by [block][g]: a NaN block's, or
+  // memory never written behind a sequence. It counts as 0 in LDS, and the rows that see
+  // such a key get their NaN from here.
   uint32_t flag[2][2][4];
 };
 
@@ -254,11 +255,11 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
       const uint32_t w[4] = {rg.v.x, rg.v.y, rg.v.z, rg.v.w};
       uint32_t odd = 0, mask = 0;
 #pragma unroll
-      for (int i = 0; i < 4; i++) odd |= (s[i] & 0x7c007c00u) + 0x04000400u;
+      for (int i = 0; i < 4; i++) odd |= (s[i] & 0x70007000u) + 0x10001000u;
       if (odd & 0x80008000u) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const bool lo = (s[i] & 0x7c00u) == 0x7c00u, hi = (s[i] & 0x7c000000u) == 0x7c000000u;
+          const bool lo = (s[i] & 0x7000u) == 0x7000u, hi = (s[i] & 0x70000000u) == 0x70000000u;
           s[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
           mask |= (lo ? 1u : 0u) << (2 * i) | (hi ? 2u : 0u) << (2 * i);
         }

@@ -167,7 +167,8 @@ def test_prologue_stores_the_f32_prologues_rows(n, H, G, D, page, pairing, stack
 class Batch:
     """Sequences of n_keys[b] keys with their pages dealt out at random, and q rows
     for the last n_new[b] of them. Pages that no visible key needs have no entry;
-    what the table's last pages hold behind a sequence is NaN and infinities."""
+    what the table's last pages hold behind a sequence is NaN, infinities and scales whose
+    products with codes are infinite."""
 
     def __init__(self, rng, n_keys, n_new, H, G, D, page, window=0, sinks=0, k=None, v=None):
         self.shape = (H, G, D, page, window, sinks)
@@ -183,7 +184,7 @@ class Batch:
         self.pool = rng.integers(0, 256, (self.P, G, page // 32, 36 * D), dtype=np.uint8)
         kb, _, ks, vb, _, vs = ref.places(D)
         for at in (np.unique(ks), np.unique(vs)):
-            bits = np.where(rng.random(self.pool[..., at].shape) < 0.5, 0x7E00, 0xFC00)
+            bits = rng.choice([0x7E00, 0xFC00, 0x7BFF, 0xF001], self.pool[..., at].shape)
             self.pool[..., at] = bits & 255
             self.pool[..., at + 1] = bits >> 8
         self.k, self.v = [], []
@@ -381,3 +382,226 @@ def test_weights_far_below_the_largest_count(rng):
     x.q[:] = 0
     x.q[0, 0, 0] = 11.0  # a score of 11 against zeros
     close(x.run(), x.want(), x)
+
+
+@pytest.mark.parametrize("new,D", [(1, 64), (3, 64), (40, 64), (2, 128)])
+def test_nan_in_a_lone_sequences_cache(new, D, rng):
+    n = 70
+    k, v = (rng.standard_normal((n, 2, D)).astype(np.float32) for _ in range(2))
+    v[n - new, 0, 33] = np.nan  # the first new token's own
+    k[n - 1, 1, 0] = np.inf     # the last one's
+    x = Batch(rng, [n], [new], 8, 2, D, 32, k=[k], v=[v])
+    got, want = x.run(), x.want()
+    close(got, want, x)
+    assert np.isnan(got[0, 0, 32:64]).all() and np.isfinite(got[0, 0, :32]).all()
+    assert np.isnan(got[-1, 4:]).all()
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_a_lone_refused_sequence(new, rng):
+    x = Batch(rng, [100], [new], 4, 2, 128, 32)
+    assert np.isnan(x.run(max_n_keys=99)).all()
+    x.n_keys = [0]
+    assert not x.run(max_n_keys=99).any()
+
+
+@pytest.mark.parametrize("S,new", [(700, (0, 1, 1)), (300, (1, 2, 3)), (70, (60, 300))])
+def test_many_sequences(S, new, rng):
+    """More sequences, or row tiles, than a workgroup has threads."""
+    keys = rng.integers(1, 90, S)
+    news = np.minimum(rng.choice(new, S), keys)
+    keys[5], news[5] = 400, max(new)
+    x = Batch(rng, keys.tolist(), news.tolist(), 4, 2, 64, 32)
+    close(x.run(), x.want(), x)
+
+
+def test_pages_behind_four_gibibytes(rng):
+    """Slots whose bytes lie past 32 bits: append, read and both attentions."""
+    H, G, D, page = 16, 8, 128, 256
+    pb = ops.kv4_page_bytes(G, D, page)
+    P = (1 << 32) // pb + 40
+    pool = B(P * pb)
+    n = 600
+    k, v = (rng.standard_normal((n, G, D)).astype(np.float32) for _ in range(2))
+    table = np.array([P - 1, P - 37, P - 2], np.uint32)
+    slots = table[np.arange(n) // page].astype(np.int64) * page + np.arange(n) % page
+    ops.kv4_append(B.from_array(k), B.from_array(v), u32(slots), pool, n, G, D, P, page)
+    gk, gv = read_back(pool, u32(slots), n, G, D, P, page)
+    kq, vq = ref.values(*ref.quantise(k)), ref.values(*ref.quantise(v))
+    np.testing.assert_array_equal(gk, kq)
+    np.testing.assert_array_equal(gv, vq)
+    for m in (1, 20):
+        q = rng.standard_normal((m, H, D)).astype(np.float32)
+        o = filled(m * H * D)
+        ws = B(max(256, ops.kv4_attn_ws_bytes(1, m, n, H, G, D)))
+        ops.kv4_attn(B.from_array(q), pool, u32(table), u32([n]), u32([0, m]), o, 1, m, m, n, 3, H,
+                     G, D, P, page, 0, 0, ws)
+        ops.sync()
+        close(o.download(m * H * D).reshape(m, H, D), ref.attention(q, kq, vq, n), None)
+    pool.free()
+
+
+# --------------------------------------------------------------- whole steps --
+class Server:
+    """A layer of a serving loop: pool, two tables and free lists that take turns, and a
+    reference that keeps every sequence's values."""
+
+    def __init__(self, rng, S, H, G, D, page, blocks, pages, tokens, window, sinks, pairing):
+        self.__dict__.update(locals())
+        inv = oracle.rope_inv_freq(D, 1e6)
+        self.gains = [rng.normal(1, 0.1, D).astype(np.float32) for _ in range(2)]
+        self.inv = inv
+        self.dev = [B.from_array(x) for x in (*self.gains, inv)]
+        self.pool = B.from_array(rng.integers(0, 256, pages * ops.kv4_page_bytes(G, D, page),
+                                              dtype=np.uint8))
+        self.table = [u32(np.full(S * blocks, ref.NONE)) for _ in range(2)]
+        free = np.concatenate([[pages], rng.permutation(pages)])
+        self.free = [u32(free), u32(np.zeros(pages + 1))]
+        self.keys, self.new = u32(np.zeros(S)), u32(np.zeros(S))
+        self.q_off, self.lost = u32(np.zeros(S + 1)), u32([0])
+        self.pos, self.slots = u32(np.zeros(tokens)), u32(np.zeros(tokens))
+        self.plan_ws = B(ops.kv4_plan_ws_bytes(S))
+        self.raw = [B(4 * tokens * h * D) for h in (H, G, G)]
+        self.qn, self.o = filled(tokens * H * D), filled(tokens * H * D)
+        self.attn_ws = {}
+        self.k = [np.zeros((0, G, D), np.float32) for _ in range(S)]
+        self.v = [np.zeros((0, G, D), np.float32) for _ in range(S)]
+
+    def call(self, turn, max_q):
+        """The step's three calls, from table and free list `turn` to the others."""
+        S, H, G, D, page = self.S, self.H, self.G, self.D, self.page
+        T, W, N = self.tokens, self.window, self.sinks
+        ops.kv4_plan(self.keys, self.new, self.table[turn], self.table[1 - turn], self.free[turn],
+                     self.free[1 - turn], self.q_off, self.pos, self.slots, self.lost, S,
+                     self.blocks, self.pages, T, page, W, N, self.plan_ws)
+        ops.kv4_prologue(*self.raw, *self.dev, EPS, self.pairing, self.pos, self.slots, self.qn,
+                         self.pool, T, H, G, D, self.pages, page)
+        most = self.blocks * page
+        if max_q not in self.attn_ws:
+            self.attn_ws[max_q] = B(max(256, ops.kv4_attn_ws_bytes(S, max_q, most, H, G, D, W, N)))
+        ops.kv4_attn(self.qn, self.pool, self.table[1 - turn], self.keys, self.q_off, self.o, S, T,
+                     max_q, most, self.blocks, H, G, D, self.pages, page, W, N,
+                     self.attn_ws[max_q])
+
+    def lengths(self, keep, new):
+        """keep[b]: keys kept of sequence b; new[b] more follow. Uploads lengths and rows."""
+        T, D = self.tokens, self.D
+        total = int(np.sum(new))
+        raw = [self.rng.standard_normal((T, h, D)).astype(np.float32)
+               for h in (self.H, self.G, self.G)]
+        pos = np.concatenate([np.arange(a, a + m) for a, m in zip(keep, new)]).astype(np.int64)
+        at = np.concatenate([[0], np.cumsum(new)])
+        kn = raw[1][:total].copy()
+        qn = raw[0][:total].copy()
+        for t in range(total):
+            for x, g in ((qn, self.gains[0]), (kn, self.gains[1])):
+                y = oracle.rmsnorm(x[t].ravel(), g, D, x.shape[1], EPS)
+                x[t] = oracle.rope(y, 1, x.shape[1], D, int(pos[t]), self.inv,
+                                   self.pairing).reshape(-1, D)
+        for b in range(self.S):
+            s = slice(at[b], at[b + 1])
+            kq, vq = (ref.values(*ref.quantise(x[s])) for x in (kn, raw[2]))
+            self.k[b] = np.concatenate([self.k[b][:keep[b]], kq])
+            self.v[b] = np.concatenate([self.v[b][:keep[b]], vq])
+        self.at, self.q_ref = at, qn
+        self.keys.upload(np.array([len(x) for x in self.k], np.uint32))
+        self.new.upload(np.array(new, np.uint32))
+        for buf, x in zip(self.raw, raw):
+            buf.upload(x)
+
+    def check(self):
+        ops.sync()
+        total, H, D = self.at[-1], self.H, self.D
+        assert self.lost.download(1, np.uint32)[0] == 0
+        np.testing.assert_array_equal(self.qn.download(total * H * D).reshape(total, H, D),
+                                      self.q_ref)
+        got = self.o.download(total * H * D).reshape(total, H, D)
+        want = np.concatenate([ref.attention(self.q_ref[self.at[b]:self.at[b + 1]], self.k[b],
+                                             self.v[b], len(self.k[b]), self.window, self.sinks)
+                               for b in range(self.S)])
+        close(got, want, None)
+        return got
+
+
+STEPS = [([0, 0, 0, 0], [40, 0, 7, 1]),      # prompts, one sequence waits
+         ([40, 0, 7, 1], [1, 33, 1, 1]),     # a prompt beside single tokens
+         ([41, 33, 8, 2], [4, 4, 4, 4]),     # drafts
+         ([42, 37, 8, 5], [1, 1, 1, 1]),     # some of them taken back
+         ([0, 38, 9, 6], [20, 1, 0, 1]),     # one ends and another begins, one idles
+         ([20, 39, 9, 7], [1, 1, 1, 1])]
+
+
+@pytest.mark.parametrize("H,G,D,page,window,sinks,pairing", [
+    (4, 2, 128, 32, 0, 0, "neox"), (8, 2, 64, 32, 20, 3, "norm")])
+def test_a_serving_loop(H, G, D, page, window, sinks, pairing, rng):
+    s = Server(rng, 4, H, G, D, page, 4, 16, 80, window, sinks, pairing)
+    for i, (keep, new) in enumerate(STEPS):
+        s.lengths(keep, new)
+        s.call(i % 2, max(new))
+        s.check()
+
+
+def test_a_serving_loop_from_captured_graphs(rng):
+    """Two graphs take turns (from one table and free list to the other and back); each
+    is replayed several times, with eager work between, and every replay is checked."""
+    s = Server(rng, 4, 4, 2, 128, 32, 4, 16, 80, 24, 2, "neox")
+    eager = Server(np.random.default_rng(0), 2, 4, 2, 128, 32, 4, 8, 8, 0, 0, "neox")
+    stream = ops.Stream()
+    ops.set_stream(stream)
+    try:
+        graphs = []
+        for max_q in (40, 4):  # prompts, and few rows
+            for turn in range(2):
+                s.attn_ws.setdefault(max_q, B(max(256, ops.kv4_attn_ws_bytes(
+                    4, max_q, 128, 4, 2, 128, 24, 2))))
+                with ops.Graph() as g:
+                    s.call(turn, max_q)
+                graphs.append(g)
+        for i, (keep, new) in enumerate(STEPS * 2):
+            if i == len(STEPS):
+                keep = [0, 0, 0, 0]
+            s.lengths(keep, new)
+            graphs[(0 if max(new) > 4 else 2) + i % 2].launch()
+            s.check()
+            eager.lengths([0, 0], [1, 4])
+            eager.call(0, 4)
+            eager.check()
+        for g in graphs:
+            g.free()
+    finally:
+        ops.sync()
+        ops.set_stream(None)
+        stream.free()
+
+
+def test_two_streams_at_once(rng):
+    """Two batches with workspaces of their own on two streams: each one's bits are those
+    of the call alone."""
+    xs = [Batch(rng, [900, 33, 500], [m] * 3, 16, 8, 128, 64) for m in (1, 30)]
+    alone = [x.run(extra=0) for x in xs]
+    H, G, D, page, window, sinks = xs[0].shape
+    streams = [ops.Stream(), ops.Stream()]
+    held, outs = [], []
+    for x, st in zip(xs, streams):
+        m = max(x.n_new)
+        o = filled(x.T * H * D)
+        ws = B(max(256, ops.kv4_attn_ws_bytes(3, m, 900, H, G, D)))
+        held.append([B.from_array(x.q), B.from_array(x.pool), u32(x.table), u32(x.n_keys),
+                     u32(x.q_off), o, ws])
+        outs.append(o)
+    ops.sync()
+    try:
+        for _ in range(4):
+            for x, st, h in zip(xs, streams, held):
+                ops.set_stream(st)
+                ops.kv4_attn(*h[:6], 3, x.T, max(x.n_new), 900, x.M, H, G, D, x.P, page, 0, 0,
+                             h[6])
+        for st in streams:
+            ops.set_stream(st)
+            ops.sync()
+    finally:
+        ops.set_stream(None)
+    for o, want, x in zip(outs, alone, xs):
+        np.testing.assert_array_equal(o.download(x.T * H * D).reshape(x.T, H, D), want)
+    for st in streams:
+        st.free()

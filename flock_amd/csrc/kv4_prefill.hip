@@ -3,7 +3,8 @@
 // in two f16 parts, twice the plain products' work.
 //
 // A work item is 128 query-head rows of one kv head and a piece of their key tiles; four
-// waves of 32 rows, two workgroups a CU. Every 64 keys the workgroup turns the two tiles'
+// waves of 32 rows, two workgroups a CU (three of 64-wide heads, which halve LDS and the
+// accumulators: 87 us for 96 with two, seven ragged prompts). Every 64 keys the workgroup turns the two tiles'
 // codes to f16 in LDS (each code once for 128 rows), into the buffer that the step before
 // has read; the next tiles' codes are loaded meanwhile. S^T = K Q^T and O^T += V^T P^T on
 // 32x32x16: a column is a row of q, and P^T is taken from the S^T accumulators as they
@@ -17,13 +18,16 @@ namespace flk {
 typedef float floatx16v __attribute__((ext_vector_type(16)));
 
 constexpr int kPreRows = 128, kPreThreads = 256, kStep = 64;
-// Pieces of a call (over its kv heads): one for each of the two workgroups a CU that are
-// resident; with as many row tiles anyway, some more, so that the heaviest are cut. None
-// has fewer than four key tiles. us, 2048 tokens / 64 at 32768 / four prompts of 500 to
-// 1500 onto up to 3000 / 8192 tokens: 512 pieces 64 / 55.6 / 166 / 545, 640 73 / 69.7 /
+// Pieces of a call (over its kv heads): one for each workgroup that is resident; with as many
+// row tiles as two a CU anyway, some more than those, so that the heaviest are cut. None has
+// fewer than four key tiles. us, 128-wide heads, 2048 tokens / 64 at 32768 / four prompts of
+// 500 to 1500 onto up to 3000 / 8192 tokens: 512 pieces 64 / 55.6 / 166 / 545, 640 73 / 69.7 /
 // 164 / 525, 1024 74 / 73 / 179 / 559; whole row tiles cut by the call's bounds 107 / 55.7 /
-// 251 / 546.
-constexpr uint32_t kPrePieces = 512, kPreMore = 640, kPreLeast = 4;
+// 251 / 546. 64-wide, 700 tokens / 1500 onto 3000 / 4096: 512 pieces 24.2 / 137 / -, 640 25.4 /
+// 153 / 164, 768 25.4 / 117 / 171.
+template <int D>
+constexpr uint32_t kPreResident = D == 64 ? 3 : 2;  // workgroups a CU
+constexpr uint32_t kPreMany = 512, kPreMore = 640, kPreLeast = 4;
 
 // The work: row tiles, those of the last queries first (they see the most keys), each in
 // equal pieces of at most `per` key tiles where there are up to kMaxCut row tiles. As for
@@ -90,7 +94,7 @@ struct PreRegs {
 };
 
 template <int D>
-__global__ __launch_bounds__(kPreThreads, 2) void kv4_prefill_kernel(
+__global__ __launch_bounds__(kPreThreads, kPreResident<D>) void kv4_prefill_kernel(
     Kv4AttnArgs a, PrePlan plan, Kv4Part part, uint32_t* first_piece, float scale_log2e) {
   constexpr int kSteps = D / 16, kOT = D / 32;
   __shared__ PreShared<D> sh;
@@ -448,15 +452,19 @@ __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Kv4AttnArgs a, P
 }
 
 static PrePlan prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys, uint32_t n_heads,
-                            uint32_t n_kv_heads, uint32_t window, uint32_t n_sinks) {
+                            uint32_t n_kv_heads, uint32_t head_dim, uint32_t window,
+                            uint32_t n_sinks) {
   PrePlan p;
   const uint32_t group = n_heads / n_kv_heads;
   p.row_tiles = (uint32_t)(((uint64_t)max_q * group + kPreRows - 1) / kPreRows);
   const uint64_t items = (uint64_t)n_seqs * p.row_tiles;
   const uint64_t tiles = kv4_max_tiles(max_n_keys, kPreRows / group + 2, window, n_sinks);
   const uint64_t most = (tiles + kPreLeast - 1) / kPreLeast;  // pieces of a row tile
-  p.pieces = std::max(1u, kPrePieces / n_kv_heads);
-  if (items >= p.pieces) p.pieces = std::max(1u, kPreMore / n_kv_heads);
+  const uint32_t pieces =
+      items >= std::max(1u, kPreMany / n_kv_heads)
+          ? kPreMore
+          : 256 * (head_dim == 64 ? kPreResident<64> : kPreResident<128>);
+  p.pieces = std::max(1u, pieces / n_kv_heads);
   if (items > kMaxCut || most == 1) {
     p.pieces = 0;
     p.runs = (uint32_t)std::min(items, (uint64_t)0xffffffffu);
@@ -471,7 +479,8 @@ static uint64_t first_bytes() { return ws_align((kMaxCut + 1) * 4); }
 uint64_t kv4_prefill_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                               uint32_t window, uint32_t n_sinks) {
-  const PrePlan p = prefill_plan(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, window, n_sinks);
+  const PrePlan p = prefill_plan(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, head_dim,
+                                 window, n_sinks);
   if (p.pieces == 0) return 0;
   const uint64_t rows = (uint64_t)p.runs * n_kv_heads * kPreRows;
   return first_bytes() + ws_align(rows * 8) + ws_align(rows * head_dim * 4);
@@ -480,7 +489,8 @@ uint64_t kv4_prefill_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_ke
 bool kv4_prefill_fits(const Kv4AttnArgs& a) {
   const uint32_t G = a.s.n_kv_heads;
   const PrePlan p =
-      prefill_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.window, a.n_sinks);
+      prefill_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.s.head_dim, a.window,
+                   a.n_sinks);
   const uint64_t items = (uint64_t)a.n_seqs * p.row_tiles;
   const uint64_t tiles = kv4_max_tiles(a.max_n_keys, a.max_q, a.window, a.n_sinks);
   return (uint64_t)p.runs * G <= 0x7fffffffull && items <= 0x7fffffffull / G &&
@@ -491,7 +501,8 @@ template <int D>
 static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
   const uint32_t G = a.s.n_kv_heads;
   const PrePlan p =
-      prefill_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.window, a.n_sinks);
+      prefill_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.s.head_dim, a.window,
+                   a.n_sinks);
   const uint64_t grid = (uint64_t)p.runs * G, items = (uint64_t)a.n_seqs * p.row_tiles * G;
   uint32_t* first_piece = nullptr;
   Kv4Part part{};

@@ -89,10 +89,11 @@ struct Kv4Seq {
 __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, uint32_t b) {
   Kv4Seq s;
   s.q0 = min(a.q_off[b], a.n_tokens);
-  const uint32_t q1 = min(a.q_off[b + 1], a.n_tokens);
+  const uint32_t end = a.q_off[b + 1], q1 = min(end, a.n_tokens);
   s.nq = q1 > s.q0 ? q1 - s.q0 : 0;
   s.n_keys = a.n_keys[b];
-  s.refused = s.n_keys > a.max_n_keys || s.nq > a.max_q;
+  // (Of rows behind n_tokens the cache has no keys, and positions count from the last.)
+  s.refused = s.n_keys > a.max_n_keys || s.nq > a.max_q || end > a.n_tokens;
   return s;
 }
 

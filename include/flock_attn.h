@@ -345,9 +345,10 @@ int32_t flk_kv4_read(const void* pool, const uint32_t* slots, float* k, float* v
  * this step must be there already). q, o: [n_tokens][n_heads][head_dim] f32; rows
  * that no sequence has are left as they were. max_q bounds every q_off[b + 1] -
  * q_off[b], max_n_keys every n_keys[b] (at most max_blocks * page): they set the
- * launch shape, so near bounds are faster. A sequence beyond either is refused on
- * the device, as is one whose visible keys lack a page: its o rows are NaN. A row
- * that sees no key (n_keys[b] below its row count) is zeros. o may be q, but not
+ * launch shape, so near bounds are faster. A sequence beyond either, or with rows
+ * behind n_tokens, is refused on the device: its o rows are NaN, as are rows that
+ * see a key without a page. A row that sees no key (n_keys[b] below its row count)
+ * is zeros. o may be q, but not
  * lie partly over it. Sums are f32, q and the weights enter the matrix products in
  * two f16 parts (22 bits), the cache's values as they are.
  * ws: flk_kv4_attn_ws_bytes of the same arguments, 256-byte aligned; calls that

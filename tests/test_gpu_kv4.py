@@ -329,6 +329,20 @@ def test_more_rows_than_max_q_are_refused(news, rng):
     assert np.isnan(got[news[0]:]).all()
 
 
+@pytest.mark.parametrize("new", [2, 70])
+def test_sequences_with_rows_behind_the_last_are_refused(new, rng):
+    """As after a plan whose tokens did not all fit: the keys of the others are missing."""
+    x = Batch(rng, [100, 100], [new, new], 4, 2, 64, 64)
+    want, T, H, D = x.want(), 2 * new, 4, 64
+    o, ws = filled(T * H * D), B(1 << 24)
+    ops.kv4_attn(B.from_array(x.q), B.from_array(x.pool), u32(x.table), u32(x.n_keys),
+                 u32(x.q_off), o, 2, T - 1, new, 100, x.M, H, 2, D, x.P, 64, 0, 0, ws)
+    ops.sync()
+    got = o.download(T * H * D).reshape(T, H, D)
+    close(got[:new], want[:new], x)
+    assert np.isnan(got[new:-1]).all() and (got[-1] == 7).all()
+
+
 @pytest.mark.parametrize("new", [1, 4, 64])
 def test_nan_and_infinity_reach_exactly_the_rows_that_see_them(new, rng):
     """A NaN in K makes rows NaN, one in V the 32 dims of its block; rows before it,

@@ -906,6 +906,14 @@ static int32_t check_kv4(const void* pool, uint32_t n_heads, uint32_t n_kv_heads
   return check_pages(n_pages, page);
 }
 
+static int32_t check_kv4_tokens(uint32_t n_tokens, uint64_t threads) {
+  if (n_tokens == 0) return fail(FLK_ERR_ARG, "n_tokens must be >= 1, got 0");
+  if (n_tokens > kMaxGroups * 256 / threads)
+    return fail(FLK_ERR_UNSUPPORTED, "%u tokens of %llu threads exceed a launch", n_tokens,
+                (unsigned long long)threads);
+  return FLK_OK;
+}
+
 uint64_t flk_kv4_page_bytes(uint32_t n_kv_heads, uint32_t head_dim, uint32_t page) {
   if (n_kv_heads == 0 || (head_dim != 64 && head_dim != 128) ||
       (page != 32 && page != 64 && page != 128 && page != 256))
@@ -938,6 +946,9 @@ int32_t flk_kv4_plan(const uint32_t* n_keys, const uint32_t* n_new, const uint32
     return fail(FLK_ERR_ARG, "kv4_plan n_seqs=%u max_blocks=%u max_tokens=%u", n_seqs, max_blocks,
                 max_tokens);
   if (n_seqs > 65535) return fail(FLK_ERR_UNSUPPORTED, "kv4_plan n_seqs %u exceeds 65535", n_seqs);
+  if ((uint64_t)n_seqs * max_blocks > 0x7fffffffull)  // counts of blocks are 32-bit numbers
+    return fail(FLK_ERR_UNSUPPORTED, "kv4_plan: a table of %u x %u blocks exceeds 2^31", n_seqs,
+                max_blocks);
   if (overlap(free_in, 4 * (1 + (uint64_t)n_pages), free_out, 4 * (1 + (uint64_t)n_pages)))
     return fail(FLK_ERR_ARG, "kv4_plan: free_out lies over free_in");
   const uint64_t table_bytes = 4ull * n_seqs * max_blocks;
@@ -966,7 +977,7 @@ int32_t flk_kv4_prologue(const float* q_raw, const float* k_raw, const float* v_
   FLK_WORDS(slots);
   FLK_NONNULL(qn_out);
   if (int32_t rc = check_kv4(pool, n_heads, n_kv_heads, head_dim, n_pages, page)) return rc;
-  if (n_tokens == 0) return fail(FLK_ERR_ARG, "n_tokens must be >= 1, got 0");
+  if (int32_t rc = check_kv4_tokens(n_tokens, 256)) return rc;
   if (pairing != FLK_ROPE_NEOX && pairing != FLK_ROPE_NORM)
     return fail(FLK_ERR_ARG, "rope pairing %d (0 = neox, 1 = norm)", pairing);
   if (in_stride != 0 && in_stride < n_heads * head_dim)
@@ -993,7 +1004,7 @@ int32_t flk_kv4_append(const float* kn, const float* v, const uint32_t* slots, v
   FLK_NONNULL(v);
   FLK_WORDS(slots);
   if (int32_t rc = check_kv4(pool, n_kv_heads, n_kv_heads, head_dim, n_pages, page)) return rc;
-  if (n_tokens == 0) return fail(FLK_ERR_ARG, "n_tokens must be >= 1, got 0");
+  if (int32_t rc = check_kv4_tokens(n_tokens, 256)) return rc;
   Kv4AppendArgs a{};
   a.k = kn, a.v = v;
   a.kv_stride = n_kv_heads * head_dim;
@@ -1013,9 +1024,7 @@ int32_t flk_kv4_read(const void* pool, const uint32_t* slots, float* k, float* v
   FLK_ALIGNED(k);
   FLK_ALIGNED(v);
   if (int32_t rc = check_kv4(pool, n_kv_heads, n_kv_heads, head_dim, n_pages, page)) return rc;
-  if (n_tokens == 0) return fail(FLK_ERR_ARG, "n_tokens must be >= 1, got 0");
-  if ((uint64_t)n_tokens * n_kv_heads * (head_dim / 4) > 0xFFFFFFFFull * 64)
-    return fail(FLK_ERR_UNSUPPORTED, "kv4_read of %u tokens exceeds the grid", n_tokens);
+  if (int32_t rc = check_kv4_tokens(n_tokens, (uint64_t)n_kv_heads * (head_dim / 4))) return rc;
   return hip_status(launch_kv4_read(static_cast<const uint8_t*>(pool), slots, k, v, n_tokens,
                                     Kv4Shape{n_kv_heads, head_dim, n_pages, page}, g_stream),
                     "flk_kv4_read");

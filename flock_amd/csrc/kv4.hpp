@@ -24,6 +24,7 @@ namespace flk {
 
 constexpr uint32_t kKv4Tile = 32;  // tokens of a tile
 constexpr uint32_t kNoPage = 0xffffffffu;
+constexpr uint64_t kMaxGroups = 0xffffff;  // workgroups of 256 threads: a grid has 2^32 at most
 
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));

@@ -158,7 +158,7 @@ __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kerne
 #pragma unroll
     for (int i = 0; i < D / 16; i++) qf[nt][i] = src[i];
   }
-  // l: the weights' sums, from a product with ones (every element of a column the same).
+  // l: the sums of this lane's weights.
   floatx4v o[NT][kOT] = {};
   float l[NT] = {};
   float m[NT];
@@ -472,8 +472,8 @@ bool kv4_decode_fits(const Kv4AttnArgs& a) {
       decode_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.s.head_dim, a.window, a.n_sinks);
   const uint64_t tiles =
       (uint64_t)a.n_seqs * kv4_max_tiles(a.max_n_keys, a.max_q, a.window, a.n_sinks);
-  return tiles <= 0xffffffffull && (uint64_t)p.runs * G <= 0x7fffffffull &&
-         (uint64_t)a.n_seqs * a.max_q * a.n_heads <= 0x7fffffffull;
+  return tiles <= 0xffffffffull && (uint64_t)p.runs * G <= kMaxGroups &&
+         (uint64_t)a.n_seqs * a.max_q * a.n_heads <= kMaxGroups;
 }
 
 template <int D>

@@ -493,8 +493,8 @@ bool kv4_prefill_fits(const Kv4AttnArgs& a) {
                    a.n_sinks);
   const uint64_t items = (uint64_t)a.n_seqs * p.row_tiles;
   const uint64_t tiles = kv4_max_tiles(a.max_n_keys, a.max_q, a.window, a.n_sinks);
-  return (uint64_t)p.runs * G <= 0x7fffffffull && items <= 0x7fffffffull / G &&
-         (p.pieces == 0 || (items * G * kPreRows <= 0x7fffffffull && items * tiles <= 0xffffffffull));
+  return items <= kMaxGroups && (uint64_t)p.runs * G <= kMaxGroups &&
+         (p.pieces == 0 || (items * G * kPreRows <= kMaxGroups && items * tiles <= 0xffffffffull));
 }
 
 template <int D>

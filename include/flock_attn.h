@@ -309,6 +309,9 @@ uint64_t flk_kv4_page_bytes(uint32_t n_kv_heads, uint32_t head_dim, uint32_t pag
  *   lost       [1]: new tokens without a slot: no page was free (a later call with
  *     the same lengths takes what is free then), a position behind the table's
  *     last block, or a row past max_tokens. 0 when all is well.
+ * The new tokens of all sequences are below 2^32, n_seqs * max_blocks below 2^31. A
+ * page that two rows of table_in hold would go back twice: tables that share pages
+ * (flk_kv4_attn reads those too) are the caller's.
  * ws: flk_kv4_plan_ws_bytes, 256-byte aligned. */
 uint64_t flk_kv4_plan_ws_bytes(uint32_t n_seqs);
 int32_t flk_kv4_plan(const uint32_t* n_keys, const uint32_t* n_new, const uint32_t* table_in,

@@ -127,6 +127,20 @@ def test_attention_refusals(kw, code, text):
     refuse(attn_call(**kw), code, text)
 
 
+def test_calls_larger_than_a_launch_are_refused():
+    L = _lib.lib()
+    refuse(plan_call(n_seqs=65535, max_blocks=32769, table_out=FAKE), -3, "65535 x 32769")
+    refuse(plan_call(n_seqs=1, max_blocks=0xFFFFFFC1), -3, "exceeds 2^31")
+    refuse(prologue_call(n=1 << 24), -3, "16777216 tokens")
+    refuse(L.flk_kv4_append(FAKE, FAKE, FAKE, FAKE, 1 << 24, 8, 128, 4, 64), -3, "exceed")
+    refuse(L.flk_kv4_read(FAKE, FAKE, FAKE, FAKE, 1 << 24, 8, 128, 4, 64), -3, "exceed")
+    big = dict(q=FAKE, o=FAKE, max_n_keys=1 << 20, max_blocks=1 << 20)
+    for kw in (dict(n_seqs=65535, max_q=1 << 20, H=64),             # whole row tiles
+               dict(n_seqs=32, max_q=128, H=8192, G=1024),         # the merge of prompts
+               dict(n_seqs=65535, max_q=1, H=512, G=256)):          # the merge of single tokens
+        refuse(attn_call(**big, **kw), -3, "exceed a launch")
+
+
 def test_attention_workspace_queries():
     L = _lib.lib()
     for bad in ((0, 1, 1, 16, 8, 128, 0, 0), (1, 0, 1, 16, 8, 128, 0, 0),

@@ -3,9 +3,13 @@
 
 namespace flk {
 
-// Up to 16 query-head rows a kv head take the decode kernel.
+// Up to 48 query-head rows a kv head take the decode kernel, in chunks of 16: the prompt
+// kernel's 128-row tiles cost the same for a few rows as for many. us, decode kernel / prompt
+// kernel, 64 sequences of up to 16000 keys / 16 of up to 4000 / one of 131072: 16 rows 180 /
+// 762, 24 / 40.5, 35 / 78; 32 rows 326 / 745, 38 / 41.6, 53 / 79; 48 rows 481 / 819, 50 / 48.6,
+// 73 / 95; 64 rows 605 / 822, 60 / 50, 90 / 96.
 static bool few_rows(uint32_t max_q, uint32_t n_heads, uint32_t n_kv_heads) {
-  return (uint64_t)max_q * (n_heads / n_kv_heads) <= 16;
+  return (uint64_t)max_q * (n_heads / n_kv_heads) <= 48;
 }
 
 uint64_t kv4_attn_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys, uint32_t n_heads,

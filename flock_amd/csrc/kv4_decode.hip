@@ -6,7 +6,9 @@
 // 16 columns are 8 query-head rows in two f16 parts each (22 bits), so the parts
 // ride in columns that the few rows would leave empty. The cache's layout gives each
 // lane its operands in 16-byte pieces, and P^T is taken from the S^T accumulators as
-// they lie (a lane's scores are of the tokens whose values it holds).
+// they lie (a lane's scores are of the tokens whose values it holds). More than 8 rows take
+// two column tiles, more than 16 go in chunks of 16, workgroups side by side so that the
+// chunks after the first find a piece's tiles in the caches.
 #include <algorithm>
 
 #include "kv4_attn.hpp"
@@ -71,8 +73,8 @@ __device__ __forceinline__ uint32_t dec_tiles(const Kv4AttnArgs& a, const Kv4Seq
 
 template <int D, int NT>
 __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kernel(
-    Kv4AttnArgs a, Kv4Part part, uint32_t* first_piece, uint32_t pieces, uint32_t least,
-    float scale_log2e) {
+    Kv4AttnArgs a, Kv4Part part, uint32_t* first_piece, uint32_t chunks, uint32_t pieces,
+    uint32_t least, float scale_log2e) {
   constexpr int kRows = 8 * NT, kSteps = D / 32, kOT = D / 16;
   __shared__ float s_o[kDecWaves][kRows][D + 4];
   __shared__ float s_m[kDecWaves][kRows], s_l[kDecWaves][kRows];
@@ -82,7 +84,8 @@ __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kerne
   const int col = lane & 15, kg = lane >> 4;
   const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
 
-  const uint32_t kvh = blockIdx.x % G, run = blockIdx.x / G;
+  const uint32_t kvh = blockIdx.x % G, chunk = blockIdx.x / G % chunks;
+  const uint32_t run = blockIdx.x / G / chunks;
   uint32_t b = 0, piece = run, n_pieces, per;
   if (a.n_seqs == 1) {
     const uint32_t count = uniform(dec_tiles(a, kv4_seq(a, 0)));
@@ -125,14 +128,16 @@ __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kerne
     b = uniform(s_found[0]), piece = uniform(s_found[1]), n_pieces = uniform(s_found[2]);
   }
   const Kv4Seq seq = kv4_seq(a, b);
-  const uint32_t n_rows = min(seq.nq * group, (uint32_t)kRows);
-  if (seq.refused) {
-    const uint64_t rows = (uint64_t)seq.nq * group;
-    for (uint64_t i = threadIdx.x; i < rows * D; i += kDecThreads) {
-      const uint32_t r = (uint32_t)(i / D);
-      a.o[((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D + i % D] =
-          __builtin_nanf("");
-    }
+  const uint32_t rows = seq.nq * group, r0 = chunk * kRows;
+  if (r0 >= rows) return;
+  const uint32_t n_rows = min(rows - r0, (uint32_t)kRows);
+  if (seq.refused) {  // the first chunk is there for all of its rows
+    if (chunk == 0)
+      for (uint64_t i = threadIdx.x; i < (uint64_t)rows * D; i += kDecThreads) {
+        const uint32_t r = (uint32_t)(i / D);
+        a.o[((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D + i % D] =
+            __builtin_nanf("");
+      }
     return;
   }
   const int64_t first = (int64_t)seq.n_keys - seq.nq, last = (int64_t)seq.n_keys - 1;
@@ -150,7 +155,7 @@ __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kerne
   int delta[NT];  // the row's position behind the first
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
-    const uint32_t r = min((uint32_t)(8 * nt + (col >> 1)), n_rows - 1);
+    const uint32_t r = r0 + min((uint32_t)(8 * nt + (col >> 1)), n_rows - 1);
     delta[nt] = (int)(r / group);
     const float4* src = reinterpret_cast<const float4*>(
         a.q + ((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D +
@@ -380,7 +385,7 @@ __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kerne
   __syncthreads();
   const size_t slot = (size_t)blockIdx.x * kRows;
   for (uint32_t i = threadIdx.x; i < n_rows * (D / 4); i += kDecThreads) {
-    const uint32_t r = i / (D / 4), e = 4 * (i % (D / 4));
+    const uint32_t r = i / (D / 4), e = 4 * (i % (D / 4)), rr = r0 + r;
     float top = s_m[0][r];
 #pragma unroll
     for (int w = 1; w < kDecWaves; w++) top = fmaxf(top, s_m[w][r]);
@@ -399,7 +404,7 @@ __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kerne
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       f.x *= inv, f.y *= inv, f.z *= inv, f.w *= inv;
       *reinterpret_cast<float4*>(
-          a.o + ((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D + e) = f;
+          a.o + ((size_t)(seq.q0 + rr / group) * a.n_heads + kvh * group + rr % group) * D + e) = f;
     } else {
       if (e == 0) part.ml[2 * (slot + r)] = top, part.ml[2 * (slot + r) + 1] = sum;
       *reinterpret_cast<float4*>(part.acc + (slot + r) * D + e) = f;
@@ -411,7 +416,7 @@ __global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kerne
 template <int D, int kThreads>
 __global__ __launch_bounds__(kThreads) void kv4_decode_merge_kernel(Kv4AttnArgs a, Kv4Part part,
                                                                     const uint32_t* first_piece,
-                                                                    uint32_t rows,
+                                                                    uint32_t rows, uint32_t chunks,
                                                                     uint32_t slot_rows) {
   const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
   const uint32_t r = blockIdx.x % rows, item = blockIdx.x / rows, kvh = item % G, b = item / G;
@@ -420,7 +425,10 @@ __global__ __launch_bounds__(kThreads) void kv4_decode_merge_kernel(Kv4AttnArgs 
   const Kv4Seq seq = kv4_seq(a, b);
   if (r >= seq.nq * group) return;
   merge_pieces<D, kThreads>(
-      part, n, [&](uint32_t i) { return ((size_t)(p0 + i) * G + kvh) * slot_rows + r; },
+      part, n,
+      [&](uint32_t i) {
+        return (((size_t)(p0 + i) * chunks + r / slot_rows) * G + kvh) * slot_rows + r % slot_rows;
+      },
       a.o + ((size_t)(seq.q0 + r / group) * a.n_heads + kvh * group + r % group) * D);
 }
 
@@ -434,17 +442,20 @@ __global__ __launch_bounds__(kThreads) void kv4_decode_merge_kernel(Kv4AttnArgs 
 // tiles 12.1, of 20 9.6.
 constexpr uint32_t kDecPieces = 1536, kDecAlone = 512, kDecLeast = 5 * kDecWaves;
 struct DecodePlan {
-  uint32_t slot_rows;  // rows of a column tile
+  uint32_t slot_rows;  // rows of a chunk
+  uint32_t chunks;     // of a sequence's rows
   uint32_t pieces, least;
-  uint32_t runs;       // workgroups of a kv head
+  uint32_t runs;       // workgroups of a kv head and chunk
 };
 static DecodePlan decode_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                               uint32_t window, uint32_t n_sinks) {
   DecodePlan p;
-  p.slot_rows = max_q * (n_heads / n_kv_heads) <= 8 ? 8 : 16;
+  const uint32_t rows = max_q * (n_heads / n_kv_heads);
+  p.slot_rows = rows <= 8 ? 8 : 16;
+  p.chunks = (rows + p.slot_rows - 1) / p.slot_rows;
   p.least = kDecLeast;
-  p.pieces = std::max(1u, (n_seqs == 1 ? kDecAlone : kDecPieces) / n_kv_heads);
+  p.pieces = std::max(1u, (n_seqs == 1 ? kDecAlone : kDecPieces) / n_kv_heads / p.chunks);
   const uint64_t tiles = kv4_max_tiles(max_n_keys, max_q, window, n_sinks);
   const uint64_t cut = (n_seqs * tiles + p.least - 1) / p.least;  // at most, plus n_seqs
   p.runs = (uint32_t)std::min(std::min((uint64_t)p.pieces, cut) + n_seqs - 1,
@@ -454,7 +465,7 @@ static DecodePlan decode_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_ke
 
 static uint64_t first_bytes(uint32_t n_seqs) { return ws_align(((uint64_t)n_seqs + 1) * 4); }
 static uint64_t slots(const DecodePlan& p, uint32_t n_kv_heads) {
-  return (uint64_t)p.runs * n_kv_heads * p.slot_rows;
+  return (uint64_t)p.runs * p.chunks * n_kv_heads * p.slot_rows;
 }
 
 uint64_t kv4_decode_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
@@ -472,7 +483,7 @@ bool kv4_decode_fits(const Kv4AttnArgs& a) {
       decode_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.s.head_dim, a.window, a.n_sinks);
   const uint64_t tiles =
       (uint64_t)a.n_seqs * kv4_max_tiles(a.max_n_keys, a.max_q, a.window, a.n_sinks);
-  return tiles <= 0xffffffffull && (uint64_t)p.runs * G <= kMaxGroups &&
+  return tiles <= 0xffffffffull && (uint64_t)p.runs * p.chunks * G <= kMaxGroups &&
          (uint64_t)a.n_seqs * a.max_q * a.n_heads <= kMaxGroups;
 }
 
@@ -490,22 +501,22 @@ static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
   const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
   const uint32_t rows = a.max_q * (a.n_heads / G);
   const uint64_t items = (uint64_t)a.n_seqs * G;
-  const dim3 grid(p.runs * G), block(kDecThreads);
+  const dim3 grid(p.runs * p.chunks * G), block(kDecThreads);
   if (p.slot_rows == 8)
     hipLaunchKernelGGL((kv4_decode_kernel<D, 1>), grid, block, 0, st, a, part, first_piece,
-                       p.pieces, p.least, scale);
+                       p.chunks, p.pieces, p.least, scale);
   else
     hipLaunchKernelGGL((kv4_decode_kernel<D, 2>), grid, block, 0, st, a, part, first_piece,
-                       p.pieces, p.least, scale);
+                       p.chunks, p.pieces, p.least, scale);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.runs <= a.n_seqs) return e;  // no more pieces than sequences: none cut
   const dim3 mgrid((uint32_t)(items * rows));
   if (p.runs >= 8 * a.n_seqs)  // many pieces a sequence
     hipLaunchKernelGGL((kv4_decode_merge_kernel<D, 256>), mgrid, dim3(256), 0, st, a, part,
-                       first_piece, rows, p.slot_rows);
+                       first_piece, rows, p.chunks, p.slot_rows);
   else
     hipLaunchKernelGGL((kv4_decode_merge_kernel<D, 64>), mgrid, dim3(64), 0, st, a, part,
-                       first_piece, rows, p.slot_rows);
+                       first_piece, rows, p.chunks, p.slot_rows);
   return hipGetLastError();
 }
 

@@ -329,6 +329,29 @@ def test_more_rows_than_max_q_are_refused(news, rng):
     assert np.isnan(got[news[0]:]).all()
 
 
+@pytest.mark.parametrize("H,G,D,news", [
+    (16, 2, 128, (3, 1, 0, 2, 3)), (16, 2, 128, (6, 4, 1, 5, 6)), (32, 8, 64, (12, 7, 4, 0, 9)),
+    (4, 4, 128, (48, 17, 33, 1, 16)), (6, 2, 64, (7, 11, 6, 16, 5))])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 5)])
+def test_drafts_of_more_rows_than_a_chunk(H, G, D, news, window, sinks, rng):
+    keys = [max(n, k) for n, k in zip(news, (2500, 40, 700, 5, 1400))]
+    x = Batch(rng, keys, news, H, G, D, 64, window, sinks)
+    want = x.want()
+    close(x.run(), want, x)
+    close(x.run(in_place=True), want, x)
+    x.n_keys[1] = 3000  # refused: more than the call's bound
+    got = x.run(max_n_keys=2500)
+    one = slice(x.q_off[1], x.q_off[2])
+    assert np.isnan(got[one]).all()
+    got[one] = want[one]
+    close(got, want, x)
+
+
+def test_a_lone_draft_of_more_rows_than_a_chunk(rng):
+    x = Batch(rng, [5000], [5], 16, 2, 128, 128)
+    close(x.run(times=2), x.want(), x)
+
+
 @pytest.mark.parametrize("new", [2, 70])
 def test_sequences_with_rows_behind_the_last_are_refused(new, rng):
     """As after a plan whose tokens did not all fit: the keys of the others are missing."""

@@ -71,8 +71,11 @@ __device__ __forceinline__ uint32_t dec_tiles(const Kv4AttnArgs& a, const Kv4Seq
   return max(1u, kv4_tiles(pos0, (int64_t)s.n_keys - 1, a.window, a.n_sinks).count());
 }
 
+// Workgroups a CU: three as far as the registers go (D = 64 with two column tiles keeps one
+// in scratch memory for it, outside the loop: 108 us for 116 with two, 64 sequences of up to
+// 16000 keys and 16 rows; D = 128 would spill in the loop).
 template <int D, int NT>
-__global__ __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) void kv4_decode_kernel(
+__global__ __launch_bounds__(kDecThreads, NT == 1 || D == 64 ? 3 : 2) void kv4_decode_kernel(
     Kv4AttnArgs a, Kv4Part part, uint32_t* first_piece, uint32_t chunks, uint32_t pieces,
     uint32_t least, float scale_log2e) {
   constexpr int kRows = 8 * NT, kSteps = D / 32, kOT = D / 16;

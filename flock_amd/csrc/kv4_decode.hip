@@ -1,6 +1,7 @@
 // Attention of a few queries a sequence over the paged 4-bit cache (single tokens,
 // drafts), split over the keys. HBM-bound: 9/16 byte a value, each read once for the
-// query-head rows of a kv head.
+// query-head rows of a kv head. 16 / 8 heads of 128: 64 sequences of 1025 to 16385 keys 108 us
+// (5.9 TB/s) and 4.6 of merge, one of 131072 28.3 us (5.3 TB/s) and 3.8.
 //
 // A wave takes 32-key tiles. S^T = K Q^T and O^T += V^T P^T on 16x16x32 f16 MFMA: the
 // 16 columns are 8 query-head rows in two f16 parts each (22 bits), so the parts
@@ -219,8 +220,8 @@ __global__ __launch_bounds__(kDecThreads, dec_per_cu<D>(NT)) void kv4_decode_ker
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < D / 16; i++)
-      amax = fmaxf(fmaxf(fmaxf(amax, fabsf(qf[nt][i].x)), fmaxf(fabsf(qf[nt][i].y), fabsf(qf[nt][i].z))),
-                   fabsf(qf[nt][i].w));
+      amax = fmaxf(fmaxf(fmaxf(amax, fabsf(qf[nt][i].x)), fabsf(qf[nt][i].y)),
+                   fmaxf(fabsf(qf[nt][i].z), fabsf(qf[nt][i].w)));
     amax = max_xor<16>(amax);
     amax = max_xor<32>(amax);
     const RowScale rs = row_scale(amax);

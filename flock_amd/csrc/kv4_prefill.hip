@@ -1,14 +1,16 @@
 // Attention of many queries a sequence over the paged 4-bit cache (prompts, chunks).
 // MFMA-bound: f16 matrix products of the cache's exact values with q and the weights
-// in two f16 parts, twice the plain products' work.
+// in two f16 parts, twice the plain products' work. 8192 tokens, 16 / 8 heads of 128: 530 us,
+// 1037 TFLOP/s of them (a plain product of 8192 x 8192 matrices reaches 1140).
 //
 // A work item is 128 query-head rows of one kv head and a piece of their key tiles; four
 // waves of 32 rows, two workgroups a CU (three of 64-wide heads, which halve LDS and the
-// accumulators: 87 us for 96 with two, seven ragged prompts). Every 64 keys the workgroup turns the two tiles'
-// codes to f16 in LDS (each code once for 128 rows), into the buffer that the step before
-// has read; the next tiles' codes are loaded meanwhile. S^T = K Q^T and O^T += V^T P^T on
-// 32x32x16: a column is a row of q, and P^T is taken from the S^T accumulators as they
-// lie, because V's keys are put in the order in which a lane holds its scores.
+// accumulators: 87 us for 96 with two, seven ragged prompts). Every 64 keys the workgroup
+// turns the two tiles' codes to f16 in LDS (each code once for 128 rows), into the buffer that
+// the step before has read; the next tiles' codes are loaded meanwhile. S^T = K Q^T and
+// O^T += V^T P^T on 32x32x16: a column is a row of q, and P^T is taken from the S^T
+// accumulators as they lie, because V's keys are put in the order in which a lane holds its
+// scores.
 #include <algorithm>
 
 #include "kv4_attn.hpp"
@@ -53,8 +55,8 @@ __device__ __forceinline__ Kv4Tiles pre_tiles(const Kv4AttnArgs& a, const Kv4Seq
                                               uint32_t group) {
   const uint32_t r0 = rt * kPreRows, rows = seq.nq * group;
   const int64_t pos0 = (int64_t)seq.n_keys - seq.nq;
-  return kv4_tiles(pos0 + r0 / group, pos0 + (min(r0 + (uint32_t)kPreRows, rows) - 1) / group, a.window,
-                   a.n_sinks);
+  const uint32_t end = min(r0 + (uint32_t)kPreRows, rows);
+  return kv4_tiles(pos0 + r0 / group, pos0 + (end - 1) / group, a.window, a.n_sinks);
 }
 __device__ __forceinline__ uint32_t pre_count(const Kv4AttnArgs& a, const PrePlan& p, uint32_t e,
                                               uint32_t group) {
@@ -250,7 +252,8 @@ __global__ __launch_bounds__(kPreThreads, kPreResident<D>) void kv4_prefill_kern
         x.x = as_u32(kv4_pair<0>(w[i], d)), x.y = as_u32(kv4_pair<1>(w[i], d));
         x.z = as_u32(kv4_pair<2>(w[i], d)), x.w = as_u32(kv4_pair<3>(w[i], d));
         // (Slots 4 part + i, or 2 part + i % 2 of half i / 2, whose rows lie 16 keys on.)
-        const uint32_t at = D == 128 ? k_to ^ (i << 4) : (k_to ^ ((i & 1) << 4)) + (i >> 1) * 32 * D;
+        const uint32_t at =
+            D == 128 ? k_to ^ (i << 4) : (k_to ^ ((i & 1) << 4)) + (i >> 1) * 32 * D;
         *reinterpret_cast<uint4*>(&sh.k[buf][at]) = x;
       }
     }

@@ -290,6 +290,16 @@ def test_prompts(H, G, D, window, sinks, rng):
     close(x.run(), x.want(), x)
 
 
+@pytest.mark.parametrize("window,sinks", [(1, 2**32 - 1), (2**32 - 1, 2**32 - 1), (2**31, 0),
+                                          (2**31 - 1, 2**31), (40, 2**31 - 1)])
+@pytest.mark.parametrize("new", [(1, 2, 1), (70, 3, 0)])
+def test_windows_and_sinks_past_the_sequences(window, sinks, new, rng):
+    x = Batch(rng, [90, 33, 200], new, 4, 2, 64, 32, window, sinks)
+    close(x.run(), x.want(), x)
+    table = np.full((3, 7), ref.NONE, np.uint32)
+    check_plan([90, 33, 200], list(new), table, list(range(30)), 80, 30, 32, window, sinks)
+
+
 @pytest.mark.parametrize("keys,new,page", [(3000, 1, 64), (5001, 1, 128), (4100, 3, 32),
                                            (2500, 130, 64), (2049, 2049, 64)])
 def test_long_sequences(keys, new, page, rng):
@@ -467,7 +477,7 @@ def test_pages_behind_four_gibibytes(rng):
     kq, vq = ref.values(*ref.quantise(k)), ref.values(*ref.quantise(v))
     np.testing.assert_array_equal(gk, kq)
     np.testing.assert_array_equal(gv, vq)
-    for m in (1, 20):
+    for m in (1, 20, 40):  # one token, chunks of rows, the prompt kernel
         q = rng.standard_normal((m, H, D)).astype(np.float32)
         o = filled(m * H * D)
         ws = B(max(256, ops.kv4_attn_ws_bytes(1, m, n, H, G, D)))

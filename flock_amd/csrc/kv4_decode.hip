@@ -59,7 +59,7 @@ __device__ __forceinline__ void load_tile(TileRegs<D>& t, const uint8_t* base,
 // The work: each sequence's tiles in equal pieces of at most `per` tiles, a workgroup for
 // each piece and kv head. `per` comes from the batch's total on the device, so pieces are
 // as many as the GPU wants whether the lengths are equal or far apart; every workgroup
-// sums the lengths and finds its piece. A sequence of several pieces goes through the
+// sums the lengths and finds its piece (of up to 256 sequences). A sequence of several pieces goes through the
 // workspace and a merge launch.
 constexpr int kDecThreads = kDecWaves * 64;
 
@@ -72,6 +72,51 @@ __device__ __forceinline__ uint32_t dec_tiles(const Kv4AttnArgs& a, const Kv4Seq
   return max(1u, kv4_tiles(pos0, (int64_t)s.n_keys - 1, a.window, a.n_sinks).count());
 }
 
+// Pieces of a batch at `per` tiles, of_thread(per) of them this thread's, `before` in the
+// threads before it. Shortest pieces, or rounding up, may make a few more than are resident
+// together: then longer ones, in one round of the GPU (16 drafts of 5 onto up to 4000 keys:
+// 26.5 us for 30.9).
+template <int kWaves, typename OfThread>
+__device__ __forceinline__ uint32_t dec_pieces(uint32_t& per, uint32_t resident, uint32_t* s_wave,
+                                               uint32_t& before, OfThread of_thread) {
+  for (int round = 0;; round++) {
+    const uint32_t all = block_scan<kWaves>(of_thread(per), s_wave, before);
+    if (all <= resident || all - resident > resident / 2 || round == 3) return all;
+    per = max(per + 1, (uint32_t)((uint64_t)per * all / resident));
+    __syncthreads();
+  }
+}
+
+// The pieces of more sequences than a workgroup has threads, by a workgroup of a launch before:
+// in every workgroup of the attention a thread's several sequences took longer than its tiles
+// (2048 sequences of 250 to 1000 keys: 338 us for 547).
+constexpr int kItemThreads = 1024;
+__global__ __launch_bounds__(kItemThreads) void kv4_decode_items_kernel(
+    Kv4AttnArgs a, uint32_t* first_piece, uint4* items, uint32_t runs, uint32_t pieces,
+    uint32_t least, uint32_t resident) {
+  __shared__ uint32_t s_wave[2][kItemThreads / 64];
+  const uint32_t each = (a.n_seqs + kItemThreads - 1) / kItemThreads;
+  const uint32_t my_b = min(threadIdx.x * each, a.n_seqs), my_end = min(my_b + each, a.n_seqs);
+  uint32_t tiles = 0, at;
+  for (uint32_t x = my_b; x < my_end; x++) tiles += dec_tiles(a, kv4_seq(a, x));
+  uint32_t per = kv4_per(block_scan<kItemThreads / 64>(tiles, s_wave[0], at), pieces, least);
+  auto pieces_of = [&](uint32_t x, uint32_t n) { return (dec_tiles(a, kv4_seq(a, x)) + n - 1) / n; };
+  const uint32_t all =
+      dec_pieces<kItemThreads / 64>(per, resident, s_wave[1], at, [&](uint32_t n) {
+        uint32_t mine = 0;
+        for (uint32_t x = my_b; x < my_end; x++) mine += pieces_of(x, n);
+        return mine;
+      });
+  for (uint32_t x = my_b; x < my_end; x++) {
+    const uint32_t n = pieces_of(x, per);
+    first_piece[x] = at;
+    for (uint32_t i = 0; i < n && at + i < runs; i++) items[at + i] = make_uint4(x, i, n, 0);
+    at += n;
+  }
+  if (threadIdx.x == 0) first_piece[a.n_seqs] = all;
+  for (uint32_t i = all + threadIdx.x; i < runs; i += kItemThreads) items[i] = make_uint4(0, 0, 0, 0);
+}
+
 // Workgroups a CU: three as far as the registers go (D = 64 with two column tiles keeps one
 // in scratch memory for it, outside the loop: 108 us for 116 with two, 64 sequences of up to
 // 16000 keys and 16 rows; D = 128 would spill in the loop).
@@ -81,8 +126,8 @@ constexpr uint32_t dec_per_cu(int nt) {
 }
 template <int D, int NT>
 __global__ __launch_bounds__(kDecThreads, dec_per_cu<D>(NT)) void kv4_decode_kernel(
-    Kv4AttnArgs a, Kv4Part part, uint32_t* first_piece, uint32_t chunks, uint32_t pieces,
-    uint32_t least, uint32_t resident, float scale_log2e) {
+    Kv4AttnArgs a, Kv4Part part, uint32_t* first_piece, const uint4* items, uint32_t chunks,
+    uint32_t pieces, uint32_t least, uint32_t resident, float scale_log2e) {
   constexpr int kRows = 8 * NT, kSteps = D / 32, kOT = D / 16;
   __shared__ float s_o[kDecWaves][kRows][D + 4];
   __shared__ float s_m[kDecWaves][kRows], s_l[kDecWaves][kRows];
@@ -95,51 +140,33 @@ __global__ __launch_bounds__(kDecThreads, dec_per_cu<D>(NT)) void kv4_decode_ker
   const uint32_t kvh = blockIdx.x % G, chunk = blockIdx.x / G % chunks;
   const uint32_t run = blockIdx.x / G / chunks;
   uint32_t b = 0, piece = run, n_pieces, per;
-  if (a.n_seqs == 1) {
+  if (a.n_seqs > kDecThreads) {
+    const uint4 item = items[run];
+    b = uniform(item.x), piece = uniform(item.y), n_pieces = uniform(item.z);
+    if (n_pieces == 0) return;
+  } else if (a.n_seqs == 1) {
     const uint32_t count = uniform(dec_tiles(a, kv4_seq(a, 0)));
     per = kv4_per(count, pieces, least);
     n_pieces = (count + per - 1) / per;
     if (blockIdx.x == 0 && threadIdx.x == 0) first_piece[0] = 0, first_piece[1] = n_pieces;
     if (piece >= n_pieces) return;
   } else {
-    // A thread per `each` sequences.
-    const uint32_t each = (a.n_seqs + kDecThreads - 1) / kDecThreads;
-    const uint32_t my_b = min(threadIdx.x * each, a.n_seqs), my_end = min(my_b + each, a.n_seqs);
-    uint32_t count = 0, tiles = 0, at;
-    for (uint32_t x = my_b; x < my_end; x++) tiles += count = dec_tiles(a, kv4_seq(a, x));
-    per = kv4_per(block_scan<kDecWaves>(tiles, s_wave[0], at), pieces, least);
-    uint32_t mine, all;
-    // Shortest pieces, or rounding up, may make a few more than are resident together: then
-    // longer ones, in one round of the GPU (16 drafts of 5 onto up to 4000 keys: 26.5 us
-    // for 30.9).
-    for (int round = 0;; round++) {
-      mine = (count + per - 1) / per;  // of each == 1
-      if (each > 1) {
-        mine = 0;
-        for (uint32_t x = my_b; x < my_end; x++)
-          mine += (dec_tiles(a, kv4_seq(a, x)) + per - 1) / per;
-      }
-      all = block_scan<kDecWaves>(mine, s_wave[1], at);
-      if (all <= resident || all - resident > resident / 2 || round == 3) break;
-      per = max(per + 1, (uint32_t)((uint64_t)per * all / resident));
-      __syncthreads();
-    }
+    // A thread per sequence.
+    const uint32_t count = threadIdx.x < a.n_seqs ? dec_tiles(a, kv4_seq(a, threadIdx.x)) : 0;
+    uint32_t mine, all, at;
+    per = kv4_per(block_scan<kDecWaves>(count, s_wave[0], at), pieces, least);
+    all = dec_pieces<kDecWaves>(per, resident, s_wave[1], at, [&](uint32_t n) {
+      return mine = (count + n - 1) / n;
+    });
     if (blockIdx.x == 0) {  // for the merge
-      uint32_t p = at;
-      for (uint32_t x = my_b; x < my_end; x++) {
-        first_piece[x] = p;
-        if (each > 1) p += (dec_tiles(a, kv4_seq(a, x)) + per - 1) / per;
-      }
+      if (threadIdx.x < a.n_seqs) first_piece[threadIdx.x] = at;
       if (threadIdx.x == 0) first_piece[a.n_seqs] = all;
     }
     if (run >= all) return;
     if (run >= at && run < at + mine) {  // one thread
-      uint32_t x = my_b, n = mine;
-      if (each > 1)
-        while (run >= at + (n = (dec_tiles(a, kv4_seq(a, x)) + per - 1) / per)) at += n, x++;
-      s_found[0] = x;
+      s_found[0] = threadIdx.x;
       s_found[1] = run - at;
-      s_found[2] = n;
+      s_found[2] = mine;
     }
     __syncthreads();
     b = uniform(s_found[0]), piece = uniform(s_found[1]), n_pieces = uniform(s_found[2]);
@@ -485,6 +512,9 @@ static DecodePlan decode_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_ke
 }
 
 static uint64_t first_bytes(uint32_t n_seqs) { return ws_align(((uint64_t)n_seqs + 1) * 4); }
+static uint64_t item_bytes(uint32_t n_seqs, const DecodePlan& p) {
+  return n_seqs > (uint32_t)kDecThreads ? ws_align((uint64_t)p.runs * sizeof(uint4)) : 0;
+}
 static uint64_t slots(const DecodePlan& p, uint32_t n_kv_heads) {
   return (uint64_t)p.runs * p.chunks * n_kv_heads * p.slot_rows;
 }
@@ -494,7 +524,7 @@ uint64_t kv4_decode_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_key
                              uint32_t window, uint32_t n_sinks) {
   const DecodePlan p =
       decode_plan(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, head_dim, window, n_sinks);
-  return first_bytes(n_seqs) + ws_align(slots(p, n_kv_heads) * 8) +
+  return first_bytes(n_seqs) + item_bytes(n_seqs, p) + ws_align(slots(p, n_kv_heads) * 8) +
          ws_align(slots(p, n_kv_heads) * head_dim * 4);
 }
 
@@ -517,21 +547,28 @@ static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
   uint32_t* first_piece = reinterpret_cast<uint32_t*>(w);
   Kv4Part part;
   w += first_bytes(a.n_seqs);
+  uint4* items = reinterpret_cast<uint4*>(w);
+  w += item_bytes(a.n_seqs, p);
   part.ml = reinterpret_cast<float*>(w);
   part.acc = reinterpret_cast<float*>(w + ws_align(slots(p, G) * 8));
   const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
   const uint32_t rows = a.max_q * (a.n_heads / G);
-  const uint64_t items = (uint64_t)a.n_seqs * G;
   const dim3 grid(p.runs * p.chunks * G), block(kDecThreads);
+  if (a.n_seqs > (uint32_t)kDecThreads) {
+    hipLaunchKernelGGL(kv4_decode_items_kernel, dim3(1), dim3(kItemThreads), 0, st, a, first_piece,
+                       items, p.runs, p.pieces, p.least, p.resident);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   if (p.slot_rows == 8)
-    hipLaunchKernelGGL((kv4_decode_kernel<D, 1>), grid, block, 0, st, a, part, first_piece,
+    hipLaunchKernelGGL((kv4_decode_kernel<D, 1>), grid, block, 0, st, a, part, first_piece, items,
                        p.chunks, p.pieces, p.least, p.resident, scale);
   else
-    hipLaunchKernelGGL((kv4_decode_kernel<D, 2>), grid, block, 0, st, a, part, first_piece,
+    hipLaunchKernelGGL((kv4_decode_kernel<D, 2>), grid, block, 0, st, a, part, first_piece, items,
                        p.chunks, p.pieces, p.least, p.resident, scale);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.runs <= a.n_seqs) return e;  // no more pieces than sequences: none cut
-  const dim3 mgrid((uint32_t)(items * rows));
+  const dim3 mgrid(a.n_seqs * G * rows);
   if (p.runs >= 8 * a.n_seqs)  // many pieces a sequence
     hipLaunchKernelGGL((kv4_decode_merge_kernel<D, 256>), mgrid, dim3(256), 0, st, a, part,
                        first_piece, rows, p.chunks, p.slot_rows);

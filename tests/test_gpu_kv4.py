@@ -452,7 +452,8 @@ def test_a_lone_refused_sequence(new, rng):
     assert not x.run(max_n_keys=99).any()
 
 
-@pytest.mark.parametrize("S,new", [(700, (0, 1, 1)), (300, (1, 2, 3)), (70, (60, 300))])
+@pytest.mark.parametrize("S,new", [(700, (0, 1, 1)), (300, (1, 2, 3)), (2500, (0, 1, 9)),
+                                   (70, (60, 300))])
 def test_many_sequences(S, new, rng):
     """More sequences, or row tiles, than a workgroup has threads."""
     keys = rng.integers(1, 90, S)

@@ -1072,6 +1072,7 @@ int32_t flk_kv4_attn(const float* q, const void* pool, const uint32_t* table,
   a.o = o;
   a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.max_q = max_q, a.max_n_keys = max_n_keys;
   a.max_blocks = max_blocks, a.n_heads = n_heads, a.window = window, a.n_sinks = n_sinks;
+  a.q_from = 0, a.q_to = 0xffffffffu;
   a.s = Kv4Shape{n_kv_heads, head_dim, n_pages, page};
   if (!kv4_attn_fits(a))
     return fail(FLK_ERR_UNSUPPORTED,

@@ -125,6 +125,7 @@ struct Kv4AttnArgs {
   const uint32_t *table, *n_keys, *q_off;
   float* o;
   uint32_t n_seqs, n_tokens, max_q, max_n_keys, max_blocks, n_heads, window, n_sinks;
+  uint32_t q_from, q_to;  // sequences of so many rows are this launch's
   Kv4Shape s;
 };
 uint64_t kv4_attn_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys, uint32_t n_heads,

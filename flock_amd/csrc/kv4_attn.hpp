@@ -91,6 +91,7 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, uint32_t b) {
   s.q0 = min(a.q_off[b], a.n_tokens);
   const uint32_t end = a.q_off[b + 1], q1 = min(end, a.n_tokens);
   s.nq = q1 > s.q0 ? q1 - s.q0 : 0;
+  if (s.nq < a.q_from || s.nq > a.q_to) s.nq = 0;
   s.n_keys = a.n_keys[b];
   // (Of rows behind n_tokens the cache has no keys, and positions count from the last.)
   s.refused = s.n_keys > a.max_n_keys || s.nq > a.max_q || end > a.n_tokens;

@@ -357,6 +357,40 @@ def test_drafts_of_more_rows_than_a_chunk(H, G, D, news, window, sinks, rng):
     close(got, want, x)
 
 
+MIXED = ([2500, 300, 3000, 0, 2100, 60, 2400], [1, 300, 4, 0, 130, 60, 9])
+
+
+@pytest.mark.parametrize("H,G,D,page,window,sinks", [
+    (16, 8, 128, 64, 0, 0), (32, 8, 64, 32, 0, 0), (8, 1, 128, 256, 2300, 4), (3, 3, 64, 128, 0, 0)])
+def test_single_tokens_and_prompts_together(H, G, D, page, window, sinks, rng):
+    """Bounds past which a call takes both kernels."""
+    x = Batch(rng, *MIXED, H, G, D, page, window, sinks)
+    want = x.want()
+    close(x.run(), want, x)
+    close(x.run(in_place=True, times=1), want, x)
+
+
+def test_refusals_of_single_tokens_and_prompts_together(rng):
+    x = Batch(rng, *MIXED, 4, 2, 128, 64)
+    want = x.want()
+    x.table[2, 7] = ref.NONE  # of a draft
+    x.table[4, 9] = x.P + 3   # of a prompt
+    x.n_keys[6] = 2700        # both past the bound
+    x.n_keys[0] = 2699
+    got = x.run(max_q=200, max_n_keys=2600)
+    for b in (0, 1, 2, 4, 6):  # (sequence 1 has more rows than max_q; 2 more keys than the bound)
+        assert np.isnan(got[x.q_off[b]:x.q_off[b + 1]]).all(), b
+    close(got[x.q_off[5]:x.q_off[6]], want[x.q_off[5]:x.q_off[6]], x)
+
+
+def test_many_single_tokens_and_prompts_together(rng):
+    keys = rng.integers(1, 60, 400)
+    news = np.minimum(rng.choice([0, 1, 1, 1, 30], 400), keys)
+    keys[[7, 300]], news[[7, 300]] = (2500, 2200), (1, 40)
+    x = Batch(rng, keys.tolist(), news.tolist(), 4, 2, 64, 32)
+    close(x.run(), x.want(), x)
+
+
 def test_a_lone_draft_of_more_rows_than_a_chunk(rng):
     x = Batch(rng, [5000], [5], 16, 2, 128, 128)
     close(x.run(times=2), x.want(), x)

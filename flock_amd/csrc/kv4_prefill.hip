@@ -32,15 +32,29 @@ constexpr uint32_t kPreResident = D == 64 ? 3 : 2;  // workgroups a CU
 constexpr uint32_t kPreMany = 512, kPreMore = 640, kPreLeast = 4;
 
 // The work: row tiles, those of the last queries first (they see the most keys), each in
-// equal pieces of at most `per` key tiles where there are up to kMaxCut row tiles. As for
-// single tokens, `per` comes from the batch's total on the device, and every workgroup finds
-// its piece; more row tiles than that fill the GPU whole.
+// equal pieces of at most `per` key tiles. As for single tokens, `per` comes from the batch's
+// total on the device, and every workgroup finds its piece; of more than kMaxCut row tiles a
+// launch before lists them.
 constexpr uint32_t kMaxCut = kPreThreads;
+// Row tiles of up to this many key tiles (2048 keys, or a window's) are whole where there are
+// more than kMaxCut, and without a list up to twice as many. us, a workgroup for every row tile
+// that the call's bounds allow / listed whole / listed and cut: 7 prompts of up to 1500 tokens,
+// 64-wide, window 1024 (329) 88.5 / 97.5 / 100.4, 20 of up to 2000 (640) 224 / 174 / 179, 100
+// (3200) 1597 / 1496 / 1494.
+constexpr uint32_t kShortTiles = 64;
 
 struct PrePlan {
   uint32_t row_tiles;  // of a sequence, at most
   uint32_t pieces;     // that the row tiles are cut into (for a kv head); 0: whole
   uint32_t runs;       // workgroups of a kv head
+  // More row tiles than kMaxCut: a launch before lists the pieces, of row tiles with rows only.
+  bool listed;
+  uint32_t many, more;  // from `many` row tiles with rows on, `more` pieces
+  uint32_t slots, cuts; // partial results, row tiles that have them: at most
+};
+// A piece (n = 0: none) and its partial result; of a cut row tile the first of them.
+struct alignas(16) PrePiece {
+  uint32_t e, cut, n, slot;
 };
 
 // Row tile e: its sequence and place, and its key tiles (none: no rows; one at least
@@ -97,7 +111,8 @@ struct PreRegs {
 
 template <int D>
 __global__ __launch_bounds__(kPreThreads, kPreResident<D>) void kv4_prefill_kernel(
-    Kv4AttnArgs a, PrePlan plan, Kv4Part part, uint32_t* first_piece, float scale_log2e) {
+    Kv4AttnArgs a, PrePlan plan, Kv4Part part, uint32_t* first_piece, const PrePiece* list,
+    float scale_log2e) {
   constexpr int kSteps = D / 16, kOT = D / 32;
   __shared__ PreShared<D> sh;
   __shared__ uint32_t s_wave[kPreThreads / 64], s_found[3];
@@ -106,8 +121,12 @@ __global__ __launch_bounds__(kPreThreads, kPreResident<D>) void kv4_prefill_kern
   const int col = lane & 31, h = lane >> 5;
   const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
   const uint32_t kvh = blockIdx.x % G, run = blockIdx.x / G;
-  uint32_t e = run, cut = 0, n_pieces = 1;
-  if (plan.pieces > 0) {
+  uint32_t e = run, cut = 0, n_pieces = 1, piece_slot = run;
+  if (plan.listed) {
+    const uint4 x = *reinterpret_cast<const uint4*>(&list[run]);
+    e = uniform(x.x), cut = uniform(x.y), n_pieces = uniform(x.z), piece_slot = uniform(x.w);
+    if (n_pieces == 0) return;
+  } else if (plan.pieces > 0) {
     // A thread per row tile.
     const uint32_t items = a.n_seqs * plan.row_tiles;
     uint32_t at;
@@ -417,7 +436,7 @@ __global__ __launch_bounds__(kPreThreads, kPreResident<D>) void kv4_prefill_kern
   float lo, hi;
   swap_pair<32>(l, lo, hi);
   l = lo + hi;
-  const size_t at = (size_t)blockIdx.x * kPreRows + wave * 32 + col;
+  const size_t at = ((size_t)piece_slot * G + kvh) * kPreRows + wave * 32 + col;
   float* dst = n_pieces == 1 ? a.o + my_at : part.acc + at * D;
   const float inv = n_pieces > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
   if (n_pieces > 1 && h == 0) part.ml[2 * at] = m, part.ml[2 * at + 1] = l;
@@ -430,16 +449,74 @@ __global__ __launch_bounds__(kPreThreads, kPreResident<D>) void kv4_prefill_kern
                       o[c][4 * i + 3] * inv);
 }
 
+// The list. us, a 2048-token prompt at 32768 beside 31 single tokens / one of 8192: 1165 / 618;
+// in workgroups for every row tile that the call's bounds allow, whole, 3372 / 1650 (those
+// without rows are started too, and the others may meet on few CUs).
+constexpr int kListThreads = 1024;
+__device__ __forceinline__ uint32_t pre_pieces(uint32_t count, uint32_t per) {
+  return count / per + (count % per != 0);
+}
+__global__ __launch_bounds__(kListThreads) void kv4_prefill_list_kernel(Kv4AttnArgs a, PrePlan plan,
+                                                                        PrePiece* list,
+                                                                        PrePiece* cuts) {
+  constexpr int kWaves = kListThreads / 64;
+  __shared__ uint32_t s_wave[5][kWaves];
+  const uint32_t group = a.n_heads / a.s.n_kv_heads, items = a.n_seqs * plan.row_tiles;
+  const uint32_t each = (items + kListThreads - 1) / kListThreads;
+  const uint32_t e0 = min(threadIdx.x * each, items), e1 = min(e0 + each, items);
+  uint32_t tiles = 0, real = 0, at, slot, c;
+  for (uint32_t e = e0; e < e1; e++) {
+    const uint32_t n = pre_count(a, plan, e, group);
+    tiles += n, real += n > 0;
+  }
+  real = block_scan<kWaves>(real, s_wave[0], at);
+  const uint32_t pieces = real >= plan.many ? plan.more : plan.pieces;
+  uint32_t per = kv4_per(block_scan<kWaves>(tiles, s_wave[1], at), pieces, kPreLeast), all;
+  if (plan.cuts == 0) per = 0xffffffffu;
+  for (int round = 0;; round++) {  // as in the attention
+    uint32_t mine = 0;
+    for (uint32_t e = e0; e < e1; e++) mine += pre_pieces(pre_count(a, plan, e, group), per);
+    all = block_scan<kWaves>(mine, s_wave[2], at);
+    if (all <= pieces || real >= pieces || plan.cuts == 0 || round == 3) break;
+    per = max(per + 1, (uint32_t)((uint64_t)per * all / pieces));
+    __syncthreads();
+  }
+  uint32_t my_slots = 0, my_cuts = 0;
+  for (uint32_t e = e0; e < e1; e++) {
+    const uint32_t n = pre_pieces(pre_count(a, plan, e, group), per);
+    if (n > 1) my_slots += n, my_cuts++;
+  }
+  block_scan<kWaves>(my_slots, s_wave[3], slot);
+  const uint32_t n_cuts = block_scan<kWaves>(my_cuts, s_wave[4], c);
+  for (uint32_t e = e0; e < e1; e++) {
+    const uint32_t n = pre_pieces(pre_count(a, plan, e, group), per);
+    // (Rows of sequences that overlap may be more than the plan's bounds: whole then, or out.)
+    const bool cut = n > 1 && slot + n <= plan.slots && c < plan.cuts;
+    for (uint32_t i = 0; i < n && at + i < plan.runs; i++)
+      list[at + i] = cut ? PrePiece{e, i, n, slot + i} : PrePiece{e, 0, i == 0 ? 1u : 0u, 0};
+    if (cut) cuts[c] = {e, 0, n, slot};
+    at += n;
+    if (n > 1) slot += n, c++;
+  }
+  for (uint32_t i = all + threadIdx.x; i < plan.runs; i += kListThreads) list[i] = {0, 0, 0, 0};
+  for (uint32_t i = n_cuts + threadIdx.x; i < plan.cuts; i += kListThreads) cuts[i] = {0, 0, 0, 0};
+}
+
 // Joins the pieces of rows: a workgroup per row, or (FEW pieces) D / 4 threads per row, for
 // there may be many rows and nothing to join.
 template <int D, bool FEW>
 __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Kv4AttnArgs a, PrePlan plan,
                                                                 Kv4Part part,
-                                                                const uint32_t* first_piece) {
+                                                                const uint32_t* first_piece,
+                                                                const PrePiece* cuts) {
   constexpr uint32_t kRows = FEW ? 1024 / D : 1, kParts = kPreRows / kRows;
   const uint32_t G = a.s.n_kv_heads, group = a.n_heads / G;
-  const uint32_t kvh = blockIdx.x / kParts % G, e = blockIdx.x / kParts / G;
-  const uint32_t p0 = first_piece[e], n = first_piece[e + 1] - p0;
+  const uint32_t kvh = blockIdx.x / kParts % G, item = blockIdx.x / kParts / G;
+  uint32_t e = item, p0, n;
+  if (plan.listed)
+    e = cuts[item].e, p0 = cuts[item].slot, n = cuts[item].n;
+  else
+    p0 = first_piece[e], n = first_piece[e + 1] - p0;
   if (n <= 1) return;  // written by the piece itself
   const PreItem i = pre_item(a, plan, e);
   const Kv4Seq seq = kv4_seq(a, i.b);
@@ -454,80 +531,106 @@ __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Kv4AttnArgs a, P
     merge_pieces<D, 256>(part, n, at, dst);
 }
 
-static PrePlan prefill_plan(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys, uint32_t n_heads,
-                            uint32_t n_kv_heads, uint32_t head_dim, uint32_t window,
-                            uint32_t n_sinks) {
-  PrePlan p;
+// n_tokens: 0xffffffff for the workspace of any.
+static PrePlan prefill_plan(uint32_t n_seqs, uint32_t n_tokens, uint32_t max_q, uint32_t max_n_keys,
+                            uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                            uint32_t window, uint32_t n_sinks) {
+  PrePlan p{};
   const uint32_t group = n_heads / n_kv_heads;
   p.row_tiles = (uint32_t)(((uint64_t)max_q * group + kPreRows - 1) / kPreRows);
   const uint64_t items = (uint64_t)n_seqs * p.row_tiles;
   const uint64_t tiles = kv4_max_tiles(max_n_keys, kPreRows / group + 2, window, n_sinks);
   const uint64_t most = (tiles + kPreLeast - 1) / kPreLeast;  // pieces of a row tile
-  const uint32_t pieces =
-      items >= std::max(1u, kPreMany / n_kv_heads)
-          ? kPreMore
-          : 256 * (head_dim == 64 ? kPreResident<64> : kPreResident<128>);
-  p.pieces = std::max(1u, pieces / n_kv_heads);
-  if (items > kMaxCut || most == 1) {
+  const uint32_t resident = 256 * (head_dim == 64 ? kPreResident<64> : kPreResident<128>);
+  p.many = std::max(1u, kPreMany / n_kv_heads);
+  p.more = std::max(1u, kPreMore / n_kv_heads);
+  p.pieces = items < p.many || items > kMaxCut ? std::max(1u, resident / n_kv_heads) : p.more;
+  if (items > kMaxCut && (items > 2 * kMaxCut || tiles > kShortTiles)) {
+    p.listed = true;
+    // Row tiles with rows; as many pieces more as the cuts make, each cut row tile being longer
+    // than its share of the total.
+    const uint64_t real = std::min(items, (uint64_t)n_tokens * group / kPreRows + n_seqs);
+    const uint32_t pieces = std::max(p.pieces, p.more);
+    p.runs = (uint32_t)std::min(real + pieces - 1, std::min(real * most, (uint64_t)0xffffffffu));
+    p.cuts = tiles <= kShortTiles ? 0 : pieces;
+    p.slots = 2 * p.cuts;
+  } else if (most == 1 || items > kMaxCut) {
     p.pieces = 0;
-    p.runs = (uint32_t)std::min(items, (uint64_t)0xffffffffu);
+    p.runs = (uint32_t)items;
   } else {
     p.runs = (uint32_t)std::min(p.pieces + items - 1, items * most);
+    p.slots = p.runs;
   }
   return p;
 }
+static PrePlan prefill_plan(const Kv4AttnArgs& a) {
+  return prefill_plan(a.n_seqs, a.n_tokens, a.max_q, a.max_n_keys, a.n_heads, a.s.n_kv_heads,
+                      a.s.head_dim, a.window, a.n_sinks);
+}
 
-static uint64_t first_bytes() { return ws_align((kMaxCut + 1) * 4); }
+static uint64_t first_bytes(const PrePlan& p) {
+  return p.listed ? ws_align(((uint64_t)p.runs + p.cuts) * sizeof(PrePiece))
+                  : ws_align((kMaxCut + 1) * 4);
+}
 
 uint64_t kv4_prefill_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,
                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                               uint32_t window, uint32_t n_sinks) {
-  const PrePlan p = prefill_plan(n_seqs, max_q, max_n_keys, n_heads, n_kv_heads, head_dim,
-                                 window, n_sinks);
+  const PrePlan p = prefill_plan(n_seqs, 0xffffffffu, max_q, max_n_keys, n_heads, n_kv_heads,
+                                 head_dim, window, n_sinks);
   if (p.pieces == 0) return 0;
-  const uint64_t rows = (uint64_t)p.runs * n_kv_heads * kPreRows;
-  return first_bytes() + ws_align(rows * 8) + ws_align(rows * head_dim * 4);
+  const uint64_t rows = (uint64_t)p.slots * n_kv_heads * kPreRows;
+  return first_bytes(p) + ws_align(rows * 8) + ws_align(rows * head_dim * 4);
 }
 
 bool kv4_prefill_fits(const Kv4AttnArgs& a) {
   const uint32_t G = a.s.n_kv_heads;
-  const PrePlan p =
-      prefill_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.s.head_dim, a.window,
-                   a.n_sinks);
+  const PrePlan p = prefill_plan(a);
   const uint64_t items = (uint64_t)a.n_seqs * p.row_tiles;
   const uint64_t tiles = kv4_max_tiles(a.max_n_keys, a.max_q, a.window, a.n_sinks);
-  return items <= kMaxGroups && (uint64_t)p.runs * G <= kMaxGroups &&
-         (p.pieces == 0 || (items * G * kPreRows <= kMaxGroups && items * tiles <= 0xffffffffull));
+  if (items > kMaxGroups || (uint64_t)p.runs * G > kMaxGroups) return false;
+  // (Tiles of every row tile that the bounds allow, whatever q_off holds.)
+  return p.pieces == 0 || ((uint64_t)(p.listed ? p.cuts : items) * G * kPreRows <= kMaxGroups &&
+                           items * tiles <= 0xffffffffull);
 }
 
 template <int D>
 static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
   const uint32_t G = a.s.n_kv_heads;
-  const PrePlan p =
-      prefill_plan(a.n_seqs, a.max_q, a.max_n_keys, a.n_heads, G, a.s.head_dim, a.window,
-                   a.n_sinks);
-  const uint64_t grid = (uint64_t)p.runs * G, items = (uint64_t)a.n_seqs * p.row_tiles * G;
+  const PrePlan p = prefill_plan(a);
+  const uint32_t items = a.n_seqs * p.row_tiles, grid = p.runs * G;
   uint32_t* first_piece = nullptr;
+  PrePiece *cuts = nullptr, *list = nullptr;
   Kv4Part part{};
   if (p.pieces > 0) {
     uint8_t* w = static_cast<uint8_t*>(ws);
-    first_piece = reinterpret_cast<uint32_t*>(w);
-    w += first_bytes();
+    if (p.listed)
+      cuts = reinterpret_cast<PrePiece*>(w), list = cuts + p.cuts;
+    else
+      first_piece = reinterpret_cast<uint32_t*>(w);
+    w += first_bytes(p);
     part.ml = reinterpret_cast<float*>(w);
-    part.acc = reinterpret_cast<float*>(w + ws_align(grid * kPreRows * 8));
+    part.acc = reinterpret_cast<float*>(w + ws_align((uint64_t)p.slots * G * kPreRows * 8));
+  }
+  if (p.listed) {
+    hipLaunchKernelGGL(kv4_prefill_list_kernel, dim3(1), dim3(kListThreads), 0, st, a, p, list,
+                       cuts);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
   const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
-  hipLaunchKernelGGL(kv4_prefill_kernel<D>, dim3((uint32_t)grid), dim3(kPreThreads), 0, st, a, p,
-                     part, first_piece, scale);
+  hipLaunchKernelGGL(kv4_prefill_kernel<D>, dim3(grid), dim3(kPreThreads), 0, st, a, p, part,
+                     first_piece, list, scale);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.pieces == 0 || p.runs <= a.n_seqs * p.row_tiles) return e;
-  if (p.runs >= 8 * a.n_seqs * p.row_tiles)  // many pieces a row tile
-    hipLaunchKernelGGL((kv4_prefill_merge_kernel<D, false>), dim3((uint32_t)(items * kPreRows)),
-                       dim3(256), 0, st, a, p, part, first_piece);
+  const uint32_t merged = p.listed ? p.cuts : p.runs > items ? items : 0;
+  if (e != hipSuccess || p.pieces == 0 || merged == 0) return e;
+  if (!p.listed && p.runs >= 8 * items)  // many pieces a row tile
+    hipLaunchKernelGGL((kv4_prefill_merge_kernel<D, false>), dim3(merged * G * kPreRows), dim3(256),
+                       0, st, a, p, part, first_piece, cuts);
   else
     hipLaunchKernelGGL((kv4_prefill_merge_kernel<D, true>),
-                       dim3((uint32_t)(items * (kPreRows * D / 1024))), dim3(256), 0, st, a, p,
-                       part, first_piece);
+                       dim3(merged * G * (kPreRows * D / 1024)), dim3(256), 0, st, a, p, part,
+                       first_piece, cuts);
   return hipGetLastError();
 }
 

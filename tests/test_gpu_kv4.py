@@ -383,6 +383,25 @@ def test_refusals_of_single_tokens_and_prompts_together(rng):
     close(got[x.q_off[5]:x.q_off[6]], want[x.q_off[5]:x.q_off[6]], x)
 
 
+@pytest.mark.parametrize("H,G,D,window,sinks", [(8, 4, 128, 0, 0), (4, 1, 64, 0, 0),
+                                                (4, 2, 64, 700, 3)])
+def test_more_row_tiles_than_threads_some_of_them_long(H, G, D, window, sinks, rng):
+    """The pieces come from a list; the long sequences' row tiles are cut."""
+    keys, news = rng.integers(1, 700, 60), rng.choice([0, 1, 5, 40, 100, 600], 60)
+    keys[[3, 30, 59]], news[[3, 30, 59]] = (5000, 3100, 2500), (300, 64, 600)
+    news = np.minimum(news, keys)
+    x = Batch(rng, keys.tolist(), news.tolist(), H, G, D, 64, window, sinks)
+    want = x.want()
+    close(x.run(times=2), want, x)
+    close(x.run(in_place=True), want, x)
+    x.n_keys[3] = 6000  # refused
+    got = x.run(max_n_keys=5000)
+    one = slice(x.q_off[3], x.q_off[4])
+    assert np.isnan(got[one]).all()
+    got[one] = want[one]
+    close(got, want, x)
+
+
 def test_many_single_tokens_and_prompts_together(rng):
     keys = rng.integers(1, 60, 400)
     news = np.minimum(rng.choice([0, 1, 1, 1, 30], 400), keys)

@@ -17,10 +17,10 @@ static bool few_rows(uint32_t max_q, uint32_t n_heads, uint32_t n_kv_heads) {
 // A call whose sequences may be prompts and single tokens: those of up to this many queries (8
 // query-head rows, one column tile) take the decode kernel in a launch of their own, for in the
 // prompt kernel each of their workgroups would go through a long context alone. 0: one launch.
-// us, one launch / two: a 2048-token prompt with 31 single tokens of up to 16384 keys 774 / 191,
-// with another of 131072 beside them 5395 / 184; a 512-token chunk with 31 of up to 4000 138 /
-// 101, of 2000 81 / 75; with 7 of up to 8000 134 / 119, of 4000 78 / 84, of 2000 54 / 66; chunks
-// alone 5 more (113 / 118). So from contexts of more than 2048 keys on.
+// us, prompt kernel / both: a 2048-token prompt with 31 single tokens of up to 16384 keys 578 /
+// 143, with another of 131072 beside them 598 / 169; a 512-token chunk with 31 of up to 4000
+// 142 / 105, of 2000 83 / 77; with 7 of up to 8000 132 / 120, of 4000 80 / 84, of 2000 55 / 66;
+// chunks alone 5 more (113 / 118). So from contexts of more than 2048 keys on.
 constexpr uint32_t kMixedTiles = 64;
 static uint32_t mixed_q(uint32_t n_seqs, uint32_t max_n_keys, uint32_t n_heads, uint32_t n_kv_heads,
                         uint32_t window, uint32_t n_sinks) {

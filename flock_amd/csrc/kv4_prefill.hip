@@ -449,7 +449,7 @@ __global__ __launch_bounds__(kPreThreads, kPreResident<D>) void kv4_prefill_kern
                       o[c][4 * i + 3] * inv);
 }
 
-// The list. us, a 2048-token prompt at 32768 beside 31 single tokens / one of 8192: 1165 / 618;
+// The list. us, a 2048-token prompt at 32768 beside 31 single tokens / one of 8192: 1117 / 598;
 // in workgroups for every row tile that the call's bounds allow, whole, 3372 / 1650 (those
 // without rows are started too, and the others may meet on few CUs).
 constexpr int kListThreads = 1024;

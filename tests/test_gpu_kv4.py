@@ -675,6 +675,40 @@ def test_a_serving_loop_from_captured_graphs(rng):
         stream.free()
 
 
+def test_a_captured_mixed_batch_follows_its_lengths(rng):
+    """One graph (both kernels, pieces from a list) replayed as sequences shrink, grow back
+    and go: every replay against the formula."""
+    H, G, D, page = 4, 2, 64, 32
+    keys = rng.integers(200, 700, 300)
+    news = rng.choice([1, 1, 1, 70], 300)
+    keys[[9, 200]], news[[9, 200]] = (3000, 2600), (1, 200)
+    x = Batch(rng, keys.tolist(), news.tolist(), H, G, D, page)
+    o, q = filled(x.T * H * D), B.from_array(x.q)
+    ws = B(ops.kv4_attn_ws_bytes(x.S, 200, 3000, H, G, D))
+    pool, table, n_keys, q_off = B.from_array(x.pool), u32(x.table), u32(keys), u32(x.q_off)
+    stream = ops.Stream()
+    ops.set_stream(stream)
+    try:
+        with ops.Graph() as g:
+            ops.kv4_attn(q, pool, table, n_keys, q_off, o, x.S, x.T, 200, 3000, x.M, H, G, D, x.P,
+                         page, 0, 0, ws)
+        for less in (0, 100, 130, 0):
+            now = np.where(np.arange(300) % 2 == 0, keys - less, keys)
+            n_keys.upload(now.astype(np.uint32))
+            g.launch()
+            ops.sync()
+            got = o.download(x.T * H * D).reshape(x.T, H, D)
+            want = np.concatenate([
+                ref.attention(x.q[a:a + m], x.k[b][:n], x.v[b][:n], n)
+                for b, (n, m, a) in enumerate(zip(now.tolist(), x.n_new, x.q_off))])
+            close(got, want, x)
+        g.free()
+    finally:
+        ops.sync()
+        ops.set_stream(None)
+        stream.free()
+
+
 def test_two_streams_at_once(rng):
     """Two batches with workspaces of their own on two streams: each one's bits are those
     of the call alone."""

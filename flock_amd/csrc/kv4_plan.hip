@@ -26,6 +26,10 @@ struct PlanSeq {
   uint32_t keys, fresh;
   // Blocks it holds after the step: below `blocks`, and from `from` on or below `sinks`.
   uint32_t blocks, from, sinks;
+  // Blocks that may take a page: from `fresh_from` on. One before holds keys of earlier steps,
+  // which were stored nowhere if it has no page: with another's page for them, attention would
+  // read what that page held before.
+  uint32_t fresh_from;
   __device__ __forceinline__ bool wants(uint32_t i) const {
     return i < blocks && (i >= from || i < sinks);
   }
@@ -42,6 +46,7 @@ __device__ __forceinline__ PlanSeq plan_seq(const Kv4PlanArgs& a, uint32_t b) {
   s.from = a.window == 0 || first <= 0 ? 0u : (uint32_t)first >> log_page;
   s.blocks = min(blocks_of(s.keys), a.max_blocks);
   s.sinks = blocks_of(a.n_sinks);
+  s.fresh_from = blocks_of(s.keys - s.fresh);
   return s;
 }
 
@@ -49,12 +54,15 @@ __device__ __forceinline__ uint32_t plan_entry(const Kv4PlanArgs& a, uint32_t b,
   return i < a.max_blocks ? a.table_in[(size_t)b * a.max_blocks + i] : kNoPage;
 }
 
-// Of block i with entry e (an entry past the row is none).
-__device__ __forceinline__ void plan_judge(const Kv4PlanArgs& a, const PlanSeq& s, uint32_t i,
-                                           uint32_t e, bool& need, bool& drop) {
-  const bool have = e < a.n_pages, want = s.wants(i);
-  need = want && !have;
-  drop = have && !want;
+// Of block i with entry e (an entry past the row is none): whether it takes a page, gives one
+// back, or has to do without.
+struct PlanJudged {
+  bool need, drop, missing;
+};
+__device__ __forceinline__ PlanJudged plan_judge(const Kv4PlanArgs& a, const PlanSeq& s, uint32_t i,
+                                                 uint32_t e) {
+  const bool have = e < a.n_pages, want = s.wants(i), fresh = i >= s.fresh_from;
+  return {want && !have && fresh, have && !want, want && !have && !fresh};
 }
 
 __device__ __forceinline__ PlanCount plan_count(const Kv4PlanArgs& a, const PlanSeq& s,
@@ -66,10 +74,9 @@ __device__ __forceinline__ PlanCount plan_count(const Kv4PlanArgs& a, const Plan
   for (uint32_t base = 0; base < a.max_blocks; base += 64) {
     const uint32_t e = next;
     next = plan_entry(a, b, base + 64 + lane);
-    bool need, drop;
-    plan_judge(a, s, base + lane, e, need, drop);
-    c.need += __popcll(__ballot(need));
-    c.drop += __popcll(__ballot(drop));
+    const PlanJudged j = plan_judge(a, s, base + lane, e);
+    c.need += __popcll(__ballot(j.need));
+    c.drop += __popcll(__ballot(j.drop));
   }
   return c;
 }
@@ -118,7 +125,7 @@ __global__ __launch_bounds__(W * 64) void kv4_plan_kernel(Kv4PlanArgs a,
   const uint32_t b = blockIdx.x * W + wave, n_wgs = (a.n_seqs + W - 1) / W;
   const uint32_t log_page = 31 - __builtin_clz(a.page);
   if (threadIdx.x == 0) s_lost = 0;
-  PlanSeq s{0, 0, 0, 0, 0};
+  PlanSeq s{0, 0, 0, 0, 0, 0};
   PlanCount own{0, 0, 0};
   uint32_t next = kNoPage;  // the first blocks are on their way while the sums are formed
   if (b < a.n_seqs) {
@@ -160,7 +167,7 @@ __global__ __launch_bounds__(W * 64) void kv4_plan_kernel(Kv4PlanArgs a,
   }
   const uint32_t left = n_free - min(all.need, n_free);  // of the old list
 
-  uint32_t mapped = 0;  // tokens of this sequence that got a slot
+  uint32_t mapped = 0, missing = 0;  // its tokens that got a slot, its blocks that lack a page
   if (b < a.n_seqs) {
     if (lane == 0) {
       a.q_off[b] = at.fresh;
@@ -175,22 +182,24 @@ __global__ __launch_bounds__(W * 64) void kv4_plan_kernel(Kv4PlanArgs a,
       const uint32_t i = base + lane;
       uint32_t e = next;
       next = plan_entry(a, b, i + 64);
-      bool need, drop;
-      plan_judge(a, s, i, e, need, drop);
-      const uint64_t needs = __ballot(need), drops = __ballot(drop);
-      if (needs | drops) {
+      const PlanJudged j = plan_judge(a, s, i, e);
+      const uint64_t needs = __ballot(j.need), drops = __ballot(j.drop);
+      const uint64_t lacks = __ballot(j.missing);
+      if (needs | drops | lacks) {
         const uint64_t below = (1ull << lane) - 1;
-        if (drop) {
+        if (j.missing) e = kNoPage;
+        if (j.drop) {
           const uint32_t to = left + drop_at + __popcll(drops & below);
           if (to < a.n_pages) a.free_out[1 + to] = e;
           e = kNoPage;
         }
-        if (need) {
+        if (j.need) {
           const uint32_t n = need_at + __popcll(needs & below);
           e = n < n_free ? a.free_in[n_free - n] : kNoPage;  // n-th from the list's end
         }
         need_at += __popcll(needs);
         drop_at += __popcll(drops);
+        missing += __popcll(lacks);
       }
       if (i < a.max_blocks) a.table_out[(size_t)b * a.max_blocks + i] = e;
       // The new tokens that lie in these 64 blocks, block by block.
@@ -219,7 +228,8 @@ __global__ __launch_bounds__(W * 64) void kv4_plan_kernel(Kv4PlanArgs a,
       a.positions[t] = (uint32_t)x;
       a.slots[t] = kNoPage;
     }
-    if (lane == 0 && mapped != s.fresh) atomicAdd(&s_lost, s.fresh - mapped);
+    const uint32_t lost = s.fresh - mapped + missing;
+    if (lane == 0 && lost) atomicAdd(&s_lost, lost);
   }
   __syncthreads();
   if (threadIdx.x == 0) {

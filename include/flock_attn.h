@@ -294,9 +294,14 @@ uint64_t flk_kv4_page_bytes(uint32_t n_kv_heads, uint32_t head_dim, uint32_t pag
  * n_keys[b] keys after the step, the last n_new[b] of them new (at most all).
  * It holds block i after the step if i * page < n_keys[b] and, where window > 0,
  * the block has a token that its first new token sees or n_sinks covers. Blocks to
- * hold that table_in has no page for take one; pages of other blocks go back (all
- * of them for n_keys[b] = 0: a finished sequence; those past the end after tokens
- * were taken back; those that left the window).
+ * hold that table_in has no page for take one if they start with a new token; pages
+ * of other blocks go back (all of them for n_keys[b] = 0: a finished sequence; those
+ * past the end after tokens were taken back; those that left the window).
+ *   A block to hold that starts before the first new token and has no page stays
+ * without: its earlier keys were stored nowhere (no page was free in their step, or
+ * with a window the sequence was taken back behind the first new token of the step
+ * before, to keys whose pages had left it). Rows that see it are NaN, its new tokens
+ * have no slot, in every step until one in which all of the block's keys are new.
  *   free_in, free_out  [1 + n_pages]: a count, then that many free page ids. The
  *     k-th block that takes a page, in order of (sequence, block), takes the k-th
  *     from the end of free_in's list. free_out's list is what is left of it, then
@@ -307,8 +312,10 @@ uint64_t flk_kv4_page_bytes(uint32_t n_kv_heads, uint32_t head_dim, uint32_t pag
  *   positions, slots  [max_tokens], by row of q: the token's position, and its
  *     slot. Entries behind the last token: position 0, no slot.
  *   lost       [1]: new tokens without a slot: no page was free (a later call with
- *     the same lengths takes what is free then), a position behind the table's
- *     last block, or a row past max_tokens. 0 when all is well.
+ *     the same lengths takes what is free then), a block without a page as above, a
+ *     position behind the table's last block, or a row past max_tokens; and one more
+ *     for each block that stays without a page for its earlier keys. 0 when all is
+ *     well: what the step's rows see has been stored.
  * The new tokens of all sequences are below 2^32, n_seqs * max_blocks below 2^31. A
  * page that two rows of table_in hold would go back twice: tables that share pages
  * (flk_kv4_attn reads those too) are the caller's.

@@ -95,7 +95,7 @@ def plan(n_keys, n_new, table, free, max_tokens, n_pages, page, window, sinks):
     """The plan, entry by entry. free: list of page ids, the last taken first."""
     table = np.array(table, np.uint32)
     out, left, back = table.copy(), list(free), []
-    q_off, pos, slots, lost = [0], [], [], 0
+    q_off, pos, slots, missing = [0], [], [], 0
     for b in range(len(n_keys)):
         n, m = int(n_keys[b]), min(int(n_new[b]), int(n_keys[b]))
         first = max(0, n - m - window + 1)
@@ -103,7 +103,10 @@ def plan(n_keys, n_new, table, free, max_tokens, n_pages, page, window, sinks):
             want = i * page < n and (not window or (i + 1) * page > first or i * page < sinks)
             have = table[b, i] < n_pages
             if want and not have:
-                out[b, i] = left.pop() if left else NONE
+                # Keys before the new ones were stored nowhere: no page would hold them.
+                before = i * page < n - m
+                missing += before
+                out[b, i] = left.pop() if left and not before else NONE
             elif have and not want:
                 back.append(int(table[b, i]))
                 out[b, i] = NONE
@@ -114,10 +117,23 @@ def plan(n_keys, n_new, table, free, max_tokens, n_pages, page, window, sinks):
             if i < table.shape[1] and out[b, i] < n_pages:
                 s = int(out[b, i]) * page + p % page
             pos.append(p), slots.append(s)
-    lost = sum(1 for t, s in enumerate(slots) if s == NONE or t >= max_tokens)
+    lost = missing + sum(1 for t, s in enumerate(slots) if s == NONE or t >= max_tokens)
     pad = max(0, max_tokens - len(pos))
     pos, slots = (pos + [0] * pad)[:max_tokens], (slots + [NONE] * pad)[:max_tokens]
     return out, left + back, q_off, pos, slots, lost
+
+
+def dealt(n_keys, n_new, blocks, page, window, sinks):
+    """(table, q_off) of sequences that hold the blocks of a step, pages in order: as after
+    the steps before it, each key new in one of them."""
+    table = np.full((len(n_keys), blocks), NONE, np.uint32)
+    ids = iter(range(table.size))
+    for b, (n, m) in enumerate(zip(n_keys, n_new)):
+        for i in range(blocks):
+            first = max(0, n - m - window + 1)
+            if i * page < n and (not window or (i + 1) * page > first or i * page < sinks):
+                table[b, i] = next(ids)
+    return table, np.concatenate([[0], np.cumsum(n_new)]).astype(int).tolist()
 
 
 def attention(q, k, v, n_keys, window=0, sinks=0):

@@ -175,9 +175,7 @@ class Batch:
         self.n_keys, self.n_new = list(n_keys), list(n_new)
         S, M = len(n_keys), max(1, -(-max(n_keys) // page))
         self.S, self.M = S, M
-        table = np.full((S, M), ref.NONE, np.uint32)
-        table, _, self.q_off, *_ = ref.plan(n_keys, n_new, table, list(range(S * M)), 1, S * M,
-                                            page, window, sinks)
+        table, self.q_off = ref.dealt(n_keys, n_new, M, page, window, sinks)
         ids = rng.permutation(S * M).astype(np.uint32)
         self.table = np.where(table < S * M, ids[np.minimum(table, S * M - 1)], ref.NONE)
         self.P = S * M

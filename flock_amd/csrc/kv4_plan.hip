@@ -23,13 +23,9 @@ struct PlanCount {
 };
 
 struct PlanSeq {
-  uint32_t keys, fresh;
+  uint32_t keys, fresh, pos0;  // pos0: position of the first new token
   // Blocks it holds after the step: below `blocks`, and from `from` on or below `sinks`.
   uint32_t blocks, from, sinks;
-  // Blocks that may take a page: from `fresh_from` on. One before holds keys of earlier steps,
-  // which were stored nowhere if it has no page: with another's page for them, attention would
-  // read what that page held before.
-  uint32_t fresh_from;
   __device__ __forceinline__ bool wants(uint32_t i) const {
     return i < blocks && (i >= from || i < sinks);
   }
@@ -41,12 +37,12 @@ __device__ __forceinline__ PlanSeq plan_seq(const Kv4PlanArgs& a, uint32_t b) {
   PlanSeq s;
   s.keys = a.n_keys[b];
   s.fresh = min(a.n_new[b], s.keys);
+  s.pos0 = s.keys - s.fresh;
   // The earliest key that the first new token sees.
-  const int64_t first = (int64_t)s.keys - s.fresh - a.window + 1;
+  const int64_t first = (int64_t)s.pos0 - a.window + 1;
   s.from = a.window == 0 || first <= 0 ? 0u : (uint32_t)first >> log_page;
   s.blocks = min(blocks_of(s.keys), a.max_blocks);
   s.sinks = blocks_of(a.n_sinks);
-  s.fresh_from = blocks_of(s.keys - s.fresh);
   return s;
 }
 
@@ -54,15 +50,40 @@ __device__ __forceinline__ uint32_t plan_entry(const Kv4PlanArgs& a, uint32_t b,
   return i < a.max_blocks ? a.table_in[(size_t)b * a.max_blocks + i] : kNoPage;
 }
 
-// Of block i with entry e (an entry past the row is none): whether it takes a page, gives one
-// back, or has to do without.
+// A page whose block has keys that were not stored (their rows lay past max_tokens) is the
+// sequence's still, but no entry that attention reads: bit 31, the page and the first such
+// key's place in it, halved where the three take more than 32 bits (its even neighbour before
+// it then). kNoPage is none of these.
+struct PlanMark {
+  uint32_t log_page, half;
+  __device__ __forceinline__ explicit PlanMark(const Kv4PlanArgs& a)
+      : log_page(31 - __builtin_clz(a.page)), half(a.n_pages >= 0x80000000u >> log_page) {}
+  __device__ __forceinline__ uint32_t of(uint32_t id, uint32_t key) const {
+    return 0x80000000u | id << (log_page - half) | key >> half;
+  }
+  __device__ __forceinline__ uint32_t page(uint32_t e) const {
+    return (e & 0x7fffffffu) >> (log_page - half);
+  }
+  __device__ __forceinline__ uint32_t key(uint32_t e) const {
+    return (e & ((1u << (log_page - half)) - 1)) << half;
+  }
+};
+
+// Of block i with entry e (an entry past the row is none): its page, whether it takes one or
+// gives it back, and whether keys of it from before the step were stored nowhere. Such a block
+// takes no page: with another's, attention would read what that held before.
 struct PlanJudged {
+  uint32_t id;
   bool need, drop, missing;
 };
 __device__ __forceinline__ PlanJudged plan_judge(const Kv4PlanArgs& a, const PlanSeq& s, uint32_t i,
                                                  uint32_t e) {
-  const bool have = e < a.n_pages, want = s.wants(i), fresh = i >= s.fresh_from;
-  return {want && !have && fresh, have && !want, want && !have && !fresh};
+  const PlanMark mark(a);
+  const bool marked = e >= 0x80000000u;
+  const uint32_t id = marked ? mark.page(e) : e, key0 = i << mark.log_page;
+  const bool have = id < a.n_pages, want = s.wants(i);
+  const bool old = key0 + (have && marked ? mark.key(e) : 0) < s.pos0;
+  return {id, want && !have && !old, have && !want, want && old && (!have || marked)};
 }
 
 __device__ __forceinline__ PlanCount plan_count(const Kv4PlanArgs& a, const PlanSeq& s,
@@ -123,9 +144,10 @@ __global__ __launch_bounds__(W * 64) void kv4_plan_kernel(Kv4PlanArgs a,
   __shared__ uint32_t s_lost;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t b = blockIdx.x * W + wave, n_wgs = (a.n_seqs + W - 1) / W;
-  const uint32_t log_page = 31 - __builtin_clz(a.page);
+  const PlanMark mark(a);
+  const uint32_t log_page = mark.log_page;
   if (threadIdx.x == 0) s_lost = 0;
-  PlanSeq s{0, 0, 0, 0, 0, 0};
+  PlanSeq s{};
   PlanCount own{0, 0, 0};
   uint32_t next = kNoPage;  // the first blocks are on their way while the sums are formed
   if (b < a.n_seqs) {
@@ -167,13 +189,16 @@ __global__ __launch_bounds__(W * 64) void kv4_plan_kernel(Kv4PlanArgs a,
   }
   const uint32_t left = n_free - min(all.need, n_free);  // of the old list
 
-  uint32_t mapped = 0, missing = 0;  // its tokens that got a slot, its blocks that lack a page
+  // Its tokens that got a slot, its blocks that lack earlier keys.
+  uint32_t mapped = 0, missing = 0;
   if (b < a.n_seqs) {
     if (lane == 0) {
       a.q_off[b] = at.fresh;
       if (b == a.n_seqs - 1) a.q_off[a.n_seqs] = at.fresh + s.fresh;
     }
-    const uint32_t pos0 = s.keys - s.fresh;
+    const uint32_t pos0 = s.pos0;
+    // Tokens whose rows are within max_tokens.
+    const uint32_t rows = min(s.fresh, at.fresh < a.max_tokens ? a.max_tokens - at.fresh : 0);
     // Blocks that the new tokens lie in.
     const uint32_t new_from = s.fresh ? pos0 >> log_page : 0xffffffffu, new_to = s.blocks;
     uint32_t need_at = at.need, drop_at = at.drop;
@@ -185,21 +210,26 @@ __global__ __launch_bounds__(W * 64) void kv4_plan_kernel(Kv4PlanArgs a,
       const PlanJudged j = plan_judge(a, s, i, e);
       const uint64_t needs = __ballot(j.need), drops = __ballot(j.drop);
       const uint64_t lacks = __ballot(j.missing);
+      uint32_t id = j.id < a.n_pages && !j.drop && !j.missing ? j.id : kNoPage;
+      // (A block that lacks keys of its page stays marked.)
+      e = j.missing && j.id < a.n_pages ? e : id;
       if (needs | drops | lacks) {
         const uint64_t below = (1ull << lane) - 1;
-        if (j.missing) e = kNoPage;
         if (j.drop) {
           const uint32_t to = left + drop_at + __popcll(drops & below);
-          if (to < a.n_pages) a.free_out[1 + to] = e;
-          e = kNoPage;
+          if (to < a.n_pages) a.free_out[1 + to] = j.id;
         }
         if (j.need) {
           const uint32_t n = need_at + __popcll(needs & below);
-          e = n < n_free ? a.free_in[n_free - n] : kNoPage;  // n-th from the list's end
+          e = id = n < n_free ? a.free_in[n_free - n] : kNoPage;  // n-th from the list's end
         }
         need_at += __popcll(needs);
         drop_at += __popcll(drops);
         missing += __popcll(lacks);
+      }
+      if (rows < s.fresh && id < a.n_pages) {  // which of them are not stored
+        const uint32_t key0 = i << log_page, from = max(pos0 + rows, key0);
+        if (from - key0 < a.page) e = mark.of(id, from - key0);
       }
       if (i < a.max_blocks) a.table_out[(size_t)b * a.max_blocks + i] = e;
       // The new tokens that lie in these 64 blocks, block by block.
@@ -208,7 +238,7 @@ __global__ __launch_bounds__(W * 64) void kv4_plan_kernel(Kv4PlanArgs a,
       for (uint32_t blk = max(base, new_from); blk < blk_end; blk++) {
         const uint32_t p = max(blk << log_page, pos0);
         const uint32_t n = min(a.page - (p & (a.page - 1)), s.keys - p);
-        const uint32_t page_id = __shfl((int)e, (int)(blk - base), kWave);
+        const uint32_t page_id = __shfl((int)id, (int)(blk - base), kWave);
         const bool ok = page_id < a.n_pages;
         const uint64_t row = (uint64_t)at.fresh + (p - pos0);
 #pragma unroll 1

@@ -302,20 +302,27 @@ uint64_t flk_kv4_page_bytes(uint32_t n_kv_heads, uint32_t head_dim, uint32_t pag
  * with a window the sequence was taken back behind the first new token of the step
  * before, to keys whose pages had left it). Rows that see it are NaN, its new tokens
  * have no slot, in every step until one in which all of the block's keys are new.
+ *   Tokens whose rows lie past max_tokens are stored nowhere either: from the first
+ * of them on a sequence's blocks keep their pages, but as marked entries, with the
+ * same consequences, until a step in which that token and those behind it are new
+ * (the same lengths again with more rows, or a step that goes on from it).
  *   free_in, free_out  [1 + n_pages]: a count, then that many free page ids. The
  *     k-th block that takes a page, in order of (sequence, block), takes the k-th
  *     from the end of free_in's list. free_out's list is what is left of it, then
  *     the pages that went back, in the same order: they can be taken in the next
  *     step. The two may not overlap (a caller keeps two and swaps them).
- *   table_out  may be table_in. Entries without a page are 0xffffffff.
+ *   table_out  may be table_in. Entries without a page are 0xffffffff, marked ones
+ *     2^31 + (page id * page + place in the page of the first key not stored), the
+ *     sum halved from n_pages * page = 2^31 on. Neither is a page to flk_kv4_attn; a
+ *     table that the caller writes holds page ids and 0xffffffff.
  *   q_off      [n_seqs + 1] as above
  *   positions, slots  [max_tokens], by row of q: the token's position, and its
  *     slot. Entries behind the last token: position 0, no slot.
  *   lost       [1]: new tokens without a slot: no page was free (a later call with
- *     the same lengths takes what is free then), a block without a page as above, a
- *     position behind the table's last block, or a row past max_tokens; and one more
- *     for each block that stays without a page for its earlier keys. 0 when all is
- *     well: what the step's rows see has been stored.
+ *     the same lengths takes what is free then), a block without a page or marked as
+ *     above, a position behind the table's last block, or a row past max_tokens; and
+ *     one more for each block to hold that lacks keys from before the step. 0 when all
+ *     is well: what the step's rows see is stored once its prologue has run.
  * The new tokens of all sequences are below 2^32, n_seqs * max_blocks below 2^31. A
  * page that two rows of table_in hold would go back twice: tables that share pages
  * (flk_kv4_attn reads those too) are the caller's.

@@ -91,31 +91,53 @@ def load(pool, page):
         return one(kb, ksh, ks), one(vb, vsh, vs)
 
 
+def mark(page_id, key, n_pages, page):
+    """The entry of a page whose block's keys from its `key`-th on were not stored."""
+    half = n_pages * page >= 1 << 31
+    return 1 << 31 | page_id * (page >> half) | key >> half
+
+
+def unmark(entry, n_pages, page):
+    """(page id, or n_pages or more for none; the first of its keys that was not stored)"""
+    if entry < 1 << 31:
+        return entry, page
+    half = n_pages * page >= 1 << 31
+    page_id, key = divmod(entry - (1 << 31), page >> half)
+    return page_id, key << half
+
+
 def plan(n_keys, n_new, table, free, max_tokens, n_pages, page, window, sinks):
     """The plan, entry by entry. free: list of page ids, the last taken first."""
     table = np.array(table, np.uint32)
-    out, left, back = table.copy(), list(free), []
+    out, left, back = np.full_like(table, NONE), list(free), []
     q_off, pos, slots, missing = [0], [], [], 0
     for b in range(len(n_keys)):
         n, m = int(n_keys[b]), min(int(n_new[b]), int(n_keys[b]))
         first = max(0, n - m - window + 1)
+        stored = n - m + min(m, max(0, max_tokens - q_off[-1]))
+        ids = [NONE] * table.shape[1]
         for i in range(table.shape[1]):
             want = i * page < n and (not window or (i + 1) * page > first or i * page < sinks)
-            have = table[b, i] < n_pages
-            if want and not have:
+            page_id, key = unmark(int(table[b, i]), n_pages, page)
+            have = page_id < n_pages
+            if have and not want:
+                back.append(page_id)
+            elif want and i * page + (key if have else 0) < n - m and (not have or key < page):
                 # Keys before the new ones were stored nowhere: no page would hold them.
-                before = i * page < n - m
-                missing += before
-                out[b, i] = left.pop() if left and not before else NONE
-            elif have and not want:
-                back.append(int(table[b, i]))
-                out[b, i] = NONE
+                missing += 1
+                if have:
+                    out[b, i] = table[b, i]
+            elif want:
+                ids[i] = page_id if have else left.pop() if left else NONE
+                out[b, i] = ids[i]
+                if stored < n and (i + 1) * page > stored and ids[i] < n_pages:
+                    out[b, i] = mark(ids[i], max(0, stored - i * page), n_pages, page)
         q_off.append(q_off[-1] + m)
         for p in range(n - m, n):
             i = p // page
             s = NONE
-            if i < table.shape[1] and out[b, i] < n_pages:
-                s = int(out[b, i]) * page + p % page
+            if i < len(ids) and ids[i] < n_pages:
+                s = ids[i] * page + p % page
             pos.append(p), slots.append(s)
     lost = missing + sum(1 for t, s in enumerate(slots) if s == NONE or t >= max_tokens)
     pad = max(0, max_tokens - len(pos))

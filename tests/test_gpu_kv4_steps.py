@@ -26,8 +26,9 @@ class Losing(Server):
             keys, new, self.want_table, self.want_free, self.tokens, self.pages, self.page,
             self.window, self.sinks)
 
-    def check(self, turn, new):
+    def check(self, turn, new, limit=None):
         """Returns, for each sequence, whether its rows are numbers."""
+        limit = limit or self.tokens
         ops.sync()
         H, D = self.H, self.D
         np.testing.assert_array_equal(
@@ -47,15 +48,22 @@ class Losing(Server):
                     seen &= (j > p - self.window) | (j < self.sinks)
                 if not there[seen].all():
                     want[i] = np.nan
+            refused = self.at[b + 1] > limit
+            if refused:
+                want = np.full((max(0, limit - self.at[b]), H, D), np.nan)
+                rows = slice(self.at[b], self.at[b] + len(want))
             close(got[rows], want, None)
-            numbers.append(bool(np.isfinite(want).all()) if m else None)
+            numbers.append(bool(np.isfinite(want).all()) and not refused if m else None)
         return numbers
 
-    def step(self, turn, keep, new, max_q):
+    def step(self, turn, keep, new, max_q, limit=None):
+        """limit: rows of the step's arrays."""
         self.lengths(keep, new)
+        whole, self.tokens = self.tokens, limit or self.tokens
         self.expect(new)
         self.call(turn, max_q)
-        return self.check(turn, new)
+        self.tokens = whole
+        return self.check(turn, new, limit)
 
 
 # (kept keys, new ones), and whose rows are numbers.
@@ -74,6 +82,26 @@ BACK = [([0, 0], [70, 40], [True, True]), ([70, 40], [1, 1], [True, True]),
         ([71, 45], [3, 1], [False, True]), ([74, 46], [22, 0], [False, None]),
         ([96, 46], [31, 1], [True, True]),  # keys from 65 on, in the block that it still had
         ([127, 47], [1, 1], [True, True])]
+
+
+# ... and the rows of the step's arrays.
+OVER = [([0, 0, 0], [40, 33, 20], [True, True, True], 93),
+        ([40, 33, 20], [1, 1, 1], [True, True, False], 2),
+        ([41, 34, 21], [1, 2, 1], [True, True, False], 4),   # past the one that was not stored
+        ([42, 36, 0], [30, 30, 22], [True, False, False], 55),
+        ([72, 66, 22], [1, 1, 0], [True, False, None], 2),
+        ([72, 32, 0], [2, 5, 24], [True, True, True], 31),
+        ([74, 37, 24], [1, 30, 1], [True, False, False], 12),
+        ([75, 48, 24], [0, 30, 1], [None, True, True], 31),  # from the first not stored on
+        ([75, 78, 25], [1, 1, 1], [True, True, True], 3)]
+
+
+@pytest.mark.parametrize("H,G,D", [(4, 2, 128), (8, 2, 64)])
+@pytest.mark.parametrize("rows", ["few", "many"])
+def test_tokens_past_the_arrays_are_not_seen(H, G, D, rows, rng):
+    s = Losing(rng, 3, H, G, D, 32, 8, 24, 120, 0, 0, "neox")
+    for i, (keep, new, want, limit) in enumerate(OVER):
+        assert s.step(i % 2, keep, new, max(new) if rows == "few" else 120, limit) == want, i
 
 
 @pytest.mark.parametrize("H,G,D", [(4, 2, 128), (8, 2, 64)])
@@ -131,3 +159,32 @@ def test_plans_that_run_dry_equal_the_reference(S, M, window, sinks, rng):
                                             sinks, in_place=step % 2 == 1)
         lost += count
     assert lost > 0
+
+
+@pytest.mark.parametrize("S,M", [(1, 4), (16, 70), (17, 5), (1300, 3)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
+def test_plans_of_more_tokens_than_rows_equal_the_reference(S, M, window, sinks, rng):
+    page, n_pages = 32, S * M + 1
+    table = np.full((S, M), ref.NONE, np.uint32)
+    free = rng.permutation(n_pages).tolist()
+    keys, marked = np.zeros(S, np.int64), 0
+    for step in range(8):
+        new = rng.choice([0, 1, 4, page, M * page // 2], S)
+        keys = np.minimum(np.where(rng.random(S) < 0.1, 0, keys + new), M * page + 5)
+        new = np.minimum(new, keys)
+        tokens = max(1, int(new.sum() * (1, 0.4, 0.9)[step % 3]) - step % 2)
+        table, free, *_ = check_plan(keys, new, table, free, tokens, n_pages, page, window, sinks,
+                                     in_place=step % 2 == 1)
+        marked += ((table >= 1 << 31) & (table != ref.NONE)).sum()
+    assert S == 1 or marked > 0
+
+
+def test_marks_of_a_pool_of_more_than_two_to_the_31_slots():
+    n_pages, table = 1 << 26, np.full((2, 3), ref.NONE, np.uint32)
+    free = [5, n_pages - 2, 0, n_pages - 1, 77]
+    for keys, new, tokens, want in (([70, 20], [70, 20], 41, 49),
+                                    ([70, 25], [29, 25], 54, 24),  # of 41 its even neighbour
+                                    ([71, 26], [31, 1], 32, 0), ([72, 27], [1, 1], 2, 0)):
+        table, free, _, _, _, lost = check_plan(keys, new, table, free, tokens, n_pages, 32, 0, 0)
+        assert lost == want
+    assert free == [5] and table[0].tolist() == [77, n_pages - 1, 0]

@@ -29,7 +29,8 @@ class Slots:
         self.steps += 1
         self.table, self.free, q_off, pos, slots, self.lost = ref.plan(
             keys, new, self.table, self.free, T, self.n_pages, page, self.window, self.sinks)
-        held = self.table[self.table < self.n_pages].tolist() + self.free
+        ids = [ref.unmark(int(e), self.n_pages, page)[0] for e in self.table.ravel()]
+        held = [e for e in ids if e < self.n_pages] + self.free
         assert sorted(held) == list(range(self.n_pages)), "a page lost, or twice"
         for b in range(S):
             for i in range(new[b]):
@@ -130,6 +131,68 @@ def test_random_steps_read_only_what_was_stored(seed):
             b = int(rng.integers(0, S))
             new[b] = keys[b]
         got = s.step(keys.tolist(), new.tolist())
+        numbers += sum(x is True for x in got)
+        if s.lost == 0:
+            assert False not in got
+    assert numbers > 0
+
+
+@pytest.mark.parametrize("n_pages,page", [(1, 32), (100, 256), ((1 << 26) - 1, 32), (1 << 26, 32),
+                                          ((1 << 27) - 1, 32), ((1 << 24) - 1, 256)])
+def test_marks_of_pages_are_no_pages_and_come_back(n_pages, page):
+    assert ref.unmark(ref.NONE, n_pages, page)[0] >= n_pages
+    for page_id in {0, n_pages // 3, n_pages // 2, n_pages - 1}:
+        for key in range(page):
+            e = ref.mark(page_id, key, n_pages, page)
+            got = ref.unmark(e, n_pages, page)
+            assert n_pages <= e < ref.NONE and got[0] == page_id
+            assert got[1] == (key & ~1 if n_pages * page >= 1 << 31 else key)
+
+
+def test_rows_past_the_arrays_leave_nothing_to_be_read():
+    s = Slots(2, 4, 32, 8)
+    s.step([40, 40], [40, 40])
+    assert s.step([41, 41], [1, 1], max_tokens=1) == [True, None] and s.lost == 1
+    assert s.step([42, 42], [1, 1]) == [True, False] and s.lost > 0
+    assert s.step([43, 43], [1, 2]) == [True, False] and s.lost > 0
+    assert s.step([44, 44], [1, 4]) == [True, True] and s.lost == 0  # from the lost one on
+
+
+def test_rows_past_the_arrays_planned_again():
+    s = Slots(2, 4, 32, 8)
+    s.step([40, 40], [40, 40])
+    assert s.step([75, 75], [35, 35], max_tokens=50) == [True, None] and s.lost == 20
+    assert s.step([75, 75], [0, 35]) == [None, True] and s.lost == 0
+
+
+def test_a_prompt_past_the_arrays_goes_on_from_what_was_stored():
+    s = Slots(1, 4, 32, 4)
+    assert s.step([100], [100], max_tokens=70) == [None] and s.lost == 30
+    assert s.step([100], [30]) == [True] and s.lost == 0
+    s = Slots(1, 4, 32, 4)
+    assert s.step([100], [100], max_tokens=70) == [None]
+    assert s.step([101], [30]) == [False] and s.lost > 0  # one was left out
+    s = Slots(1, 4, 32, 4)
+    assert s.step([100], [100], max_tokens=70) == [None]
+    assert s.step([65], [1]) == [True] and s.step([66], [1]) == [True] and s.lost == 0
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_random_steps_of_more_tokens_than_rows(seed):
+    rng = np.random.default_rng(100 + seed)
+    S, M, page = int(rng.integers(1, 6)), int(rng.integers(1, 7)), 32
+    window, sinks = (0, 0) if seed % 2 else (int(rng.integers(1, 90)), int(rng.integers(0, 50)))
+    s = Slots(S, M, page, int(rng.integers(S * M // 2 + 1, S * M + 2)), window, sinks)
+    keys = np.zeros(S, int)
+    numbers = 0
+    for _ in range(80):
+        new = rng.choice([0, 1, 1, 5, 33], S)
+        keys = np.where(rng.random(S) < 0.1, 0, keys) + new
+        fit = keys <= M * page
+        new, keys = np.where(fit, new, 0), np.where(fit, keys, 0)
+        short = rng.random() < 0.3
+        got = s.step(keys.tolist(), new.tolist(),
+                     max(1, int(new.sum()) - int(rng.integers(1, 40))) if short else None)
         numbers += sum(x is True for x in got)
         if s.lost == 0:
             assert False not in got

@@ -7,7 +7,7 @@ import pytest
 
 import kv4_ref as ref
 from flock_amd import ops
-from test_gpu_kv4 import B, Server, check_plan, close
+from test_gpu_kv4 import B, Batch, Server, check_plan, close, u32
 
 pytestmark = pytest.mark.gpu
 
@@ -188,3 +188,49 @@ def test_marks_of_a_pool_of_more_than_two_to_the_31_slots():
         table, free, _, _, _, lost = check_plan(keys, new, table, free, tokens, n_pages, 32, 0, 0)
         assert lost == want
     assert free == [5] and table[0].tolist() == [77, n_pages - 1, 0]
+
+
+def test_a_captured_mixed_batch_as_sequences_end_begin_and_change(rng):
+    """One graph (both kernels, pieces from lists) whose lengths and rows all change: sequences
+    end and come back, prompts become single tokens and single tokens prompts, row tiles that
+    were cut are whole and cut again. Rows of no sequence stay as they were."""
+    H, G, D, page, S, T = 4, 2, 64, 32, 300, 6000
+    most = rng.integers(80, 500, S)
+    most[[9, 200, 250]] = 3000, 2600, 2200
+    x = Batch(rng, most.tolist(), [1] * S, H, G, D, page)
+    q = rng.standard_normal((T, H, D)).astype(np.float32)
+    dq, o = B.from_array(q), B(4 * T * H * D)
+    ws = B(ops.kv4_attn_ws_bytes(S, 200, 3000, H, G, D))
+    pool, table, n_keys, q_off = B.from_array(x.pool), u32(x.table), u32(most), u32([0] * (S + 1))
+    stream = ops.Stream()
+    ops.set_stream(stream)
+    try:
+        with ops.Graph() as g:
+            ops.kv4_attn(dq, pool, table, n_keys, q_off, o, S, T, 200, 3000, x.M, H, G, D, x.P,
+                         page, 0, 0, ws)
+        for i in range(5):
+            keys = np.where(rng.random(S) < 0.2, 0, most - rng.integers(0, 80, S))
+            news = np.minimum(rng.choice([0, 1, 1, 1, 1, 1, 2, 2, 40, 70], S), keys)
+            if i % 2 == 0:  # a long prompt, a chunk and a single token, all far on
+                keys[[9, 200, 250]] = most[[9, 200, 250]]
+                news[[9, 200, 250]] = (1, 200, 64) if i < 4 else (200, 1, 64)
+            else:
+                keys[[9, 200, 250]], news[[9, 200, 250]] = (90, 2000, 0), (70, 1, 0)
+            off = np.concatenate([[0], np.cumsum(news)])
+            assert off[-1] < T
+            n_keys.upload(keys.astype(np.uint32))
+            q_off.upload(off.astype(np.uint32))
+            o.upload(np.full(T * H * D, 7, np.float32))
+            g.launch()
+            ops.sync()
+            got = o.download(T * H * D).reshape(T, H, D)
+            want = np.concatenate([
+                ref.attention(q[a:a + m], x.k[b][:n], x.v[b][:n], n)
+                for b, (n, m, a) in enumerate(zip(keys.tolist(), news.tolist(), off.tolist()))])
+            assert (got[off[-1]:] == 7).all()
+            close(got[:off[-1]], want, x)
+        g.free()
+    finally:
+        ops.sync()
+        ops.set_stream(None)
+        stream.free()

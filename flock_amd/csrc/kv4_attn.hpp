@@ -65,9 +65,10 @@ __device__ __forceinline__ halfx2 rest_half2(float a, float b, halfx2 hi, float 
   return pack_half2(mix_fma<0>(hi, s, a), mix_fma<1>(hi, s, b));
 }
 
-// A power of two that brings a row's largest |q| to 2^14 .. 2^15, and its inverse:
-// the row's two f16 parts then hold 22 bits of every element down to 2^-39 of the
-// largest. Rows below 2^-97 keep the largest factor (their scores are 0 next to 1);
+// A power of two that brings a row's largest |q| to 2^14 .. 2^15, and its inverse. Two f16
+// parts are off by at most 2^-23 of an element from 2^-2 on (2^-16 of the largest at most),
+// and by 2^-25, half of the second part's last subnormal bit, of smaller ones: 2^-39 of the
+// largest, which is what counts in a sum over the row. Rows below 2^-97 keep the largest factor (their scores are 0 next to 1);
 // infinities stay infinite, and their second part is NaN.
 struct RowScale {
   float up, down;
@@ -77,9 +78,11 @@ __device__ __forceinline__ RowScale row_scale(float amax) {
   return {__builtin_bit_cast(float, (268u - e) << 23), __builtin_bit_cast(float, (e - 14u) << 23)};
 }
 
-// Weights are exp2(score - reference + kBias), at most 2^15: the second parts of
-// weights down to 2^-14 of the largest are then normal f16 numbers. The reference
-// moves when a score passes it by more than kSlack.
+// Weights are exp2(score - reference + kBias): 2^10 for the reference's own key, at most 2^15.
+// Two f16 parts are off by at most 2^-23 of a weight down to 2^-12 of the largest (as above,
+// from 2^-2 on), and by 2^-25, which is 2^-35 of the largest, below: n keys of them by n 2^-35
+// of the largest |v|, also where their scores are equal and the errors do not average out
+// (2^20 keys: 3e-5). The reference moves when a score passes it by more than kSlack.
 constexpr float kBias = 10.f, kSlack = 5.f;
 
 struct Kv4Seq {

@@ -234,3 +234,30 @@ def test_a_captured_mixed_batch_as_sequences_end_begin_and_change(rng):
         ops.sync()
         ops.set_stream(None)
         stream.free()
+
+
+@pytest.mark.parametrize("below", [17.3, 20.5, 26.3])
+@pytest.mark.parametrize("H,m", [(1, 1), (8, 7)])  # the kernel for few rows, and for prompts
+def test_a_million_equal_weights_far_below_the_largest(below, H, m):
+    """A key of weight 1 and value 0, and 2^20 of weight 2^-below and value 1. Weights are held
+    as 2^10 and less in two f16 parts, the second of them to half of 2^-24: 2^-35 of the largest
+    for each key. 1e-5 for the rest (see close)."""
+    n, D, page = 1 << 20, 64, 256
+    k, v = np.zeros((n, 1, D), np.float32), np.ones((n, 1, D), np.float32)
+    k[0, 0, 0], v[0] = 8, 0
+    q = np.zeros((m, H, D), np.float32)
+    q[..., 0] = below * np.log(2)  # over sqrt(64), times 8
+    P = n // page
+    pool, ids = B(P * ops.kv4_page_bytes(1, D, page)), u32(np.arange(P))
+    slots, dk, dv = u32(np.arange(n)), B.from_array(k), B.from_array(v)
+    ops.kv4_append(dk, dv, slots, pool, n, 1, D, P, page)
+    o, ws = B(4 * q.size), B(ops.kv4_attn_ws_bytes(1, m, n, H, 1, D))
+    ops.kv4_attn(B.from_array(q), pool, ids, u32([n]), u32([0, m]), o, 1, m, m, n, P, H, 1, D, P,
+                 page, 0, 0, ws)
+    ops.sync()
+    got = o.download(q.size).reshape(m, H * D).astype(np.float64)
+    weight = np.exp(-q[0, 0, 0].astype(np.float64))
+    for i in range(m):
+        others = n - m + i
+        want = others * weight / (1 + others * weight)
+        assert np.abs(got[i] - want).max() <= others * 2.0 ** -35 + 1e-5 * want

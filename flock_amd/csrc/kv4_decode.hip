@@ -4,7 +4,7 @@
 // (5.9 TB/s) and 4.6 of merge, one of 131072 28.3 us (5.3 TB/s) and 3.8.
 //
 // A wave takes 32-key tiles. S^T = K Q^T and O^T += V^T P^T on 16x16x32 f16 MFMA: the
-// 16 columns are 8 query-head rows in two f16 parts each (22 bits), so the parts
+// 16 columns are 8 query-head rows in two f16 parts each, so the parts
 // ride in columns that the few rows would leave empty. The cache's layout gives each
 // lane its operands in 16-byte pieces, and P^T is taken from the S^T accumulators as
 // they lie (a lane's scores are of the tokens whose values it holds). More than 8 rows take

@@ -366,8 +366,10 @@ int32_t flk_kv4_read(const void* pool, const uint32_t* slots, float* k, float* v
  * behind n_tokens, is refused on the device: its o rows are NaN, as are rows that
  * see a key without a page. A row that sees no key (n_keys[b] below its row count)
  * is zeros. o may be q, but not
- * lie partly over it. Sums are f32, q and the weights enter the matrix products in
- * two f16 parts (22 bits), the cache's values as they are.
+ * lie partly over it. Sums are f32, the cache's values enter the matrix
+ * products as they are, q and the weights in two f16 parts: off by at most 2^-23 of a q
+ * down to 2^-16 of its row's largest and of a weight down to 2^-12 of the largest, by
+ * 2^-39 and 2^-35 of the largest below.
  * ws: flk_kv4_attn_ws_bytes of the same arguments, 256-byte aligned; calls that
  * share one must be ordered on one stream. */
 uint64_t flk_kv4_attn_ws_bytes(uint32_t n_seqs, uint32_t max_q, uint32_t max_n_keys,

@@ -86,10 +86,6 @@ __device__ __forceinline__ Kv4Tiles kv4_tiles(int64_t first, int64_t last, uint3
   const uint64_t s = ((uint64_t)n_sinks + kKv4Tile - 1) / kKv4Tile;
   return {(uint32_t)(s < from ? s : from), from, to};
 }
-__device__ __forceinline__ bool kv4_sees(int64_t pos, int64_t key, uint32_t window,
-                                         uint32_t n_sinks) {
-  return key <= pos && (window == 0 || key > pos - (int64_t)window || key < (int64_t)n_sinks);
-}
 
 struct Kv4Shape {
   uint32_t n_kv_heads, head_dim, n_pages, page;

@@ -6,7 +6,7 @@
 
 namespace flk {
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr double kLog2e = 1.44269504088896340736;
 
 // Four packed pairs of a dword's eight codes as (c - 8) * d, d a pair of scales: pair i
 // is nibbles i and i + 4. A masked nibble under 0x6400 is the f16 1024 + c (or 1024 +

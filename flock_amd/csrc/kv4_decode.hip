@@ -551,7 +551,7 @@ static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
   w += item_bytes(a.n_seqs, p);
   part.ml = reinterpret_cast<float*>(w);
   part.acc = reinterpret_cast<float*>(w + ws_align(slots(p, G) * 8));
-  const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
+  const float scale = (float)(kLog2e / sqrt((double)D));
   const uint32_t rows = a.max_q * (a.n_heads / G);
   const dim3 grid(p.runs * p.chunks * G), block(kDecThreads);
   if (a.n_seqs > (uint32_t)kDecThreads) {

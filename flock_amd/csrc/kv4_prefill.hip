@@ -618,7 +618,7 @@ static hipError_t launch(const Kv4AttnArgs& a, void* ws, hipStream_t st) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  const float scale = (float)(1.44269504088896340736 / sqrt((double)D));
+  const float scale = (float)(kLog2e / sqrt((double)D));
   hipLaunchKernelGGL(kv4_prefill_kernel<D>, dim3(grid), dim3(kPreThreads), 0, st, a, p, part,
                      first_piece, list, scale);
   const hipError_t e = hipGetLastError();

@@ -1,10 +1,11 @@
 // Block tables and slot maps of a paged cache from request lengths, on the GPU.
 //
-// Integers only, bound by latency (2048 sequences of 512 blocks: 8 MB and 10.4 us, two
-// launches). Each sequence's row of the table is looked at by one wave, 64 blocks at a time;
+// Integers only, bound by latency (2048 sequences of 512 blocks: 8 MB and 10.6 us, two
+// launches, in both of which a wave waits for the loads of its row eight times in turn). Each
+// sequence's row of the table is looked at by one wave, 64 blocks at a time;
 // what needs a number over the whole batch (which free page a block takes, where a released
 // page goes, where a sequence's tokens start) is a prefix sum in (sequence, block) order. Up
-// to 16 sequences, a wave of one workgroup each, count and write in one launch (6.8 us from
+// to 16 sequences, a wave of one workgroup each, count and write in one launch (6.4 us from
 // the host, 3.9 of kernel); more are counted by a launch of its own, and every workgroup of
 // the second sums the counts of those before it.
 //

@@ -31,15 +31,18 @@ template <int D>
 constexpr uint32_t kPreResident = D == 64 ? 3 : 2;  // workgroups a CU
 constexpr uint32_t kPreMany = 512, kPreMore = 640, kPreLeast = 4;
 
-// The work: row tiles, those of the last queries first (they see the most keys), each in
-// equal pieces of at most `per` key tiles. As for single tokens, `per` comes from the batch's
+// The work: row tiles, those of the last queries first (in a prompt without a window they see the
+// most keys), the sequences in turn, each in equal pieces of at most `per` key tiles. Where
+// lengths differ or a window evens them out this is no order by weight: seven ragged prompts
+// with a window, 143 row tiles of 1 to 35 key tiles, take the time of 55 key tiles as ordered and
+// of 37 heaviest first, in a greedy model of 96 workgroups a kv head. As for single tokens, `per` comes from the batch's
 // total on the device, and every workgroup finds its piece; of more than kMaxCut row tiles a
 // launch before lists them.
 constexpr uint32_t kMaxCut = kPreThreads;
 // Row tiles of up to this many key tiles (2048 keys, or a window's) are whole where there are
 // more than kMaxCut, and without a list up to twice as many. us, a workgroup for every row tile
 // that the call's bounds allow / listed whole / listed and cut: 7 prompts of up to 1500 tokens,
-// 64-wide, window 1024 (329) 88.5 / 97.5 / 100.4, 20 of up to 2000 (640) 224 / 174 / 179, 100
+// 64-wide, window 1024 (294) 88.5 / 97.5 / 100.4, 20 of up to 2000 (640) 224 / 174 / 179, 100
 // (3200) 1597 / 1496 / 1494.
 constexpr uint32_t kShortTiles = 64;
 
@@ -451,7 +454,9 @@ __global__ __launch_bounds__(kPreThreads, kPreResident<D>) void kv4_prefill_kern
 
 // The list. us, a 2048-token prompt at 32768 beside 31 single tokens / one of 8192: 1117 / 598;
 // in workgroups for every row tile that the call's bounds allow, whole, 3372 / 1650 (those
-// without rows are started too, and the others may meet on few CUs).
+// without rows are started too, and the others may meet on few CUs). One workgroup goes over the
+// row tiles of the bounds, not of the lengths, some passes of dependent loads: 512 of them 12 us,
+// 65536 (512 sequences, max_q 8192, eight prompts of 1000 tokens in it) 124, 524288 891.
 constexpr int kListThreads = 1024;
 __device__ __forceinline__ uint32_t pre_pieces(uint32_t count, uint32_t per) {
   return count / per + (count % per != 0);

@@ -294,7 +294,8 @@ def kv4_plan(n_keys, n_new, table_in, table_out, free_in, free_out, q_off, posit
              n_seqs: int, max_blocks: int, n_pages: int, max_tokens: int, page: int, window: int,
              n_sinks: int, ws) -> None:
     """Block table, free list, row offsets, positions and slots of a step, from
-    the lengths after it and the new tokens of each sequence (flk_kv4_plan)."""
+    the lengths after it and the new tokens of each sequence (flk_kv4_plan).
+    ``lost`` counts what attention cannot read: rows that would see it are NaN."""
     w, nb = _ws(ws)
     check(lib().flk_kv4_plan(ptr(n_keys), ptr(n_new), ptr(table_in), ptr(table_out), ptr(free_in),
                              ptr(free_out), ptr(q_off), ptr(positions), ptr(slots), ptr(lost),

@@ -83,8 +83,15 @@ __device__ __forceinline__ PlanJudged plan_judge(const Kv4PlanArgs& a, const Pla
   const bool marked = e >= 0x80000000u;
   const uint32_t id = marked ? mark.page(e) : e, key0 = i << mark.log_page;
   const bool have = id < a.n_pages, want = s.wants(i);
-  const bool old = key0 + (have && marked ? mark.key(e) : 0) < s.pos0;
-  return {id, want && !have && !old, have && !want, want && old && (!have || marked)};
+  const bool fresh = key0 >= s.pos0;
+  return {id, want && !have && fresh, have && !want,
+          want && (have ? marked && key0 + mark.key(e) < s.pos0 : !fresh)};
+}
+
+// Whether block i is as it has to be already, which most are.
+__device__ __forceinline__ bool plan_settled(const Kv4PlanArgs& a, const PlanSeq& s, uint32_t i,
+                                             uint32_t e) {
+  return s.wants(i) ? e < a.n_pages : e == kNoPage;
 }
 
 __device__ __forceinline__ PlanCount plan_count(const Kv4PlanArgs& a, const PlanSeq& s,
@@ -96,6 +103,7 @@ __device__ __forceinline__ PlanCount plan_count(const Kv4PlanArgs& a, const Plan
   for (uint32_t base = 0; base < a.max_blocks; base += 64) {
     const uint32_t e = next;
     next = plan_entry(a, b, base + 64 + lane);
+    if (__ballot(!plan_settled(a, s, base + lane, e)) == 0) continue;
     const PlanJudged j = plan_judge(a, s, base + lane, e);
     c.need += __popcll(__ballot(j.need));
     c.drop += __popcll(__ballot(j.drop));
@@ -208,14 +216,14 @@ __global__ __launch_bounds__(W * 64) void kv4_plan_kernel(Kv4PlanArgs a,
       const uint32_t i = base + lane;
       uint32_t e = next;
       next = plan_entry(a, b, i + 64);
-      const PlanJudged j = plan_judge(a, s, i, e);
-      const uint64_t needs = __ballot(j.need), drops = __ballot(j.drop);
-      const uint64_t lacks = __ballot(j.missing);
-      uint32_t id = j.id < a.n_pages && !j.drop && !j.missing ? j.id : kNoPage;
-      // (A block that lacks keys of its page stays marked.)
-      e = j.missing && j.id < a.n_pages ? e : id;
-      if (needs | drops | lacks) {
+      uint32_t id = e;
+      if (__ballot(!plan_settled(a, s, i, e))) {
+        const PlanJudged j = plan_judge(a, s, i, e);
+        const uint64_t needs = __ballot(j.need), drops = __ballot(j.drop);
         const uint64_t below = (1ull << lane) - 1;
+        id = j.id < a.n_pages && !j.drop && !j.missing ? j.id : kNoPage;
+        // (A block that lacks keys of its page stays marked.)
+        e = j.missing && j.id < a.n_pages ? e : id;
         if (j.drop) {
           const uint32_t to = left + drop_at + __popcll(drops & below);
           if (to < a.n_pages) a.free_out[1 + to] = j.id;
@@ -226,7 +234,7 @@ __global__ __launch_bounds__(W * 64) void kv4_plan_kernel(Kv4PlanArgs a,
         }
         need_at += __popcll(needs);
         drop_at += __popcll(drops);
-        missing += __popcll(lacks);
+        missing += __popcll(__ballot(j.missing));
       }
       if (rows < s.fresh && id < a.n_pages) {  // which of them are not stored
         const uint32_t key0 = i << log_page, from = max(pos0 + rows, key0);

@@ -71,8 +71,8 @@ struct PlanMark {
 };
 
 // Of block i with entry e (an entry past the row is none): its page, whether it takes one or
-// gives it back, and whether keys of it from before the step were stored nowhere. Such a block
-// takes no page: with another's, attention would read what that held before.
+// gives it back, and whether keys of it from before the step, which its rows see, were stored
+// nowhere. Such a block takes no page: with another's, attention would read what that held before.
 struct PlanJudged {
   uint32_t id;
   bool need, drop, missing;
@@ -83,9 +83,10 @@ __device__ __forceinline__ PlanJudged plan_judge(const Kv4PlanArgs& a, const Pla
   const bool marked = e >= 0x80000000u;
   const uint32_t id = marked ? mark.page(e) : e, key0 = i << mark.log_page;
   const bool have = id < a.n_pages, want = s.wants(i);
-  const bool fresh = key0 >= s.pos0;
-  return {id, want && !have && fresh, have && !want,
-          want && (have ? marked && key0 + mark.key(e) < s.pos0 : !fresh)};
+  // (A window of one token shows a row no key before the step, but for sinks.)
+  const bool seen = a.window != 1 || i < s.sinks;
+  const bool lacks = seen && key0 + (have && marked ? mark.key(e) : 0) < s.pos0;
+  return {id, want && !have && !lacks, have && !want, want && lacks && (!have || marked)};
 }
 
 // Whether block i is as it has to be already, which most are.

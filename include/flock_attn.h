@@ -302,6 +302,7 @@ uint64_t flk_kv4_page_bytes(uint32_t n_kv_heads, uint32_t head_dim, uint32_t pag
  * with a window the sequence was taken back behind the first new token of the step
  * before, to keys whose pages had left it). Rows that see it are NaN, its new tokens
  * have no slot, in every step until one in which all of the block's keys are new.
+ * (With window = 1 no row sees an earlier key, so a block behind the sinks takes one.)
  *   Tokens whose rows lie past max_tokens are stored nowhere either: from the first
  * of them on a sequence's blocks keep their pages, but as marked entries, with the
  * same consequences, until a step in which that token and those behind it are new

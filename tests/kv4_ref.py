@@ -122,8 +122,9 @@ def plan(n_keys, n_new, table, free, max_tokens, n_pages, page, window, sinks):
             have = page_id < n_pages
             if have and not want:
                 back.append(page_id)
-            elif want and i * page + (key if have else 0) < n - m and (not have or key < page):
-                # Keys before the new ones were stored nowhere: no page would hold them.
+            elif (want and i * page + (key if have else 0) < n - m and (not have or key < page)
+                  and (window != 1 or i * page < sinks)):
+                # Keys before the new ones that rows see were stored nowhere: no page holds them.
                 missing += 1
                 if have:
                     out[b, i] = table[b, i]

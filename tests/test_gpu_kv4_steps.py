@@ -162,7 +162,7 @@ def test_plans_that_run_dry_equal_the_reference(S, M, window, sinks, rng):
 
 
 @pytest.mark.parametrize("S,M", [(1, 4), (16, 70), (17, 5), (1300, 3)])
-@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3), (1, 40)])
 def test_plans_of_more_tokens_than_rows_equal_the_reference(S, M, window, sinks, rng):
     page, n_pages = 32, S * M + 1
     table = np.full((S, M), ref.NONE, np.uint32)

@@ -100,6 +100,18 @@ def test_lengths_taken_back_behind_the_window():
     assert s.step([150], [150]) == [True] and s.lost == 0
 
 
+def test_a_window_of_one_sees_no_key_that_was_lost():
+    s = Slots(2, 4, 32, 2, window=1)
+    assert s.step([32, 32], [32, 32]) == [True, True]
+    assert s.step([33, 33], [1, 1]) == [False, False] and s.lost == 2
+    assert s.step([34, 34], [1, 1]) == [True, True] and s.lost == 0  # their first pages came back
+    assert s.step([36, 36], [2, 2], max_tokens=1) == [None, None] and s.lost == 3
+    assert s.step([37, 37], [1, 1]) == [True, True] and s.lost == 0
+    s = Slots(1, 4, 32, 1, window=1, sinks=33)
+    s.step([32], [32])
+    assert s.step([33], [1]) == [False] and s.step([34], [1]) == [False]  # a sink was lost
+
+
 def test_drafts_taken_back_never_reach_behind_the_window():
     """Verified tokens and a draft in turn: what a step keeps is what the next one sees."""
     s = Slots(1, 20, 32, 20, window=40, sinks=3)
@@ -197,3 +209,28 @@ def test_random_steps_of_more_tokens_than_rows(seed):
         if s.lost == 0:
             assert False not in got
     assert numbers > 0
+
+
+@pytest.mark.parametrize("window", [1, 2, 31, 33])
+@pytest.mark.parametrize("sinks", [0, 1, 33])
+def test_random_steps_with_narrow_windows(window, sinks):
+    """Pages run out, rows are short and lengths are taken back, all at once."""
+    for seed in range(6):
+        rng = np.random.default_rng(seed)
+        S, M, page = 4, 6, 32
+        s = Slots(S, M, page, 9, window, sinks)
+        keys = np.zeros(S, int)
+        numbers = 0
+        for _ in range(80):
+            new = rng.choice([0, 1, 1, 5, 40], S)
+            what = rng.random(S)
+            back = np.maximum(keys - rng.integers(0, 70, S), 0)
+            keys = np.where(what < 0.08, 0, np.where(what < 0.2, back, keys)) + new
+            fit = keys <= M * page
+            new, keys = np.where(fit, new, 0), np.where(fit, keys, 0)
+            short = int(rng.integers(1, 40)) * (rng.random() < 0.2)
+            got = s.step(keys.tolist(), new.tolist(), max(1, int(new.sum()) - short))
+            numbers += sum(x is True for x in got)
+            if s.lost == 0:
+                assert False not in got
+        assert numbers > 0

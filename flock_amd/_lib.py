@@ -71,6 +71,11 @@ SIGNATURES: dict[str, tuple] = {
         _i32,
         [_p, _p, _p, _p, _p, _p, _f32, _i32, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32,
          _u32, _p, _u64]),
+    "flk_decode_shared_ws_bytes": (_u64, [_u32] * 7),
+    "flk_attn_decode_shared": (_i32, [_p] * 9 + [_u32] * 7 + [_p, _u64]),
+    "flk_decode_layer_shared": (
+        _i32,
+        [_p, _p, _p, _u32, _p, _p, _p, _f32, _i32] + [_p] * 9 + [_u32] * 7 + [_p, _u64]),
     "flk_kv4_page_bytes": (_u64, [_u32, _u32, _u32]),
     "flk_kv4_plan_ws_bytes": (_u64, [_u32]),
     "flk_kv4_plan": (_i32, [_p] * 10 + [_u32] * 7 + [_p, _u64]),
@@ -110,6 +115,10 @@ SIGNATURES: dict[str, tuple] = {
     "flk_argmax": (_i32, [_p, _u32, _p, _p, _p, _u64]),
     "flk_lm_head_ws_bytes": (_u64, [_u32, _u32]),
     "flk_lm_head": (_i32, [_p, _p, _f32, _p, _p, _u32, _u32, _p, _p, _p, _p, _p, _u64]),
+    "flk_tokens_ws_bytes": (_u64, [_u32, _u32, _u32]),
+    "flk_token_logprobs": (_i32, [_p, _u64, _p, _p, _p, _p, _p, _u32, _u32, _u32, _p, _u64]),
+    "flk_sample": (
+        _i32, [_p, _u64, _p, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _p, _u64]),
 }
 
 

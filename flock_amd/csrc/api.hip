@@ -12,6 +12,8 @@
 
 #include "common.hpp"
 #include "kv4.hpp"
+#include "shared.hpp"
+#include "tokens.hpp"
 
 namespace flk {
 
@@ -1082,4 +1084,215 @@ int32_t flk_kv4_attn(const float* q, const void* pool, const uint32_t* table,
                                           window, n_sinks);
   if (int32_t rc = check_ws(ws, ws_bytes, need)) return rc;
   return hip_status(launch_kv4_attn(a, ws, g_stream), "flk_kv4_attn");
+}
+
+// ------------------------------------------------------- shared prefixes ---
+static int32_t check_rows64(const void* p, const char* name) {
+  if (reinterpret_cast<uintptr_t>(p) % 8 != 0)
+    return fail(FLK_ERR_ARG, "%s must be 8-byte aligned", name);
+  return FLK_OK;
+}
+
+static bool shared_shape(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix,
+                         uint32_t max_n_keys) {
+  return n_groups != 0 && n_seqs != 0 && n_groups <= 65535 && n_seqs <= 65535 &&
+         (max_prefix != 0 || max_n_keys != 0) &&
+         (uint64_t)max_prefix + max_n_keys <= 0xFFFFFFFFull;
+}
+
+uint64_t flk_decode_shared_ws_bytes(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix,
+                                    uint32_t max_n_keys, uint32_t n_heads, uint32_t n_kv_heads,
+                                    uint32_t head_dim) {
+  if (!shared_shape(n_groups, n_seqs, max_prefix, max_n_keys) || n_kv_heads == 0 ||
+      n_heads == 0 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 8 ||
+      (head_dim != 64 && head_dim != 128))
+    return 0;
+  return shared_ws_bytes(n_groups, n_seqs, max_prefix, max_n_keys, n_heads, n_kv_heads, head_dim);
+}
+
+// Checks and arguments that the two shared entry points have in common.
+static int32_t shared_args(const float* q, const float* kcache, const float* vcache,
+                           const uint64_t* prefix_row, const uint32_t* n_prefix,
+                           const uint32_t* seq_off, const uint64_t* seq_row_off,
+                           const uint32_t* n_keys, float* o, uint32_t n_groups, uint32_t n_seqs,
+                           uint32_t max_prefix, uint32_t max_n_keys, uint32_t n_heads,
+                           uint32_t n_kv_heads, uint32_t head_dim, void* ws, uint64_t ws_bytes,
+                           const char* what, SharedArgs& a) {
+  FLK_NONNULL(kcache);
+  FLK_NONNULL(vcache);
+  FLK_NONNULL(prefix_row);
+  FLK_WORDS(n_prefix);
+  FLK_WORDS(seq_off);
+  FLK_NONNULL(seq_row_off);
+  FLK_WORDS(n_keys);
+  FLK_NONNULL(o);
+  FLK_ALIGNED(kcache);
+  FLK_ALIGNED(vcache);
+  FLK_ALIGNED(o);
+  if (int32_t rc = check_rows64(prefix_row, "prefix_row")) return rc;
+  if (int32_t rc = check_rows64(seq_row_off, "seq_row_off")) return rc;
+  if (int32_t rc = check_heads(n_heads, n_kv_heads, head_dim)) return rc;
+  if (n_groups == 0 || n_seqs == 0 || (max_prefix == 0 && max_n_keys == 0))
+    return fail(FLK_ERR_ARG, "%s n_groups=%u n_seqs=%u max_prefix=%u max_n_keys=%u", what,
+                n_groups, n_seqs, max_prefix, max_n_keys);
+  if (n_seqs > 65535 || n_groups > 65535)
+    return fail(FLK_ERR_UNSUPPORTED, "%s: %u groups, %u sequences (65535 at most)", what, n_groups,
+                n_seqs);
+  if (!shared_shape(n_groups, n_seqs, max_prefix, max_n_keys))
+    return fail(FLK_ERR_ARG, "%s: max_prefix %u + max_n_keys %u overflows", what, max_prefix,
+                max_n_keys);
+  // A tile of 64 rows is addressed with 32-bit byte offsets.
+  if ((uint64_t)n_kv_heads * head_dim * 4 * 64 > 0x7FFFFFFFull)
+    return fail(FLK_ERR_UNSUPPORTED, "%s: %u kv heads x %u dims exceed a 64-row tile's 2 GiB", what,
+                n_kv_heads, head_dim);
+  const uint64_t bytes = 4ull * n_seqs * n_heads * head_dim;
+  if (q != o && overlap(q, bytes, o, bytes))
+    return fail(FLK_ERR_ARG, "%s: o lies partly over q", what);
+  if (int32_t rc = check_ws(ws, ws_bytes,
+                            shared_ws_bytes(n_groups, n_seqs, max_prefix, max_n_keys, n_heads,
+                                            n_kv_heads, head_dim)))
+    return rc;
+  a = SharedArgs{q,      kcache,   vcache,     prefix_row, seq_row_off, n_prefix,   seq_off, n_keys,
+                 o,      n_groups, n_seqs,     max_prefix, max_n_keys,  n_heads,    n_kv_heads,
+                 head_dim, false};
+  return FLK_OK;
+}
+
+int32_t flk_attn_decode_shared(const float* q, const float* kcache, const float* vcache,
+                               const uint64_t* prefix_row, const uint32_t* n_prefix,
+                               const uint32_t* seq_off, const uint64_t* seq_row_off,
+                               const uint32_t* n_keys, float* o, uint32_t n_groups,
+                               uint32_t n_seqs, uint32_t max_prefix, uint32_t max_n_keys,
+                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, void* ws,
+                               uint64_t ws_bytes) {
+  FLK_NONNULL(q);
+  FLK_ALIGNED(q);
+  SharedArgs a;
+  if (int32_t rc = shared_args(q, kcache, vcache, prefix_row, n_prefix, seq_off, seq_row_off,
+                               n_keys, o, n_groups, n_seqs, max_prefix, max_n_keys, n_heads,
+                               n_kv_heads, head_dim, ws, ws_bytes, "attn_decode_shared", a))
+    return rc;
+  return hip_status(launch_shared(a, nullptr, 0, 0, ws, g_stream), "flk_attn_decode_shared");
+}
+
+int32_t flk_decode_layer_shared(const float* q_raw, const float* k_raw, const float* v_raw,
+                                uint32_t in_stride, const float* gq, const float* gk,
+                                const float* inv_freq, float eps, int32_t pairing, float* qn_out,
+                                float* kcache, float* vcache, const uint64_t* prefix_row,
+                                const uint32_t* n_prefix, const uint32_t* seq_off,
+                                const uint64_t* seq_row_off, const uint32_t* n_keys, float* o,
+                                uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix,
+                                uint32_t max_n_keys, uint32_t n_heads, uint32_t n_kv_heads,
+                                uint32_t head_dim, void* ws, uint64_t ws_bytes) {
+  FLK_NONNULL(q_raw);
+  FLK_NONNULL(k_raw);
+  FLK_NONNULL(v_raw);
+  FLK_NONNULL(gq);
+  FLK_NONNULL(gk);
+  FLK_NONNULL(inv_freq);
+  FLK_NONNULL(qn_out);
+  FLK_ALIGNED(qn_out);
+  if (pairing != FLK_ROPE_NEOX && pairing != FLK_ROPE_NORM)
+    return fail(FLK_ERR_ARG, "rope pairing %d (0 = neox, 1 = norm)", pairing);
+  if (in_stride != 0 && in_stride < n_heads * head_dim)
+    return fail(FLK_ERR_ARG, "in_stride %u is shorter than a q row (%u floats)", in_stride,
+                n_heads * head_dim);
+  if (qn_out == o) return fail(FLK_ERR_ARG, "decode_layer_shared: o lies over qn_out");
+  SharedArgs a;
+  if (int32_t rc = shared_args(qn_out, kcache, vcache, prefix_row, n_prefix, seq_off, seq_row_off,
+                               n_keys, o, n_groups, n_seqs, max_prefix, max_n_keys, n_heads,
+                               n_kv_heads, head_dim, ws, ws_bytes, "decode_layer_shared", a))
+    return rc;
+  a.step = true;
+  DecodeFused f;
+  f.q_raw = q_raw;
+  f.k_raw = k_raw;
+  f.v_raw = v_raw;
+  f.gq = gq;
+  f.gk = gk;
+  f.inv_freq = inv_freq;
+  f.eps = eps;
+  f.pairing = pairing;
+  f.qn_out = qn_out;
+  f.kcache_w = kcache;
+  f.vcache_w = vcache;
+  return hip_status(launch_shared(a, &f, in_stride ? in_stride : n_heads * head_dim,
+                                  in_stride ? in_stride : n_kv_heads * head_dim, ws, g_stream),
+                    "flk_decode_layer_shared");
+}
+
+// ---------------------------------------------------------------- tokens ---
+uint64_t flk_tokens_ws_bytes(uint32_t n_rows, uint32_t n_vocab, uint32_t n_top) {
+  return n_rows == 0 || n_vocab == 0 || n_top > kMaxTop ? 0 : tokens_ws_bytes(n_rows, n_vocab, n_top);
+}
+
+static int32_t token_args(const float* logits, uint64_t ld, uint32_t n_rows, uint32_t n_vocab,
+                          uint32_t n_top, void* ws, uint64_t ws_bytes, const char* what,
+                          TokenArgs& a) {
+  FLK_WORDS(logits);
+  if (n_rows == 0 || n_vocab == 0)
+    return fail(FLK_ERR_ARG, "%s n_rows=%u n_vocab=%u", what, n_rows, n_vocab);
+  if (ld != 0 && ld < n_vocab)
+    return fail(FLK_ERR_ARG, "%s: rows of %u logits lie %llu floats apart", what, n_vocab,
+                (unsigned long long)ld);
+  if (n_top > kMaxTop)
+    return fail(FLK_ERR_UNSUPPORTED, "%s: %u alternatives (%u at most)", what, n_top, kMaxTop);
+  if (n_vocab > 0x7fffffffu)
+    return fail(FLK_ERR_UNSUPPORTED, "%s: a vocabulary of %u ids", what, n_vocab);
+  if (n_rows > kMaxGroups)
+    return fail(FLK_ERR_UNSUPPORTED, "%s: %u rows exceed a launch", what, n_rows);
+  if (int32_t rc = check_ws(ws, ws_bytes, tokens_ws_bytes(n_rows, n_vocab, n_top))) return rc;
+  a = TokenArgs{};
+  a.logits = logits;
+  a.ld = ld ? ld : n_vocab;
+  a.n_rows = n_rows, a.n_vocab = n_vocab, a.n_top = n_top;
+  return FLK_OK;
+}
+
+// An optional device array of 32-bit words.
+#define FLK_MAYBE_WORDS(p)                                do {                                                      if (int32_t rc_ = check_words((p), #p)) return rc_;   } while (0)
+
+int32_t flk_token_logprobs(const float* logits, uint64_t ld, const uint32_t* tokens,
+                           float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs,
+                           uint32_t n_rows, uint32_t n_vocab, uint32_t n_top, void* ws,
+                           uint64_t ws_bytes) {
+  FLK_MAYBE_WORDS(tokens);
+  FLK_MAYBE_WORDS(logprob);
+  FLK_MAYBE_WORDS(entropy);
+  FLK_MAYBE_WORDS(top_ids);
+  FLK_MAYBE_WORDS(top_logprobs);
+  if (logprob != nullptr && tokens == nullptr)
+    return fail(FLK_ERR_ARG, "token_logprobs: logprob needs tokens");
+  if ((n_top != 0) != (top_ids != nullptr) || (n_top != 0) != (top_logprobs != nullptr))
+    return fail(FLK_ERR_ARG, "token_logprobs: %u alternatives, top_ids %s, top_logprobs %s", n_top,
+                top_ids ? "given" : "null", top_logprobs ? "given" : "null");
+  if (logprob == nullptr && entropy == nullptr && n_top == 0)
+    return fail(FLK_ERR_ARG, "token_logprobs: no output is wanted");
+  TokenArgs a;
+  if (int32_t rc = token_args(logits, ld, n_rows, n_vocab, n_top, ws, ws_bytes, "token_logprobs", a))
+    return rc;
+  a.tokens = tokens, a.logprob = logprob, a.entropy = entropy;
+  a.top_ids = top_ids, a.top_logprobs = top_logprobs;
+  return hip_status(launch_tokens(a, ws, g_stream), "flk_token_logprobs");
+}
+
+int32_t flk_sample(const float* logits, uint64_t ld, const float* temperature,
+                   const uint32_t* top_k, const float* top_p, const float* min_p,
+                   const float* uniform, uint32_t* token, float* logprob, uint32_t n_rows,
+                   uint32_t n_vocab, uint32_t max_top_k, void* ws, uint64_t ws_bytes) {
+  FLK_MAYBE_WORDS(temperature);
+  FLK_MAYBE_WORDS(top_k);
+  FLK_MAYBE_WORDS(top_p);
+  FLK_MAYBE_WORDS(min_p);
+  FLK_WORDS(uniform);
+  FLK_WORDS(token);
+  FLK_MAYBE_WORDS(logprob);
+  if (max_top_k == 0) return fail(FLK_ERR_ARG, "sample: max_top_k must be >= 1");
+  TokenArgs a;
+  if (int32_t rc = token_args(logits, ld, n_rows, n_vocab, max_top_k, ws, ws_bytes, "sample", a))
+    return rc;
+  a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
+  a.uniform = uniform;
+  a.token = token, a.logprob = logprob;
+  return hip_status(launch_tokens(a, ws, g_stream), "flk_sample");
 }

@@ -3,6 +3,7 @@
 // be bit-exact with the CPU oracle so that the KV cache a prefill writes is the
 // cache N decode steps write (test_prefill.ts:119-132).
 #include "common.hpp"
+#include "shared.hpp"
 
 namespace flk {
 
@@ -113,7 +114,11 @@ hipError_t launch_kv_append(const float* kn, const float* v, float* kcache, floa
 // fills that sequence's o with NaN too). Workgroup 0 also zeroes the
 // n_queue item counters of the batch decode kernel that follows on the
 // stream, so the ragged step needs no separate reset launch.
+//
+// Batches that share prefixes (SHARED, flk_decode_layer_shared): as RAGGED, with the
+// position behind the group's prefix, n_prefix + n_keys[b] - 1.
 constexpr int kPrologueThreads = 256;
+enum PrologueKind { TOKENS, RAGGED, SHARED };
 
 struct RaggedTokens {
   const uint32_t* n_keys = nullptr;       // [n_seqs]
@@ -123,13 +128,13 @@ struct RaggedTokens {
   uint32_t n_queue = 0;
 };
 
-template <int D, bool RAGGED>
+template <int D, PrologueKind KIND>
 __global__ __launch_bounds__(kPrologueThreads) void qk_prologue_kernel(
     const float* __restrict__ q_raw, const float* __restrict__ k_raw,
     const float* __restrict__ v_raw, const float* __restrict__ gq, const float* __restrict__ gk,
     const float* __restrict__ inv_freq, float eps, int32_t pairing, float* __restrict__ qn_out,
     float* __restrict__ kcache, float* __restrict__ vcache, uint32_t pos0, uint32_t n_heads,
-    uint32_t n_kv_heads, uint32_t q_stride, uint32_t kv_stride, RaggedTokens rt) {
+    uint32_t n_kv_heads, uint32_t q_stride, uint32_t kv_stride, RaggedTokens rt, SharedArgs sh) {
   __shared__ float2 s_cs[D / 2];
   const int lane = threadIdx.x & 63;
   // The wave index in a scalar register: the compiler then knows each vector
@@ -139,7 +144,18 @@ __global__ __launch_bounds__(kPrologueThreads) void qk_prologue_kernel(
   const uint32_t tok = blockIdx.x;
   uint32_t pos = pos0 + tok;
   uint64_t cache_row = pos;
-  if constexpr (RAGGED) {
+  if constexpr (KIND == SHARED) {
+    const SharedSeq s = shared_seq<kPrologueThreads>(sh, tok);
+    if (s.refused || s.idle) {
+      const float fill = s.idle ? 0.f : __builtin_nanf("");
+      float* dq = qn_out + (size_t)tok * n_heads * D;
+      for (uint32_t i = threadIdx.x; i < n_heads * D; i += kPrologueThreads) dq[i] = fill;
+      return;  // uniform per workgroup
+    }
+    pos = s.prefix + s.own - 1;
+    cache_row = sh.seq_row_off[tok] + s.own - 1;
+  }
+  if constexpr (KIND == RAGGED) {
     if (tok == 0 && threadIdx.x < rt.n_queue) rt.queue[threadIdx.x] = 0u;
     const uint32_t nk = rt.n_keys[tok];
     if (nk == 0 || nk > rt.max_n_keys) {  // idle (zeros) or refused (NaN): no append
@@ -246,13 +262,13 @@ hipError_t launch_qk_prologue(const float* q_raw, const float* k_raw, const floa
   const uint32_t kv_stride = in_stride ? in_stride : n_kv_heads * head_dim;
   const RaggedTokens none{};
   if (head_dim == 128)
-    hipLaunchKernelGGL((qk_prologue_kernel<128, false>), dim3(n_tokens), dim3(kPrologueThreads), 0,
+    hipLaunchKernelGGL((qk_prologue_kernel<128, TOKENS>), dim3(n_tokens), dim3(kPrologueThreads), 0,
                        st, q_raw, k_raw, v_raw, gq, gk, inv_freq, eps, pairing, qn_out, kcache,
-                       vcache, pos0, n_heads, n_kv_heads, q_stride, kv_stride, none);
+                       vcache, pos0, n_heads, n_kv_heads, q_stride, kv_stride, none, SharedArgs{});
   else
-    hipLaunchKernelGGL((qk_prologue_kernel<64, false>), dim3(n_tokens), dim3(kPrologueThreads), 0,
+    hipLaunchKernelGGL((qk_prologue_kernel<64, TOKENS>), dim3(n_tokens), dim3(kPrologueThreads), 0,
                        st, q_raw, k_raw, v_raw, gq, gk, inv_freq, eps, pairing, qn_out, kcache,
-                       vcache, pos0, n_heads, n_kv_heads, q_stride, kv_stride, none);
+                       vcache, pos0, n_heads, n_kv_heads, q_stride, kv_stride, none, SharedArgs{});
   return hipGetLastError();
 }
 
@@ -268,15 +284,26 @@ hipError_t launch_ragged_prologue(const DecodeFused& f, const uint64_t* seq_row_
   rt.n_queue = queue != nullptr ? n_queue : 0;
   const uint32_t q_stride = n_heads * head_dim, kv_stride = n_kv_heads * head_dim;
   if (head_dim == 128)
-    hipLaunchKernelGGL((qk_prologue_kernel<128, true>), dim3(n_seqs), dim3(kPrologueThreads), 0,
+    hipLaunchKernelGGL((qk_prologue_kernel<128, RAGGED>), dim3(n_seqs), dim3(kPrologueThreads), 0,
                        st, f.q_raw, f.k_raw, f.v_raw, f.gq, f.gk, f.inv_freq, f.eps, f.pairing,
                        f.qn_out, f.kcache_w, f.vcache_w, 0u, n_heads, n_kv_heads, q_stride,
-                       kv_stride, rt);
+                       kv_stride, rt, SharedArgs{});
   else
-    hipLaunchKernelGGL((qk_prologue_kernel<64, true>), dim3(n_seqs), dim3(kPrologueThreads), 0,
+    hipLaunchKernelGGL((qk_prologue_kernel<64, RAGGED>), dim3(n_seqs), dim3(kPrologueThreads), 0,
                        st, f.q_raw, f.k_raw, f.v_raw, f.gq, f.gk, f.inv_freq, f.eps, f.pairing,
                        f.qn_out, f.kcache_w, f.vcache_w, 0u, n_heads, n_kv_heads, q_stride,
-                       kv_stride, rt);
+                       kv_stride, rt, SharedArgs{});
+  return hipGetLastError();
+}
+
+hipError_t launch_shared_prologue(const SharedArgs& a, const DecodeFused& f, uint32_t q_stride,
+                                  uint32_t kv_stride, hipStream_t st) {
+  const auto kernel = a.head_dim == 128 ? qk_prologue_kernel<128, SHARED>
+                                        : qk_prologue_kernel<64, SHARED>;
+  hipLaunchKernelGGL(kernel, dim3(a.n_seqs), dim3(kPrologueThreads), 0, st, f.q_raw, f.k_raw,
+                     f.v_raw, f.gq, f.gk, f.inv_freq, f.eps, f.pairing, f.qn_out, f.kcache_w,
+                     f.vcache_w, 0u, a.n_heads, a.n_kv_heads, q_stride, kv_stride, RaggedTokens{},
+                     a);
   return hipGetLastError();
 }
 

@@ -54,6 +54,18 @@ export const hip = Deno.dlopen(Deno.env.get("FLOCK_ATTN_LIB") ?? "libflock_attn.
     parameters: [P, P, P, P, P, P, F32, I32, P, P, P, P, P, P, U32, U32, U32, U32, U32, P, U64],
     result: I32,
   },
+  flk_decode_shared_ws_bytes: { parameters: [U32, U32, U32, U32, U32, U32, U32], result: U64 },
+  flk_attn_decode_shared: {
+    parameters: [P, P, P, P, P, P, P, P, P, U32, U32, U32, U32, U32, U32, U32, P, U64],
+    result: I32,
+  },
+  flk_decode_layer_shared: {
+    parameters: [
+      P, P, P, U32, P, P, P, F32, I32, P, P, P, P, P, P, P, P, P, U32, U32, U32, U32, U32, U32, U32,
+      P, U64,
+    ],
+    result: I32,
+  },
   flk_kv4_page_bytes: { parameters: [U32, U32, U32], result: U64 },
   flk_kv4_plan_ws_bytes: { parameters: [U32], result: U64 },
   flk_kv4_plan: {
@@ -82,6 +94,15 @@ export const hip = Deno.dlopen(Deno.env.get("FLOCK_ATTN_LIB") ?? "libflock_attn.
   flk_argmax: { parameters: [P, U32, P, P, P, U64], result: I32 },
   flk_lm_head_ws_bytes: { parameters: [U32, U32], result: U64 },
   flk_lm_head: { parameters: [P, P, F32, P, P, U32, U32, P, P, P, P, P, U64], result: I32 },
+  flk_tokens_ws_bytes: { parameters: [U32, U32, U32], result: U64 },
+  flk_token_logprobs: {
+    parameters: [P, U64, P, P, P, P, P, U32, U32, U32, P, U64],
+    result: I32,
+  },
+  flk_sample: {
+    parameters: [P, U64, P, P, P, P, P, P, P, U32, U32, U32, P, U64],
+    result: I32,
+  },
   // include/flock_graph.h
   flk_decode_layer_dev: {
     parameters: [P, P, P, P, P, P, F32, I32, P, P, P, P, P, U32, U32, U32, U32, P, U64],

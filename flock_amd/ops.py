@@ -277,6 +277,42 @@ def decode_layer_ragged(q_raw, k_raw, v_raw, gq, gk, inv_freq, eps: float, pairi
                                         head_dim, w, nb), "flk_decode_layer_ragged")
 
 
+# ------------------------------------------------------------ shared prefixes
+def decode_shared_ws_bytes(n_groups: int, n_seqs: int, max_prefix: int, max_n_keys: int,
+                           n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    return int(lib().flk_decode_shared_ws_bytes(n_groups, n_seqs, max_prefix, max_n_keys, n_heads,
+                                                n_kv_heads, head_dim))
+
+
+def attn_decode_shared(q, kcache, vcache, prefix_row, n_prefix, seq_off, seq_row_off, n_keys, o,
+                       n_groups: int, n_seqs: int, max_prefix: int, max_n_keys: int, n_heads: int,
+                       n_kv_heads: int, head_dim: int, ws) -> None:
+    """Decode attention of sequences in groups that share a prefix
+    (flk_attn_decode_shared): group g is the sequences seq_off[g] .. seq_off[g + 1] - 1,
+    its prefix n_prefix[g] cache rows from prefix_row[g]; own keys as in attn_decode_ragged."""
+    w, nb = _ws(ws)
+    check(lib().flk_attn_decode_shared(ptr(q), ptr(kcache), ptr(vcache), ptr(prefix_row),
+                                       ptr(n_prefix), ptr(seq_off), ptr(seq_row_off), ptr(n_keys),
+                                       ptr(o), n_groups, n_seqs, max_prefix, max_n_keys, n_heads,
+                                       n_kv_heads, head_dim, w, nb), "flk_attn_decode_shared")
+
+
+def decode_layer_shared(q_raw, k_raw, v_raw, gq, gk, inv_freq, eps: float, pairing, qn_out, kcache,
+                        vcache, prefix_row, n_prefix, seq_off, seq_row_off, n_keys, o,
+                        n_groups: int, n_seqs: int, max_prefix: int, max_n_keys: int, n_heads: int,
+                        n_kv_heads: int, head_dim: int, ws, in_stride: int = 0) -> None:
+    """decode_layer_ragged for sequences that share prefixes (flk_decode_layer_shared):
+    sequence b's new token is at position n_prefix[g] + n_keys[b] - 1."""
+    w, nb = _ws(ws)
+    check(lib().flk_decode_layer_shared(ptr(q_raw), ptr(k_raw), ptr(v_raw), in_stride, ptr(gq),
+                                        ptr(gk), ptr(inv_freq), eps, _pairing(pairing),
+                                        ptr(qn_out), ptr(kcache), ptr(vcache), ptr(prefix_row),
+                                        ptr(n_prefix), ptr(seq_off), ptr(seq_row_off),
+                                        ptr(n_keys), ptr(o), n_groups, n_seqs, max_prefix,
+                                        max_n_keys, n_heads, n_kv_heads, head_dim, w, nb),
+          "flk_decode_layer_shared")
+
+
 # ------------------------------------------------------ paged cache in 4 bits
 def kv4_page_bytes(n_kv_heads: int, head_dim: int, page: int) -> int:
     """Bytes of a page of ``page`` tokens of a 4-bit pool."""
@@ -442,6 +478,30 @@ def lm_head(x, gain, eps: float, w: "Q8Matrix", normed, logits, oval, oidx, ws) 
                             ptr(normed), ptr(logits), ptr(oval), ptr(oidx), wsp, nb),
           "flk_lm_head")
 
+
+def tokens_ws_bytes(n_rows: int, n_vocab: int, n_top: int) -> int:
+    return int(lib().flk_tokens_ws_bytes(n_rows, n_vocab, n_top))
+
+
+def token_logprobs(logits, tokens, logprob, n_rows: int, n_vocab: int, ws=None, entropy=None,
+                   n_top: int = 0, top_ids=None, top_logprobs=None, ld: int = 0) -> None:
+    """Log probabilities of tokens[r] in row r of the logits, the rows' entropies and
+    their n_top largest alternatives (flk_token_logprobs); outputs may be None."""
+    w, nb = _ws(ws)
+    check(lib().flk_token_logprobs(ptr(logits), ld, ptr(tokens), ptr(logprob), ptr(entropy),
+                                   ptr(top_ids), ptr(top_logprobs), n_rows, n_vocab, n_top, w, nb),
+          "flk_token_logprobs")
+
+
+def sample(logits, uniform, token, n_rows: int, n_vocab: int, max_top_k: int, ws=None,
+           temperature=None, top_k=None, top_p=None, min_p=None, logprob=None,
+           ld: int = 0) -> None:
+    """A token of each row from its largest logits, by the row's uniform number
+    (flk_sample); the settings are device arrays with an entry a row, or None."""
+    w, nb = _ws(ws)
+    check(lib().flk_sample(ptr(logits), ld, ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p),
+                           ptr(uniform), ptr(token), ptr(logprob), n_rows, n_vocab, max_top_k, w,
+                           nb), "flk_sample")
 
 
 # ------------------------------------------------------------- graphs

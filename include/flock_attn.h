@@ -252,6 +252,65 @@ int32_t flk_decode_layer_ragged(const float* q_raw, const float* k_raw, const fl
                                 uint32_t max_n_keys, uint32_t n_heads, uint32_t n_kv_heads,
                                 uint32_t head_dim, void* ws, uint64_t ws_bytes);
 
+/* ------------------------------------------------------ shared prefixes -- */
+
+/* Extension, no reference counterpart (the reference runs one sequence per
+ * Layer, layer.ts:203-204): decode for sequences that share long prefixes --
+ * several answers to one prompt, questions about one document -- where the
+ * prefix is stored once and read once for all of them.
+ *
+ *   groups        group g is the sequences seq_off[g] .. seq_off[g + 1] - 1
+ *                 ([n_groups + 1], never falling, at most n_seqs). A group may be
+ *                 empty; a sequence in none has no prefix.
+ *   prefix        group g's is n_prefix[g] rows from row prefix_row[g] of kcache
+ *                 and vcache (rows of n_kv_heads * head_dim floats); 0: none
+ *   own keys      sequence b's are n_keys[b] rows from row seq_row_off[b], as in
+ *                 flk_attn_decode_ragged. They follow the prefix: the newest is at
+ *                 position n_prefix[g] + n_keys[b] - 1.
+ *
+ * All five are DEVICE arrays (prefix_row and seq_row_off 8-byte aligned, the others
+ * 4-byte), so that a captured step replays as they change; the rows they name must lie
+ * inside kcache and vcache. max_prefix and max_n_keys bound n_prefix and n_keys (their
+ * sum is below 2^32, and at least 1) and set the launch shape. What the host cannot
+ * see is refused on the device, with NaN rows: a count beyond its bound (the
+ * sequence, or the group's), and seq_off that falls or passes n_seqs (every row).
+ *
+ * A sequence that sees a key or a value with an infinity or NaN has NaN where they
+ * reach. Sums are f32. Results are the
+ * same bits on every call. ws: flk_decode_shared_ws_bytes of the same arguments, 256-byte
+ * aligned; calls that share one must be ordered on one stream. */
+uint64_t flk_decode_shared_ws_bytes(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix,
+                                    uint32_t max_n_keys, uint32_t n_heads, uint32_t n_kv_heads,
+                                    uint32_t head_dim);
+
+/* Attention of one query per sequence. q, o: [n_seqs][n_heads][head_dim]. A sequence
+ * without any key is zeros. o may be q, but not lie partly over it. */
+int32_t flk_attn_decode_shared(const float* q, const float* kcache, const float* vcache,
+                               const uint64_t* prefix_row, const uint32_t* n_prefix,
+                               const uint32_t* seq_off, const uint64_t* seq_row_off,
+                               const uint32_t* n_keys, float* o, uint32_t n_groups,
+                               uint32_t n_seqs, uint32_t max_prefix, uint32_t max_n_keys,
+                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                               void* ws, uint64_t ws_bytes);
+
+/* flk_decode_layer_ragged for such a batch: n_keys[b] counts sequence b's own keys AFTER
+ * the step; q and k are normed and rotated at position n_prefix[g] + n_keys[b] - 1, k
+ * and v appended at row seq_row_off[b] + n_keys[b] - 1 (no two sequences' the same, and
+ * none in a prefix), then the attention above over qn_out. n_keys[b] = 0 is an idle
+ * sequence: its qn and o rows are zeros. Nothing is appended for it or for a refused
+ * one, whose qn and o rows are NaN. Raw rows lie in_stride floats apart (0: packed), as in
+ * flk_qk_prologue_strided. qn_out and o may not overlap. */
+int32_t flk_decode_layer_shared(const float* q_raw, const float* k_raw, const float* v_raw,
+                                uint32_t in_stride, const float* gq, const float* gk,
+                                const float* inv_freq, float eps, int32_t pairing,
+                                float* qn_out, float* kcache, float* vcache,
+                                const uint64_t* prefix_row, const uint32_t* n_prefix,
+                                const uint32_t* seq_off, const uint64_t* seq_row_off,
+                                const uint32_t* n_keys, float* o, uint32_t n_groups,
+                                uint32_t n_seqs, uint32_t max_prefix, uint32_t max_n_keys,
+                                uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                void* ws, uint64_t ws_bytes);
+
 /* ------------------------------------------------- paged cache in 4 bits -- */
 
 /* Extension, no reference counterpart (the reference keeps one contiguous f32

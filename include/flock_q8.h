@@ -97,6 +97,47 @@ int32_t flk_lm_head(const float* x, const float* norm_gain, float eps, const int
                     const uint16_t* scales, uint32_t vocab, uint32_t hidden, float* normed,
                     float* logits, float* oval, uint32_t* oidx, void* ws, uint64_t ws_bytes);
 
+/* ---- beyond the greedy token (no reference counterpart) ---- */
+
+/* Log probabilities over rows of logits: n_rows rows of n_vocab floats, ld floats from one
+ * to the next (0: n_vocab). DEVICE pointers; any of the outputs may be NULL.
+ *   logprob [n_rows]  of token tokens[r] in row r: x - log(sum of exp); NaN for an id
+ *                     of n_vocab or more (needs tokens)
+ *   entropy [n_rows]  of the row's distribution, in nats
+ *   top_ids, top_logprobs [n_rows][n_top]  the n_top (0 .. 64) largest logits in falling
+ *                     order, ties by the lowest id, with their log probabilities. -infinity
+ *                     and NaN are no alternatives; places left over are 0xffffffff and
+ *                     -infinity. Both, or neither.
+ * Ids at -infinity have no weight. A row that holds a NaN or +infinity, or nothing else
+ * than -infinity, has no distribution: its log probabilities and entropy are NaN. Weights are
+ * summed in f32 apart from the largest, logarithms taken in 64 bits. The same bits on every
+ * call. ws: flk_tokens_ws_bytes (0: none needed), 256-byte aligned; calls that share one
+ * must be ordered on one stream. */
+uint64_t flk_tokens_ws_bytes(uint32_t n_rows, uint32_t n_vocab, uint32_t n_top);
+int32_t flk_token_logprobs(const float* logits, uint64_t ld, const uint32_t* tokens,
+                           float* logprob, float* entropy, uint32_t* top_ids,
+                           float* top_logprobs, uint32_t n_rows, uint32_t n_vocab,
+                           uint32_t n_top, void* ws, uint64_t ws_bytes);
+
+/* A token of each row, drawn from its largest logits by a given uniform number. Row r's
+ * settings are entries r of DEVICE arrays; a NULL one stands for its default.
+ *   top_k        1 .. max_top_k (1 .. 64): so many alternatives as above (default max_top_k)
+ *   temperature  finite t >= 0 (default 1): weight exp((x - x0) / t), x0 the largest logit;
+ *                0: the largest itself
+ *   top_p        > 0 (default 1): alternatives stay until their weights reach top_p of the
+ *                top_k's sum
+ *   min_p        0 .. 1 (default 0): those below min_p of the largest weight go
+ *   uniform      0 <= u < 1: the token is the first whose running sum of weights exceeds u
+ *                of the sum of those that stay
+ * Weights and sums are formed in 64 bits. logprob (may be NULL): the token's log probability in
+ * the row as flk_token_logprobs gives it, whatever the settings. Settings outside these
+ * ranges, and rows without an alternative, give token 0xffffffff and logprob NaN.
+ * ws: flk_tokens_ws_bytes(n_rows, n_vocab, max_top_k). */
+int32_t flk_sample(const float* logits, uint64_t ld, const float* temperature,
+                   const uint32_t* top_k, const float* top_p, const float* min_p,
+                   const float* uniform, uint32_t* token, float* logprob, uint32_t n_rows,
+                   uint32_t n_vocab, uint32_t max_top_k, void* ws, uint64_t ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1145,6 +1145,9 @@ static int32_t shared_args(const float* q, const float* kcache, const float* vca
   if ((uint64_t)n_kv_heads * head_dim * 4 * 64 > 0x7FFFFFFFull)
     return fail(FLK_ERR_UNSUPPORTED, "%s: %u kv heads x %u dims exceed a 64-row tile's 2 GiB", what,
                 n_kv_heads, head_dim);
+  if (!shared_fits(n_groups, n_seqs, max_prefix, max_n_keys, n_heads, n_kv_heads, head_dim))
+    return fail(FLK_ERR_UNSUPPORTED, "%s: %u sequences of %u heads exceed a launch", what, n_seqs,
+                n_heads);
   const uint64_t bytes = 4ull * n_seqs * n_heads * head_dim;
   if (q != o && overlap(q, bytes, o, bytes))
     return fail(FLK_ERR_ARG, "%s: o lies partly over q", what);

@@ -116,7 +116,8 @@ hipError_t launch_kv_append(const float* kn, const float* v, float* kcache, floa
 // stream, so the ragged step needs no separate reset launch.
 //
 // Batches that share prefixes (SHARED, flk_decode_layer_shared): as RAGGED, with the
-// position behind the group's prefix, n_prefix + n_keys[b] - 1.
+// position behind the group's prefix, n_prefix + n_keys[b] - 1. One workgroup more makes
+// the plan of the attention that follows.
 constexpr int kPrologueThreads = 256;
 enum PrologueKind { TOKENS, RAGGED, SHARED };
 
@@ -134,7 +135,8 @@ __global__ __launch_bounds__(kPrologueThreads) void qk_prologue_kernel(
     const float* __restrict__ v_raw, const float* __restrict__ gq, const float* __restrict__ gk,
     const float* __restrict__ inv_freq, float eps, int32_t pairing, float* __restrict__ qn_out,
     float* __restrict__ kcache, float* __restrict__ vcache, uint32_t pos0, uint32_t n_heads,
-    uint32_t n_kv_heads, uint32_t q_stride, uint32_t kv_stride, RaggedTokens rt, SharedArgs sh) {
+    uint32_t n_kv_heads, uint32_t q_stride, uint32_t kv_stride, RaggedTokens rt, SharedArgs sh,
+    SharedPlan plan) {
   __shared__ float2 s_cs[D / 2];
   const int lane = threadIdx.x & 63;
   // The wave index in a scalar register: the compiler then knows each vector
@@ -145,6 +147,10 @@ __global__ __launch_bounds__(kPrologueThreads) void qk_prologue_kernel(
   uint32_t pos = pos0 + tok;
   uint64_t cache_row = pos;
   if constexpr (KIND == SHARED) {
+    if (tok == sh.n_seqs) {  // the workgroup behind the last sequence
+      shared_plan<kPrologueThreads>(sh, plan);
+      return;
+    }
     const SharedSeq s = shared_seq<kPrologueThreads>(sh, tok);
     if (s.refused || s.idle) {
       const float fill = s.idle ? 0.f : __builtin_nanf("");
@@ -264,11 +270,13 @@ hipError_t launch_qk_prologue(const float* q_raw, const float* k_raw, const floa
   if (head_dim == 128)
     hipLaunchKernelGGL((qk_prologue_kernel<128, TOKENS>), dim3(n_tokens), dim3(kPrologueThreads), 0,
                        st, q_raw, k_raw, v_raw, gq, gk, inv_freq, eps, pairing, qn_out, kcache,
-                       vcache, pos0, n_heads, n_kv_heads, q_stride, kv_stride, none, SharedArgs{});
+                       vcache, pos0, n_heads, n_kv_heads, q_stride, kv_stride, none, SharedArgs{},
+                       SharedPlan{});
   else
     hipLaunchKernelGGL((qk_prologue_kernel<64, TOKENS>), dim3(n_tokens), dim3(kPrologueThreads), 0,
                        st, q_raw, k_raw, v_raw, gq, gk, inv_freq, eps, pairing, qn_out, kcache,
-                       vcache, pos0, n_heads, n_kv_heads, q_stride, kv_stride, none, SharedArgs{});
+                       vcache, pos0, n_heads, n_kv_heads, q_stride, kv_stride, none, SharedArgs{},
+                       SharedPlan{});
   return hipGetLastError();
 }
 
@@ -287,23 +295,25 @@ hipError_t launch_ragged_prologue(const DecodeFused& f, const uint64_t* seq_row_
     hipLaunchKernelGGL((qk_prologue_kernel<128, RAGGED>), dim3(n_seqs), dim3(kPrologueThreads), 0,
                        st, f.q_raw, f.k_raw, f.v_raw, f.gq, f.gk, f.inv_freq, f.eps, f.pairing,
                        f.qn_out, f.kcache_w, f.vcache_w, 0u, n_heads, n_kv_heads, q_stride,
-                       kv_stride, rt, SharedArgs{});
+                       kv_stride, rt, SharedArgs{},
+                       SharedPlan{});
   else
     hipLaunchKernelGGL((qk_prologue_kernel<64, RAGGED>), dim3(n_seqs), dim3(kPrologueThreads), 0,
                        st, f.q_raw, f.k_raw, f.v_raw, f.gq, f.gk, f.inv_freq, f.eps, f.pairing,
                        f.qn_out, f.kcache_w, f.vcache_w, 0u, n_heads, n_kv_heads, q_stride,
-                       kv_stride, rt, SharedArgs{});
+                       kv_stride, rt, SharedArgs{},
+                       SharedPlan{});
   return hipGetLastError();
 }
 
-hipError_t launch_shared_prologue(const SharedArgs& a, const DecodeFused& f, uint32_t q_stride,
-                                  uint32_t kv_stride, hipStream_t st) {
+hipError_t launch_shared_prologue(const SharedArgs& a, const SharedPlan& p, const DecodeFused& f,
+                                  uint32_t q_stride, uint32_t kv_stride, hipStream_t st) {
   const auto kernel = a.head_dim == 128 ? qk_prologue_kernel<128, SHARED>
                                         : qk_prologue_kernel<64, SHARED>;
-  hipLaunchKernelGGL(kernel, dim3(a.n_seqs), dim3(kPrologueThreads), 0, st, f.q_raw, f.k_raw,
-                     f.v_raw, f.gq, f.gk, f.inv_freq, f.eps, f.pairing, f.qn_out, f.kcache_w,
+  hipLaunchKernelGGL(kernel, dim3(a.n_seqs + 1), dim3(kPrologueThreads), 0, st, f.q_raw,
+                     f.k_raw, f.v_raw, f.gq, f.gk, f.inv_freq, f.eps, f.pairing, f.qn_out, f.kcache_w,
                      f.vcache_w, 0u, a.n_heads, a.n_kv_heads, q_stride, kv_stride, RaggedTokens{},
-                     a);
+                     a, p);
   return hipGetLastError();
 }
 

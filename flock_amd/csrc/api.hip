@@ -1244,7 +1244,7 @@ static int32_t token_args(const float* logits, uint64_t ld, uint32_t n_rows, uin
     return fail(FLK_ERR_UNSUPPORTED, "%s: a vocabulary of %u ids", what, n_vocab);
   if (n_rows > kMaxGroups)
     return fail(FLK_ERR_UNSUPPORTED, "%s: %u rows exceed a launch", what, n_rows);
-  if (int32_t rc = check_ws(ws, ws_bytes, tokens_ws_bytes(n_rows, n_vocab, n_top))) return rc;
+  if (int32_t rc = check_ws(ws, ws_bytes, tokens_need(n_rows, n_vocab, n_top))) return rc;
   a = TokenArgs{};
   a.logits = logits;
   a.ld = ld ? ld : n_vocab;

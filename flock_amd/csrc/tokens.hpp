@@ -21,6 +21,7 @@ struct TokenArgs {
   const uint32_t* top_k;
   uint32_t* token;
 };
+uint64_t tokens_need(uint32_t n_rows, uint32_t n_vocab, uint32_t n_top);
 uint64_t tokens_ws_bytes(uint32_t n_rows, uint32_t n_vocab, uint32_t n_top);
 hipError_t launch_tokens(const TokenArgs& a, void* ws, hipStream_t st);
 

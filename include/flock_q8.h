@@ -111,8 +111,8 @@ int32_t flk_lm_head(const float* x, const float* norm_gain, float eps, const int
  * Ids at -infinity have no weight. A row that holds a NaN or +infinity, or nothing else
  * than -infinity, has no distribution: its log probabilities and entropy are NaN. Weights are
  * summed in f32 apart from the largest, logarithms taken in 64 bits. The same bits on every
- * call. ws: flk_tokens_ws_bytes (0: none needed), 256-byte aligned; calls that share one
- * must be ordered on one stream. */
+ * call. ws: flk_tokens_ws_bytes, which holds calls of fewer rows too (0: none needed), 256-byte
+ * aligned; calls that share one must be ordered on one stream. */
 uint64_t flk_tokens_ws_bytes(uint32_t n_rows, uint32_t n_vocab, uint32_t n_top);
 int32_t flk_token_logprobs(const float* logits, uint64_t ld, const uint32_t* tokens,
                            float* logprob, float* entropy, uint32_t* top_ids,

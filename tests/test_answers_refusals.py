@@ -127,4 +127,8 @@ def test_samples():
     if need:
         refused(WORKSPACE, draw, rows=1, vocab=151936, ws=None)
         refused(WORKSPACE, draw, rows=1, vocab=151936, ws=(P, need - 1))
+        refused(WORKSPACE, draw, rows=1, vocab=151936, ws=(P + 4, need))
+    for rows in (1, 2, 63, 700, 1024, 1025, 5000):
+        assert need <= ops.tokens_ws_bytes(rows, 151936, 20) <= ops.tokens_ws_bytes(
+            rows + 1, 151936, 20)
     assert ops.tokens_ws_bytes(0, 100, 5) == 0 and ops.tokens_ws_bytes(1, 100, 65) == 0

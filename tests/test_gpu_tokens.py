@@ -156,6 +156,33 @@ def test_orders_that_are_hard(V, rng):
         check(x, np.full(len(x), V - 1), k)
 
 
+@pytest.mark.parametrize("n,V", [(256, 170001), (520, 90001)])
+def test_rows_that_waves_take_in_segments(n, V, rng):
+    """Many long rows: a workgroup each, whose waves look for alternatives more than once.
+    Some rows are checked, hard ones among them."""
+    x = rng.standard_normal((1, V), np.float32).repeat(n, 0) + np.arange(n, dtype=np.float32)[:, None]
+    i = np.arange(V, dtype=np.float32)
+    x[3], x[4], x[5], x[6] = i, -i, 2.5, (i // 1000) % 7
+    x[7, 100:] = -INF
+    x[8, :-40] = -INF
+    rows = [0, 3, 4, 5, 6, 7, 8, n // 2, n - 1]
+    buf = dev(x)
+    tokens = np.full(n, V - 1)
+    for k in (1, 64):
+        lp, ids, tops = B(4 * n), B(4 * n * k), B(4 * n * k)
+        ops.token_logprobs(buf, dev(tokens, np.uint32), lp, n, V, workspace(n, V, k), n_top=k,
+                           top_ids=ids, top_logprobs=tops)
+        ops.sync()
+        got = ids.download(n * k, np.uint32).reshape(n, k)
+        values, logs = tops.download(n * k).reshape(n, k), lp.download(n)
+        for r in rows:
+            l, _, w, top = want(x[r], k)
+            assert np.array_equal(got[r], w), r
+            close(logs[r], l[-1], slack(V) + 2.0 ** -23 * abs(l[-1]))
+            for a, b in zip(values[r], top):
+                close(a, b, slack(V) + 2.0 ** -23 * abs(b))
+
+
 def test_masks_and_what_is_not_finite(rng):
     V = 3000
     x = language(rng, 10, V)

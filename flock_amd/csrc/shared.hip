@@ -7,13 +7,13 @@
 // scaled by powers of two first: q by its row's largest, K by its tile's largest (both
 // undone in the score's factor), V by a factor that moves with its tiles' largest.
 //
-// An item is 128 rows of q (query heads of one kv head, of as many sequences) and a piece of
-// their keys; four waves of 32 rows, two workgroups a CU. A tile of 32 keys (64 of 64-wide
-// heads) of K and V comes through registers, is split there and put into LDS, in the order of
-// the matrix operands, once for all rows; the next tile's loads are in flight meanwhile. S^T = K
-// Q^T and O^T += V^T P^T on 32x32x16: a column is a row of q, and P^T is taken from the S^T
-// accumulators as they lie, because V's keys are put in the order in which a lane holds its
-// scores. Own keys are items of the sequence's few rows; waves without rows only stage.
+// A workgroup takes a run of tiles, 32 keys each (64 of 64-wide heads) that meet up to 128
+// rows of q; four waves of 32 rows, two workgroups a CU. A tile's K and V come through
+// registers, are split there and put into LDS, in the order of the matrix operands, once for all
+// rows; the next tile's loads are in flight meanwhile, also where a chain ends and the next begins.
+// S^T = K Q^T and O^T += V^T P^T on 32x32x16: a column is a row of q, and P^T is taken from the
+// S^T accumulators as they lie, because V's keys are put in the order in which a lane holds its
+// scores. Waves without rows (a sequence's own keys meet few) only stage.
 #include <algorithm>
 
 #include "shared.hpp"
@@ -44,13 +44,15 @@ struct alignas(16) SharedLds {
   float top[2][2][kShThreads / 64];  // the largest |k| and |v| of a tile, by wave
 };
 
-// Two f16 parts of four values times s (a power of two), 8 bytes each.
-__device__ __forceinline__ void split4(float x, float y, float z, float w, float s, uint2& hi,
-                                       uint2& lo) {
-  x *= s, y *= s, z *= s, w *= s;
-  const halfx2 a = pack_half2(x, y), b = pack_half2(z, w);
-  hi = make_uint2(as_u32(a), as_u32(b));
-  lo = make_uint2(as_u32(rest_half2(x, y, a)), as_u32(rest_half2(z, w, b)));
+// f16(x s) and f16(y s), and what is left of x s and y s (a difference that is formed exactly),
+// rounded likewise; s a power of two.
+__device__ __forceinline__ uint32_t first_part(float x, float y, float s) {
+  return as_u32(pack_half2(x * s, y * s));
+}
+__device__ __forceinline__ uint32_t second_part(float x, float y, float s, uint32_t first) {
+  const halfx2 h = as_half2(first);
+  const halfx2 l = {(_Float16)fmaf(x, s, -(float)h[0]), (_Float16)fmaf(y, s, -(float)h[1])};
+  return as_u32(l);
 }
 __device__ __forceinline__ float wave_max(float v) {
   v = fmaxf(v, xor_lane<1>(v));
@@ -60,26 +62,62 @@ __device__ __forceinline__ float wave_max(float v) {
   v = max_xor<16>(v);
   return max_xor<32>(v);
 }
+__device__ __forceinline__ float uniform_f(float v) {  // in a scalar register
+  return __builtin_bit_cast(float, uniform(__builtin_bit_cast(uint32_t, v)));
+}
 __device__ __forceinline__ float power_of_two(int e) {  // 2^e, |e| < 127
   return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
 }
+
+// v, in a way that what is computed from it is not moved out of a loop: the kernel's registers
+// are full, and a few instructions a tile cost less than registers held or spilled.
+__device__ __forceinline__ uint32_t here(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// What of a tile is known when its loads are sent, and goes with it.
+struct SharedTile {
+  uint32_t keys;          // it holds
+  uint32_t row0, n_rows;  // they meet
+  uint32_t part;          // where the rows' results go
+  uint32_t first, last;   // of the run's tiles of its chain: 1
+};
 
 template <int D>
 __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a, SharedPlan p,
                                                                    float scale_log2e) {
   constexpr int kTile = 4096 / D, kBlocks = kTile / 32, kSteps = D / 16, kOT = D / 32;
+  constexpr int kPart = SharedLds<D>::kPart;
   constexpr int kChunks = D / 4;          // float4s of a row
   constexpr int kGroups = 64 / kChunks;   // rows of a load
   __shared__ SharedLds<D> sh;
-  if (blockIdx.x >= *p.n_items) return;
-  const SharedItem* it = p.item + blockIdx.x;
-  const uint64_t key_row = it->key_row;
-  const uint32_t n_keys = it->n_keys, row0 = it->row0, n_rows = it->n_rows, kvh = it->kvh;
   const uint32_t G = a.n_kv_heads, m = a.n_heads / G;
+  const uint32_t kvh = blockIdx.x % G, run = blockIdx.x / G;
+  if (run >= uniform(*p.n_runs)) return;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
-  const uint32_t n_tiles = (n_keys + kTile - 1) / kTile;
+  const uint32_t rows = a.n_seqs * m;
+  const size_t part0 = kvh * shared_parts(rows, p.max_runs);
+
+  // The chain that tiles are fetched from.
+  uint32_t e = uniform(p.run[run].chain), tile = uniform(p.run[run].tile0);
+  const uint32_t end = uniform(p.run[run].tile1);
+  uint64_t key_row;
+  uint32_t n_keys, in_chain, kind;
+  SharedTile next;
+  auto open = [&] {
+    typedef const __attribute__((address_space(4))) uint32_t* ConstPtr;
+    const ConstPtr c = (ConstPtr)(uintptr_t)(p.chain + e);
+    key_row = uniform(c[0]) | (uint64_t)uniform(c[1]) << 32;
+    n_keys = uniform(c[2]), next.row0 = uniform(c[3]), next.n_rows = uniform(c[4]);
+    in_chain = uniform(tile - c[5]);
+    kind = uniform(c[7]);
+    next.part = uniform(c[6]) == run ? next.row0 + (kind & kSharedOwn ? rows : 0)
+                            : 2 * rows + run * kSharedRows;
+    next.first = 1;
+  };
 
   // Staging: a thread loads chunk c of four rows of K, and of four rows of V that are
   // neighbours in the operands' order of keys: of a 16-key step, lane half h holds the scores of
@@ -89,23 +127,46 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
   const int v_unit = D == 128 ? (wave & 1) + 2 * gr : gr;
   const uint32_t stride = G * D * 4;  // bytes of a cache row
   const uint32_t k_key = wave * (kTile / 4) + gr, v_key = 16 * v_step + 4 * v_unit;
-  const size_t base = (key_row * G + kvh) * D;
+  // (Rows 2 i, or 4 i, further of K lie 512 i bytes on, their slots xored with 2 i; V's rows of
+  // dims j modulo 4 2048 j bytes on.)
+  const uint32_t k_to = sh_k_at<D>(k_key, c >> 1) + 8 * (c & 1);
+  const uint32_t v_to = sh_v_at<D>(c, 2 * v_step + (v_unit & 1)) + 8 * (v_unit >> 1);
+  const uint32_t k_from = sh_k_at<D>(col, h), v_from = sh_v_at<D>(col, h);
+  const uint32_t k_off = k_key * stride + 16 * c, v_off = v_key * stride + 16 * c;
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
   u4 rk[4], rv[4];
-  auto fetch = [&](uint32_t tile) {
-    const size_t at = base + (size_t)tile * kTile * G * D;
-    const uint32_t keys = min(n_keys - tile * kTile, (uint32_t)kTile);
-    const uint32_t bytes = (keys - 1) * stride + D * 4;  // rows behind the last read as zeros
+  // Sends the loads of the next tile; what goes with it is in `next` then.
+  auto fetch = [&] {
+    if (next.last) {
+      e++;
+      open();
+    }
+    const size_t at = ((key_row + (uint64_t)in_chain * kTile) * G + kvh) * D;
+    next.keys = min(n_keys - in_chain * kTile, (uint32_t)kTile);
+    // (Rows behind the last read as zeros: the descriptors end with the tile's last row.)
+    const uint32_t bytes = (next.keys - 1) * stride + D * 4;
     const auto ks = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.kcache + at), 0, bytes,
                                                       0x00020000);
     const auto vs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.vcache + at), 0, bytes,
                                                       0x00020000);
+    const uint32_t ko = here(k_off), vo = here(v_off);
+    if (kind & kSharedOnce) {  // not to stay in the caches
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      rk[i] = __builtin_amdgcn_raw_buffer_load_b128(ks, (k_key + kGroups * i) * stride + 16 * c, 0, 0);
+      for (int i = 0; i < 4; i++)
+        rk[i] = __builtin_amdgcn_raw_buffer_load_b128(ks, ko + kGroups * i * stride, 0, 2);
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      rv[i] = __builtin_amdgcn_raw_buffer_load_b128(vs, (v_key + i) * stride + 16 * c, 0, 0);
+      for (int i = 0; i < 4; i++)
+        rv[i] = __builtin_amdgcn_raw_buffer_load_b128(vs, vo + i * stride, 0, 2);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        rk[i] = __builtin_amdgcn_raw_buffer_load_b128(ks, ko + kGroups * i * stride, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        rv[i] = __builtin_amdgcn_raw_buffer_load_b128(vs, vo + i * stride, 0, 0);
+    }
+    next.last = uniform(tile + 1 == end || (in_chain + 1) * kTile >= n_keys ? 1 : 0);
+    tile++, in_chain++;
   };
   auto f = [](uint32_t x) { return __builtin_bit_cast(float, x); };
   auto note_top = [&](int buf) {
@@ -120,55 +181,57 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     k = wave_max(k), v = wave_max(v);
     if (lane == 0) sh.top[buf][0][wave] = k, sh.top[buf][1][wave] = v;
   };
-  // K's and V's factors of the tile in registers. V's stays while the tile's largest value
-  // lies in 2^7 .. 2^15 with it, so that accumulators seldom change theirs.
+  // K's factor of the tile in registers, undone (k_down), and V's, 2^v_e (or NaN for a tile with
+  // an infinity, whose rows are NaN then). V's stays while the tile's largest value lies in
+  // 2^7 .. 2^15 with it, so that accumulators seldom change theirs.
   float k_down = 0.f, v_up = 1.f;
+  int v_e = 0;
   auto stage = [&](int buf, bool first) {
     const float4 kt = *reinterpret_cast<const float4*>(sh.top[buf][0]);
     const float4 vt = *reinterpret_cast<const float4*>(sh.top[buf][1]);
-    const RowScale rs = row_scale(fmaxf(fmaxf(kt.x, kt.y), fmaxf(kt.z, kt.w)));
+    const RowScale rs = row_scale(uniform_f(fmaxf(fmaxf(kt.x, kt.y), fmaxf(kt.z, kt.w))));
     k_down = rs.down;
-    const float top = fmaxf(fmaxf(vt.x, vt.y), fmaxf(vt.z, vt.w)), now = top * v_up;
-    if (first || !(now >= 128.f && now < 32768.f)) {
-      const int e = (int)((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 127;
-      const int old = (int)((__builtin_bit_cast(uint32_t, v_up) >> 23) & 255u) - 127;
-      // (2^12 .. 2^13; by at most 2^60 up, so that accumulators stay finite.)
-      int up = min(12 - max(e, -100), first ? 112 : old + 60);
-      if (top == 0.f && !first) up = old;
-      v_up = top < INFINITY ? power_of_two(max(up, -115)) : __builtin_nanf("");
-    }
+    const float top = uniform_f(fmaxf(fmaxf(vt.x, vt.y), fmaxf(vt.z, vt.w)));
+    const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, now = e + v_e;
+    if (first)
+      v_e = min(12 - max(e, -100), 112);
+    else if ((now < 7 || now > 14) && e != -127)  // 2^12; by at most 2^60 up: finite accumulators
+      v_e = max(min(12 - max(e, -100), v_e + 60), -115);
+    v_up = e < 128 ? power_of_two(v_e) : __builtin_nanf("");
 #pragma unroll
     for (int i = 0; i < 4; i++) {
+      const float x = f(rk[i][0]), y = f(rk[i][1]), z = f(rk[i][2]), w = f(rk[i][3]);
       uint2 hi, lo;
-      split4(f(rk[i][0]), f(rk[i][1]), f(rk[i][2]), f(rk[i][3]), rs.up, hi, lo);
-      const uint32_t at = sh_k_at<D>(k_key + kGroups * i, c >> 1) + 8 * (c & 1);
-      *reinterpret_cast<uint2*>(&sh.k[buf][0][at]) = hi;
-      *reinterpret_cast<uint2*>(&sh.k[buf][1][at]) = lo;
+      hi.x = first_part(x, y, rs.up), hi.y = first_part(z, w, rs.up);
+      lo.x = second_part(x, y, rs.up, hi.x), lo.y = second_part(z, w, rs.up, hi.y);
+      uint8_t* at = &sh.k[0][0][(k_to + buf * (2 * kPart)) ^ (i << 5)] + 512 * i;
+      *reinterpret_cast<uint2*>(at) = hi;
+      *reinterpret_cast<uint2*>(at + kPart) = lo;
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
+      const float x = f(rv[0][j]), y = f(rv[1][j]), z = f(rv[2][j]), w = f(rv[3][j]);
       uint2 hi, lo;
-      split4(f(rv[0][j]), f(rv[1][j]), f(rv[2][j]), f(rv[3][j]), v_up, hi, lo);
-      const uint32_t at = sh_v_at<D>(j * kChunks + c, 2 * v_step + (v_unit & 1)) + 8 * (v_unit >> 1);
-      *reinterpret_cast<uint2*>(&sh.v[buf][0][at]) = hi;
-      *reinterpret_cast<uint2*>(&sh.v[buf][1][at]) = lo;
+      hi.x = first_part(x, y, v_up), hi.y = first_part(z, w, v_up);
+      lo.x = second_part(x, y, v_up, hi.x), lo.y = second_part(z, w, v_up, hi.y);
+      uint8_t* at = &sh.v[0][0][v_to + buf * (2 * kPart)] + 2048 * j;
+      *reinterpret_cast<uint2*>(at) = hi;
+      *reinterpret_cast<uint2*>(at + kPart) = lo;
     }
   };
 
-  fetch(0);
   // This wave's rows (lanes behind the last repeat it), q in two parts: dims 16 s + 8 h ..
-  const bool idle = wave * 32u >= n_rows;
-  const uint32_t my = row0 + min(wave * 32u + col, n_rows - 1);
   Half8 qh[kSteps], ql[kSteps];
-  float c_s;
-  {
-    const float* src = a.q + ((size_t)(my / m) * a.n_heads + kvh * m + my % m) * D;
+  float c_s = 0.f;
+  auto load_q = [&](uint32_t row0, uint32_t n_rows) {
+    const uint32_t l = here(lane), my = row0 + min(wave * 32u + (l & 31), n_rows - 1);
+    const float* src = a.q + ((size_t)(my / m) * a.n_heads + kvh * m + my % m) * D + 8 * (l >> 5);
     float x[D / 2], amax = 0.f;
 #pragma unroll
     for (int s = 0; s < kSteps; s++)
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        const float4 y = *reinterpret_cast<const float4*>(src + 16 * s + 8 * h + 4 * i);
+        const float4 y = *reinterpret_cast<const float4*>(src + 16 * s + 4 * i);
         x[8 * s + 4 * i] = y.x, x[8 * s + 4 * i + 1] = y.y;
         x[8 * s + 4 * i + 2] = y.z, x[8 * s + 4 * i + 3] = y.w;
       }
@@ -179,25 +242,31 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     c_s = rs.down * scale_log2e;
 #pragma unroll
     for (int i = 0; i < D / 4; i++) {
-      const float u = x[2 * i] * rs.up, v = x[2 * i + 1] * rs.up;
-      const halfx2 hi = pack_half2(u, v);
-      qh[i >> 2].u[i & 3] = as_u32(hi);
-      ql[i >> 2].u[i & 3] = as_u32(rest_half2(u, v, hi));
+      const uint32_t hi = first_part(x[2 * i], x[2 * i + 1], rs.up);
+      qh[i >> 2].u[i & 3] = hi;
+      ql[i >> 2].u[i & 3] = second_part(x[2 * i], x[2 * i + 1], rs.up, hi);
     }
-  }
+  };
 
-  floatx16v o[kOT] = {};
+  floatx16v o[kOT];
   float ref = -INFINITY, l = 0.f;
   auto block = [&](int buf, int kb, float c_t, uint32_t keys) {
     floatx16v s = {};
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
-      const uint32_t at = sh_k_at<D>(kb * 32 + col, 2 * i + h);
-      const halfx8 kh = *reinterpret_cast<const halfx8*>(&sh.k[buf][0][at]);
-      const halfx8 kl = *reinterpret_cast<const halfx8*>(&sh.k[buf][1][at]);
+      const uint8_t* at = &sh.k[0][0][(k_from + buf * (2 * kPart)) ^ (i << 5)] + kb * (64 * D);
+      const halfx8 kh = *reinterpret_cast<const halfx8*>(at);
+      const halfx8 kl = *reinterpret_cast<const halfx8*>(at + kPart);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[i].h, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[i].h, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[i].h, s, 0, 0, 0);
+    }
+    // (K's operands two steps ahead of the products.)
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
     if (keys < kTile) {
 #pragma unroll
@@ -226,106 +295,144 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     Half8 ph[2], pl[2];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const halfx2 hi = pack_half2(s[2 * i], s[2 * i + 1]);
-      ph[i >> 2].u[i & 3] = as_u32(hi);
-      pl[i >> 2].u[i & 3] = as_u32(rest_half2(s[2 * i], s[2 * i + 1], hi));
+      const uint32_t hi = as_u32(pack_half2(s[2 * i], s[2 * i + 1]));
+      ph[i >> 2].u[i & 3] = hi;
+      pl[i >> 2].u[i & 3] = second_part(s[2 * i], s[2 * i + 1], 1.f, hi);
     }
 #pragma unroll
-    for (int ks = 0; ks < 2; ks++)
+    for (int ks = 0; ks < 2; ks++) {
+      // (Half of V's operands may be read ahead, during the weights; all of them are too many
+      // registers.)
+      if (ks > 0) asm volatile("" ::: "memory");
 #pragma unroll
       for (int x = 0; x < kOT; x++) {
-        const uint32_t at = sh_v_at<D>(32 * x + col, 4 * kb + 2 * ks + h);
-        const halfx8 vh = *reinterpret_cast<const halfx8*>(&sh.v[buf][0][at]);
-        const halfx8 vl = *reinterpret_cast<const halfx8*>(&sh.v[buf][1][at]);
+        const uint8_t* at =
+            &sh.v[0][0][(v_from + buf * (2 * kPart)) ^ ((4 * kb + 2 * ks) << 4)] + x * (kPart / kOT);
+        const halfx8 vh = *reinterpret_cast<const halfx8*>(at);
+        const halfx8 vl = *reinterpret_cast<const halfx8*>(at + kPart);
         o[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[ks].h, o[x], 0, 0, 0);
         o[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[ks].h, o[x], 0, 0, 0);
         o[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[ks].h, o[x], 0, 0, 0);
       }
+    }
+  };
+  // The rows' results so far: accumulator i of block x is row 8 (i / 4) + 4 h + i % 4 of V's
+  // 32 x .., so dim 4 (row % (D / 4)) + row / (D / 4).
+  auto store = [&](uint32_t part, uint32_t n_rows, int unit) {
+    float lo, hi;
+    swap_pair<32>(l, lo, hi);
+    const float sum = lo + hi;
+    const uint32_t ln = here(lane), row = wave * 32u + (ln & 31);
+    if (row >= n_rows) return;
+    const size_t at = part0 + part + row;
+    if (ln < 32) p.ml[at] = make_float2(ref, sum);
+    // (One after the other: their product may overflow.)
+    const float inv = 1.f / sum, down = power_of_two(-unit);
+    float* dst = p.acc + at * D + 16 * (ln >> 5);
+#pragma unroll
+    for (int i = 0; i < D / 8; i++) {
+      const int r = 8 * (i >> 2) + (i & 3);  // (and 4 h)
+      if constexpr (D == 128)
+        *reinterpret_cast<float4*>(dst + 4 * r) =
+            make_float4(o[0][i] * inv * down, o[1][i] * inv * down, o[2][i] * inv * down,
+                        o[3][i] * inv * down);
+      else
+        *reinterpret_cast<float4*>(dst + 4 * r) =
+            make_float4(o[0][i] * inv * down, o[0][i + 8] * inv * down, o[1][i] * inv * down,
+                        o[1][i + 8] * inv * down);
+    }
   };
 
+  const uint32_t n = end - tile;
+  next.last = 0;
+  open();
+  fetch();
   note_top(0);
+  SharedTile staged = next;
   lds_barrier();
   stage(0, true);
-  float unit = v_up;  // of the accumulators
-  if (n_tiles > 1) {
-    fetch(1);
+  float k_now = k_down, v_now = v_up;  // of the tile in LDS
+  int e_now = v_e, unit;               // unit: accumulators hold O^T 2^unit
+  if (n > 1) {
+    next.first = 0;
+    fetch();
+    note_top(1);
   }
-  float c_t = c_s * k_down, v_now = v_up;
-  if (n_tiles > 1) note_top(1);
   lds_barrier();
-  for (uint32_t t = 0; t < n_tiles; t++) {
-    const int buf = t & 1;
-    const float c_now = c_t, u_now = v_now;
-    if (t + 1 < n_tiles) {
-      stage(buf ^ 1, false);
-      c_t = c_s * k_down, v_now = v_up;
-      if (t + 2 < n_tiles) fetch(t + 2);
-    }
-    if (!idle) {
-      if (u_now != unit) {  // uniform
-        const float alpha = u_now / unit;
+  for (uint32_t t = 0; t < n;) {  // chains
+    const uint32_t n_rows = staged.n_rows, part = staged.part;
+    const bool busy = wave * 32u < n_rows;
+    if (busy) load_q(staged.row0, n_rows);
+    ref = -INFINITY, l = 0.f, unit = e_now;
 #pragma unroll
-        for (int x = 0; x < kOT; x++) o[x] *= alpha;
-        unit = u_now;
+    for (int x = 0; x < kOT; x++) o[x] = floatx16v{};
+    uint32_t last;
+    do {  // their tiles
+      const int buf = t & 1;
+      const uint32_t keys = staged.keys;
+      const float k_t = k_now, v_t = v_now;
+      const int e_t = e_now;
+      last = staged.last;
+      if (t + 1 < n) {
+        stage(buf ^ 1, next.first);
+        staged = next;
+        k_now = k_down, v_now = v_up, e_now = v_e;
+        if (t + 2 < n) {
+          next.first = 0;
+          fetch();
+        }
       }
-      const uint32_t keys = min(n_keys - t * kTile, (uint32_t)kTile);
+      if (busy) {
+        if (e_t != unit || !(v_t > 0.f)) {  // uniform
+          const float alpha = v_t > 0.f ? ldexpf(1.f, e_t - unit) : v_t;
 #pragma unroll
-      for (int kb = 0; kb < kBlocks; kb++) block(buf, kb, c_now, keys);
-    }
-    if (t + 2 < n_tiles) note_top(buf);
-    lds_barrier();
-  }
-  if (idle || wave * 32u + col >= n_rows) return;
-  float lo, hi;
-  swap_pair<32>(l, lo, hi);
-  l = lo + hi;
-  const size_t at = it->part + wave * 32u + col;
-  if (h == 0) p.ml[at] = make_float2(ref, l);
-  const float inv = 1.f / l, down = 1.f / unit;  // (one after the other: l * unit may overflow)
-  float* dst = p.acc + at * D;
-  // Accumulator i of block x: row 8 (i / 4) + 4 h + i % 4 of V's 32 x .., so dim 4 (row % (D / 4))
-  // + row / (D / 4).
+          for (int x = 0; x < kOT; x++) o[x] *= alpha;
+          unit = e_t;
+        }
 #pragma unroll
-  for (int i = 0; i < D / 8; i++) {
-    const int r = 8 * (i >> 2) + 4 * h + (i & 3);
-    if constexpr (D == 128)
-      *reinterpret_cast<float4*>(dst + 4 * r) =
-          make_float4(o[0][i] * inv * down, o[1][i] * inv * down, o[2][i] * inv * down,
-                      o[3][i] * inv * down);
-    else
-      *reinterpret_cast<float4*>(dst + 4 * r) =
-          make_float4(o[0][i] * inv * down, o[0][i + 8] * inv * down, o[1][i] * inv * down,
-                      o[1][i + 8] * inv * down);
+        for (int kb = 0; kb < kBlocks; kb++) block(buf, kb, c_s * k_t, keys);
+      }
+      if (t + 2 < n) note_top(buf);
+      lds_barrier();
+      t++;
+    } while (!last);
+    if (busy) store(part, n_rows, unit);
   }
 }
 
-// Joins the partial results of rows, D / 4 threads a row: o = sum w o_i / sum w, w = l 2^ref.
-template <int D>
+// Joins the partial results of rows: o = sum w o_i / sum w, w = l 2^ref. D / 4 threads over a
+// row's dims, kGroups of them over its pieces.
+template <int D, int kGroups>
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a, SharedPlan p) {
-  constexpr uint32_t kRows = 1024 / D;
-  const uint32_t row = blockIdx.x * kRows + threadIdx.x / (D / 4), e = threadIdx.x % (D / 4);
-  if (row >= a.n_seqs * a.n_heads) return;
-  const uint32_t b = row / a.n_heads, head = row % a.n_heads, G = a.n_kv_heads, m = a.n_heads / G;
-  const uint32_t kvh = head / m, j = head % m;
+  constexpr uint32_t kLanes = D / 4, kRows = 256 / (kLanes * kGroups);
+  __shared__ float4 s_acc[kGroups > 1 ? kRows : 1][kGroups][kLanes];
+  __shared__ float s_sum[kGroups > 1 ? kRows : 1][kGroups];
+  const uint32_t mine = threadIdx.x / (kLanes * kGroups), g = threadIdx.x / kLanes % kGroups;
+  const uint32_t e = threadIdx.x % kLanes, all_rows = a.n_seqs * a.n_heads;
+  const uint32_t row = min(blockIdx.x * kRows + mine, all_rows - 1);
+  const uint32_t b = row / a.n_heads, head = row % a.n_heads, m = a.n_heads / a.n_kv_heads;
+  const uint32_t kvh = head / m, at_row = b * m + head % m, rows = a.n_seqs * m;
   const SharedRecord r = p.record[b];
-  float4* dst = reinterpret_cast<float4*>(a.o + (size_t)row * D) + e;
-  if (r.own_n >= kSharedIdle || r.prefix_n == kSharedRefused) {
-    const bool idle = r.own_n == kSharedIdle && r.prefix_n != kSharedRefused;
-    const float x = idle ? 0.f : __builtin_nanf("");
-    *dst = make_float4(x, x, x, x);
-    return;
-  }
-  const uint32_t n = r.prefix_n + r.own_n;
+  const bool refused = r.own_n == kSharedRefused || r.prefix_n == kSharedRefused;
+  const bool idle = r.own_n == kSharedIdle;
+  const uint32_t n = refused || idle ? 0 : r.prefix_n + r.own_n;
+  const size_t part0 = kvh * shared_parts(rows, p.max_runs);
   auto at = [&](uint32_t i) {
-    return i < r.prefix_n ? (size_t)r.prefix + i * r.prefix_step + kvh * r.prefix_head + j
-                          : (size_t)r.own + ((i - r.prefix_n) * G + kvh) * m + j;
+    if (i == 0 && r.prefix_n > 0) return part0 + at_row;
+    if (i < r.prefix_n)
+      return part0 + 2 * rows + (size_t)(r.prefix_run + i) * kSharedRows + (at_row - r.row0);
+    i -= r.prefix_n;
+    if (i == 0) return part0 + rows + at_row;
+    return part0 + 2 * rows + (size_t)(r.own_run + i) * kSharedRows + head % m;
   };
   float top = -INFINITY;
-  for (uint32_t i = 0; i < n; i++) top = fmaxf(top, p.ml[at(i)].x);
+  for (uint32_t i = e; i < n; i += kLanes) top = fmaxf(top, p.ml[at(i)].x);
+#pragma unroll
+  for (uint32_t x = 1; x < kLanes; x <<= 1) top = fmaxf(top, shfl_xor(top, x));
   float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
 #pragma unroll 4
-  for (uint32_t i = 0; i < n; i++) {
+  for (uint32_t i = g; i < n; i += kGroups) {
     const size_t x = at(i);
     const float2 ml = p.ml[x];
     const float4 y = reinterpret_cast<const float4*>(p.acc + x * D)[e];
@@ -334,8 +441,21 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a, SharedP
     f.x = fmaf(y.x, w, f.x), f.y = fmaf(y.y, w, f.y);
     f.z = fmaf(y.z, w, f.z), f.w = fmaf(y.w, w, f.w);
   }
-  const float inv = n == 0 ? 0.f : 1.f / sum;
-  *dst = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+  if constexpr (kGroups > 1) {
+    s_acc[mine][g][e] = f;
+    if (e == 0) s_sum[mine][g] = sum;
+    __syncthreads();
+    if (g != 0) return;
+    for (int i = 1; i < kGroups; i++) {
+      const float4 y = s_acc[mine][i][e];
+      f.x += y.x, f.y += y.y, f.z += y.z, f.w += y.w;
+      sum += s_sum[mine][i];
+    }
+  }
+  if (blockIdx.x * kRows + mine >= all_rows) return;
+  const float inv = refused ? __builtin_nanf("") : n == 0 ? 0.f : 1.f / sum;
+  reinterpret_cast<float4*>(a.o + (size_t)row * D)[e] =
+      make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
 }
 
 constexpr int kPlanThreads = 1024;
@@ -343,36 +463,35 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedArgs a,
   shared_plan<kPlanThreads>(a, p);
 }
 
-// Two workgroups a CU.
-constexpr uint32_t kSharedSlots = 512;
+#ifndef MERGE_ROWS
+#define MERGE_ROWS 4096
+#endif
+constexpr uint32_t kSharedSlots = 512;  // workgroups: two a CU
 
 static SharedPlan plan_of(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix,
                           uint32_t max_n_keys, uint32_t n_heads, uint32_t n_kv_heads,
-                          uint32_t head_dim, uint64_t* items_out = nullptr) {
+                          uint32_t head_dim, uint64_t* tiles_out = nullptr) {
   SharedPlan p{};
-  const uint64_t G = n_kv_heads, m = n_heads / n_kv_heads;
   p.tile = 4096 / head_dim;
-  p.pieces = std::max(1u, kSharedSlots / n_kv_heads);
-  const uint64_t rows = (uint64_t)n_seqs * m;
-  const uint64_t row_tiles = std::min(n_groups, n_seqs) + rows / kSharedRows;
-  auto most = [&](uint64_t keys) {  // pieces that so many keys are cut into
-    const uint64_t tiles = (keys + p.tile - 1) / p.tile;
-    return (tiles + kSharedLeast - 1) / kSharedLeast;
-  };
-  // Each piece but a row tile's last has the share of one of `pieces`.
-  const uint64_t pre = std::min(p.pieces + row_tiles, row_tiles * most(max_prefix));
-  const uint64_t own = std::min((uint64_t)p.pieces + n_seqs, n_seqs * most(max_n_keys));
-  const uint64_t items = G * (pre + own);
-  p.items = (uint32_t)std::min(items, (uint64_t)0xffffffffu);
-  p.parts = G * (std::min(pre * kSharedRows, rows * std::min((uint64_t)p.pieces + 1, most(max_prefix))) +
-                 own * m);
-  if (items_out) *items_out = items;
+  const uint64_t tile_seqs = kSharedRows / (n_heads / n_kv_heads);
+  const uint64_t row_tiles = std::min(n_groups, n_seqs) + n_seqs / tile_seqs;
+  auto tiles_of = [&](uint64_t keys) { return (keys + p.tile - 1) / p.tile; };
+  const uint64_t tiles = row_tiles * tiles_of(max_prefix) + n_seqs * tiles_of(max_n_keys);
+  p.max_runs = (uint32_t)std::min((uint64_t)std::max(1u, kSharedSlots / n_kv_heads),
+                                  (tiles + kSharedLeast - 1) / kSharedLeast);
+  p.chains = (uint32_t)(row_tiles + n_seqs);
+  if (tiles_out) *tiles_out = tiles;
   return p;
 }
 
 static uint64_t list_bytes(const SharedPlan& p, uint32_t n_seqs) {
-  return 256 + ws_align((uint64_t)p.items * sizeof(SharedItem)) +
+  return 256 + ws_align(p.max_runs * sizeof(SharedRun)) +
+         ws_align((uint64_t)p.chains * sizeof(SharedChain)) +
          ws_align((uint64_t)n_seqs * sizeof(SharedRecord));
+}
+static uint64_t part_rows(const SharedPlan& p, uint32_t n_seqs, uint32_t n_heads,
+                          uint32_t n_kv_heads) {
+  return n_kv_heads * shared_parts(n_seqs * (n_heads / n_kv_heads), p.max_runs);
 }
 
 uint64_t shared_ws_bytes(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix,
@@ -380,15 +499,17 @@ uint64_t shared_ws_bytes(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix
                          uint32_t head_dim) {
   const SharedPlan p = plan_of(n_groups, n_seqs, max_prefix, max_n_keys, n_heads, n_kv_heads,
                                head_dim);
-  return list_bytes(p, n_seqs) + ws_align(p.parts * 8) + ws_align(p.parts * head_dim * 4);
+  const uint64_t parts = part_rows(p, n_seqs, n_heads, n_kv_heads);
+  return list_bytes(p, n_seqs) + ws_align(parts * 8) + ws_align(parts * head_dim * 4);
 }
 
 bool shared_fits(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix, uint32_t max_n_keys,
                  uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
-  uint64_t items;
+  uint64_t tiles;
   const SharedPlan p = plan_of(n_groups, n_seqs, max_prefix, max_n_keys, n_heads, n_kv_heads,
-                               head_dim, &items);
-  return items <= kMaxGroups && p.parts <= 0xffffffffull &&
+                               head_dim, &tiles);
+  return tiles <= 0xfffffffeull && (uint64_t)p.max_runs * n_kv_heads <= kMaxGroups &&
+         shared_parts(n_seqs * (n_heads / n_kv_heads), p.max_runs) <= 0xffffffffull &&
          (uint64_t)n_seqs * n_heads <= kMaxGroups;
 }
 
@@ -398,12 +519,15 @@ static hipError_t launch(const SharedArgs& a, const DecodeFused* fused, uint32_t
   SharedPlan p = plan_of(a.n_groups, a.n_seqs, a.max_prefix, a.max_n_keys, a.n_heads,
                          a.n_kv_heads, a.head_dim);
   uint8_t* w = static_cast<uint8_t*>(ws);
-  p.n_items = reinterpret_cast<uint32_t*>(w);
-  p.item = reinterpret_cast<SharedItem*>(w + 256);
-  p.record = reinterpret_cast<SharedRecord*>(w + 256 + ws_align((uint64_t)p.items * sizeof(SharedItem)));
+  p.n_runs = reinterpret_cast<uint32_t*>(w);
+  p.run = reinterpret_cast<SharedRun*>(w + 256);
+  p.chain = reinterpret_cast<SharedChain*>(w + 256 + ws_align(p.max_runs * sizeof(SharedRun)));
+  p.record = reinterpret_cast<SharedRecord*>(
+      reinterpret_cast<uint8_t*>(p.chain) + ws_align((uint64_t)p.chains * sizeof(SharedChain)));
   w += list_bytes(p, a.n_seqs);
   p.ml = reinterpret_cast<float2*>(w);
-  p.acc = reinterpret_cast<float*>(w + ws_align(p.parts * 8));
+  p.acc = reinterpret_cast<float*>(
+      w + ws_align(part_rows(p, a.n_seqs, a.n_heads, a.n_kv_heads) * 8));
   hipError_t e;
   if (fused != nullptr) {
     e = launch_shared_prologue(a, p, *fused, q_stride, kv_stride, st);
@@ -413,12 +537,20 @@ static hipError_t launch(const SharedArgs& a, const DecodeFused* fused, uint32_t
   }
   if (e != hipSuccess) return e;
   const float scale = (float)(kLog2e / sqrt((double)D));
-  hipLaunchKernelGGL(shared_attn_kernel<D>, dim3(p.items), dim3(kShThreads), 0, st, a, p, scale);
+  hipLaunchKernelGGL(shared_attn_kernel<D>, dim3(p.max_runs * a.n_kv_heads), dim3(kShThreads), 0,
+                     st, a, p, scale);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  constexpr uint32_t kRows = 1024 / D;
-  hipLaunchKernelGGL(shared_merge_kernel<D>, dim3((a.n_seqs * a.n_heads + kRows - 1) / kRows),
-                     dim3(256), 0, st, a, p);
+  const uint32_t rows = a.n_seqs * a.n_heads;
+  auto merge = [&](auto kernel, uint32_t groups) {
+    const uint32_t per = 1024 / (D * groups);
+    hipLaunchKernelGGL(kernel, dim3((rows + per - 1) / per), dim3(256), 0, st, a, p);
+  };
+  // (With more rows each has fewer pieces, and the GPU is full without dividing them.)
+  if (rows <= MERGE_ROWS)
+    merge(shared_merge_kernel<D, 1024 / D>, 1024 / D);
+  else
+    merge(shared_merge_kernel<D, 1>, 1);
   return hipGetLastError();
 }
 

@@ -16,185 +16,247 @@ struct SharedArgs {
 };
 
 // Rows of q that meet the same keys are taken together: the m = n_heads / n_kv_heads query
-// heads of a kv head, of every sequence of a group (its row of q is sequence * m + head of the
-// kv head), in row tiles of 128, and the m of one sequence for its own keys. An item is a row tile
-// and a piece of its keys for one kv head; its partial results are rows `part` .. of them.
+// heads of a kv head, of every sequence of a group (a row is sequence * m + head of the kv
+// head), in row tiles of up to 128 rows of whole sequences, and the m of one sequence for its
+// own keys. A chain is a row tile and its keys, in tiles. The tiles of all chains, one after the
+// other, are cut into runs of the same length: a run is one workgroup's work for one kv
+// head, whatever the lengths of the chains in it.
 constexpr uint32_t kSharedRows = 128;
-struct alignas(16) SharedItem {
-  uint64_t key_row;  // of the caches
-  uint32_t n_keys, row0, n_rows, part, kvh, pad;
+struct alignas(16) SharedChain {
+  uint64_t key_row;               // of the caches
+  uint32_t n_keys, row0, n_rows;
+  uint32_t start;                 // its first tile among all
+  uint32_t first_run;             // the run that holds it
+  uint32_t kind;                  // kSharedOwn: a sequence's own keys; kSharedOnce: read once
 };
-// Where a sequence's partial results lie: of piece p, kv head h and head j of it at
-// prefix + p * prefix_step + h * prefix_head + j and own + (p * n_kv_heads + h) * m + j.
+constexpr uint32_t kSharedOwn = 1, kSharedOnce = 2;
+struct alignas(16) SharedRun {
+  uint32_t chain, tile0, tile1, pad;
+};
+// A sequence's partial results: prefix_n of its prefix (the first by run prefix_run, for a row
+// tile whose first row is row0) and own_n of its own keys.
 struct alignas(16) SharedRecord {
-  uint32_t prefix, prefix_n, prefix_step, prefix_head, own, own_n, pad[2];
+  uint32_t prefix_run, prefix_n, row0, own_run, own_n, pad[3];
 };
 constexpr uint32_t kSharedRefused = 0xffffffffu, kSharedIdle = 0xfffffffeu;  // counts
 
 struct SharedPlan {
-  uint32_t tile;     // keys of a tile
-  uint32_t pieces;   // of a kv head's tiles, over all of its row tiles: about so many items
-  uint32_t items;    // at most
-  uint64_t parts;    // rows of partial results, at most
-  uint32_t* n_items;
-  SharedItem* item;
+  uint32_t tile;      // keys of a tile
+  uint32_t max_runs;  // of a kv head
+  uint32_t chains;    // at most
+  uint32_t* n_runs;   // of a kv head
+  SharedRun* run;
+  SharedChain* chain;
   SharedRecord* record;
-  float2* ml;        // (reference, sum) of a row
-  float* acc;        // its output, normalised
+  float2* ml;         // (reference, sum) of a partial result's row
+  float* acc;         // its output, normalised
 };
 
-constexpr uint32_t kSharedLeast = 2;  // tiles of an item at least, where there are as many
-
-// Sum over the workgroup, and over the threads before this one, in 64 bits.
-template <int kWaves>
-__device__ __forceinline__ uint64_t shared_scan(uint64_t v, uint64_t* s_wave, uint64_t& before) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t scan = v;
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) {
-    const uint64_t y = __shfl_up((unsigned long long)scan, x, kWave);
-    if (lane >= x) scan += y;
-  }
-  __syncthreads();  // s_wave may still be read
-  if (lane == 63) s_wave[wave] = scan;
-  __syncthreads();
-  uint64_t total = 0;
-  before = scan - v;
-  for (int w = 0; w < kWaves; w++) {
-    if (w < wave) before += s_wave[w];
-    total += s_wave[w];
-  }
-  return total;
+// Rows of partial results of a kv head: the first piece of every row's prefix, then of its
+// own keys; a run that does not begin with a chain has room of its own for the first (only that
+// piece is not the chain's first).
+__host__ __device__ __forceinline__ uint64_t shared_parts(uint32_t rows, uint32_t runs) {
+  return 2ull * rows + (uint64_t)runs * kSharedRows;
 }
 
-// The items of a call and the sequences' records, by one workgroup. Lengths come from the
-// device, so the pieces are cut by the work there is: `pieces` of them over all row tiles of
-// a kv head, each of as many tiles, a row tile's last one shorter. All row tiles of a group
-// have the same pieces, neighbours in the list, so that they read a piece's keys at the same time.
+constexpr uint32_t kSharedLeast = 2;  // tiles of a run at least
+
+// The run that holds tile x of `tiles`, cut into `runs`: run r has the tiles from tiles * r / runs on.
+__device__ __forceinline__ uint32_t shared_run_of(uint32_t x, uint32_t tiles, uint32_t runs) {
+  const uint64_t n = ((uint64_t)x + 1) * runs - 1;
+  return n >> 32 ? (uint32_t)(n / tiles) : (uint32_t)n / tiles;
+}
+__device__ __forceinline__ uint32_t shared_run_start(uint32_t r, uint32_t tiles, uint32_t runs) {
+  const uint64_t n = (uint64_t)tiles * r;
+  return n >> 32 ? (uint32_t)(n / runs) : (uint32_t)n / runs;
+}
+
+// Exclusive sums over the workgroup's threads of two pairs (chains, tiles); the totals come back
+// in a and b.
+struct SharedPair {
+  uint32_t chains, tiles;
+};
+template <int kWaves>
+__device__ __forceinline__ void shared_scan(SharedPair& a, SharedPair& b, uint4* s_wave,
+                                            SharedPair& before_a, SharedPair& before_b) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint4 v = make_uint4(a.chains, a.tiles, b.chains, b.tiles);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    const uint32_t p = __shfl_up(v.x, x, kWave), q = __shfl_up(v.y, x, kWave);
+    const uint32_t r = __shfl_up(v.z, x, kWave), s = __shfl_up(v.w, x, kWave);
+    if (lane >= x) v.x += p, v.y += q, v.z += r, v.w += s;
+  }
+  __syncthreads();  // s_wave may still be read
+  if (lane == 63) s_wave[wave] = v;
+  __syncthreads();
+  before_a = {v.x - a.chains, v.y - a.tiles};
+  before_b = {v.z - b.chains, v.w - b.tiles};
+  a = b = {0, 0};
+  for (int w = 0; w < kWaves; w++) {
+    const uint4 y = s_wave[w];
+    if (w < wave) {
+      before_a.chains += y.x, before_a.tiles += y.y;
+      before_b.chains += y.z, before_b.tiles += y.w;
+    }
+    a.chains += y.x, a.tiles += y.y, b.chains += y.z, b.tiles += y.w;
+  }
+}
+
+// A call's chains, runs and records, by one workgroup, from the lengths on the device. The chains
+// of the groups come first, each group's row tiles one after the other.
 template <int kThreads>
 __device__ __forceinline__ void shared_plan(const SharedArgs& a, const SharedPlan& p) {
   constexpr int kWaves = kThreads / 64;
-  __shared__ uint64_t s_wave[kWaves];
-  __shared__ uint32_t s_first[kThreads + 1], s_off[kThreads + 1], s_n[kThreads], s_part[kThreads];
+  __shared__ uint4 s_wave[kWaves];
+  __shared__ uint32_t s_chain[kThreads], s_start[kThreads], s_off[kThreads + 1], s_keys[kThreads];
   __shared__ uint32_t s_bad;
-  const uint32_t t = threadIdx.x, G = a.n_kv_heads, m = a.n_heads / G;
+  const uint32_t t = threadIdx.x, m = a.n_heads / a.n_kv_heads;
+  const uint32_t tile_seqs = kSharedRows / m;  // sequences of a row tile
   auto tiles_of = [&](uint32_t keys) { return keys / p.tile + (keys % p.tile != 0); };
-  auto row_tiles = [&](uint32_t seqs) { return (seqs * m + kSharedRows - 1) / kSharedRows; };
+  auto row_tiles = [&](uint32_t seqs) { return seqs / tile_seqs + (seqs % tile_seqs != 0); };
+  struct Group {
+    uint32_t lo, hi, keys;  // keys = 0: refused too
+    bool refused;
+  };
+  auto group = [&](uint32_t g) {
+    Group x{0, 0, 0, false};
+    if (g < a.n_groups) {
+      x.lo = a.seq_off[g], x.hi = a.seq_off[g + 1], x.keys = a.n_prefix[g];
+      x.refused = x.keys > a.max_prefix;
+      if (x.refused) x.keys = 0;
+    }
+    return x;
+  };
+  auto group_pair = [&](const Group& x) {
+    const uint32_t nt = tiles_of(x.keys), rts = nt ? row_tiles(x.hi - x.lo) : 0;
+    return SharedPair{rts, rts * nt};
+  };
+  auto own_keys = [&](uint32_t b) {  // 0xffffffff: refused
+    if (b >= a.n_seqs) return 0u;
+    const uint32_t n = a.n_keys[b];
+    return n > a.max_n_keys ? kSharedRefused : n;
+  };
+  auto own_pair = [&](uint32_t n) {
+    const uint32_t nt = n == kSharedRefused ? 0 : tiles_of(n);
+    return SharedPair{nt > 0, nt};
+  };
   if (t == 0) s_bad = 0;
   __syncthreads();
-  uint64_t work = 0, before;
+  // Whole sums first; of the first group and sequence of a thread what it has read stays.
+  const Group mine = group(t);
+  const uint32_t mine_own = own_keys(t);
+  SharedPair groups{0, 0}, owns{0, 0}, before_g, before_o;
   for (uint32_t g = t; g < a.n_groups; g += kThreads) {
-    const uint32_t lo = a.seq_off[g], hi = a.seq_off[g + 1], n = a.n_prefix[g];
-    if (lo > hi || hi > a.n_seqs)
+    const Group x = g == t ? mine : group(g);
+    if (x.lo > x.hi || x.hi > a.n_seqs) {
       s_bad = 1;
-    else if (n <= a.max_prefix)
-      work += (uint64_t)row_tiles(hi - lo) * tiles_of(n);
+    } else {
+      const SharedPair y = group_pair(x);
+      groups.chains += y.chains, groups.tiles += y.tiles;
+    }
   }
   for (uint32_t b = t; b < a.n_seqs; b += kThreads) {
-    const uint32_t n = a.n_keys[b];
-    if (n <= a.max_n_keys) work += tiles_of(n);
+    const SharedPair y = own_pair(b == t ? mine_own : own_keys(b));
+    owns.chains += y.chains, owns.tiles += y.tiles;
   }
-  work = shared_scan<kWaves>(work, s_wave, before);
-  if (s_bad) {  // (seen by all: the sum's barriers)
+  shared_scan<kWaves>(groups, owns, s_wave, before_g, before_o);
+  if (s_bad) {  // (seen by all: the sums' barriers)
     for (uint32_t b = t; b < a.n_seqs; b += kThreads)
-      p.record[b] = SharedRecord{0, kSharedRefused, 0, 0, 0, kSharedRefused, {0, 0}};
-    if (t == 0) *p.n_items = 0;
+      p.record[b] = SharedRecord{0, kSharedRefused, 0, 0, kSharedRefused, {0, 0, 0}};
+    if (t == 0) *p.n_runs = 0;
     return;
   }
-  const uint64_t share = (work + p.pieces - 1) / p.pieces;
-  const uint32_t per = share > kSharedLeast ? (uint32_t)share : kSharedLeast;
-  uint64_t item0 = 0, part0 = 0;
+  const uint32_t tiles = groups.tiles + owns.tiles;
+  const uint32_t runs = min(p.max_runs, (tiles + kSharedLeast - 1) / kSharedLeast);
+  if (t == 0) *p.n_runs = runs;
 
-  // The entry of s_first that an item lies in, of n.
-  auto find = [&](const uint32_t* first, uint32_t n, uint32_t x) {
+  // The last entry of a rising list of n that is not above x.
+  auto find = [&](const uint32_t* list, uint32_t n, uint32_t x) {
     uint32_t lo = 0, hi = n;
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
-      if (first[mid] <= x) lo = mid; else hi = mid;
+      if (list[mid] <= x) lo = mid; else hi = mid;
     }
     return lo;
   };
-  for (uint32_t g0 = 0; g0 < a.n_groups; g0 += kThreads) {
-    const uint32_t n_here = min((uint32_t)kThreads, a.n_groups - g0), g = g0 + t;
-    uint32_t lo = 0, hi = 0, n = 0, pieces = 0;
-    if (t < n_here) {
-      lo = a.seq_off[g], hi = a.seq_off[g + 1], n = a.n_prefix[g];
-      if (n <= a.max_prefix && hi > lo) pieces = (tiles_of(n) + per - 1) / per;
+  auto put_runs = [&](uint32_t from, uint32_t to, auto chain_at) {  // those that start there
+    for (uint32_t r = t; r < runs; r += kThreads) {
+      const uint32_t x = shared_run_start(r, tiles, runs);
+      if (x >= from && x < to)
+        p.run[r] = SharedRun{chain_at(x), x, shared_run_start(r + 1, tiles, runs), 0};
     }
-    uint64_t at_item, at_part;
-    const uint32_t items = pieces * row_tiles(hi - lo) * G;
-    const uint64_t all = shared_scan<kWaves>(items, s_wave, at_item);
-    const uint64_t parts = shared_scan<kWaves>((uint64_t)pieces * (hi - lo) * m * G, s_wave, at_part);
-    s_first[t] = (uint32_t)at_item;
-    if (t < n_here) s_off[t] = lo;
-    s_n[t] = n > a.max_prefix ? kSharedRefused : pieces;
-    s_part[t] = (uint32_t)(part0 + at_part);
-    if (t + 1 == n_here) s_off[n_here] = hi;
+  };
+  uint32_t chain0 = 0, tile0 = 0;
+  for (uint32_t g0 = 0; g0 < a.n_groups; g0 += kThreads) {
+    const uint32_t n_here = min((uint32_t)kThreads, a.n_groups - g0);
+    const Group x = g0 == 0 ? mine : group(g0 + t);
+    SharedPair here = t < n_here ? group_pair(x) : SharedPair{0, 0}, none{0, 0};
+    shared_scan<kWaves>(here, none, s_wave, before_g, before_o);
+    s_chain[t] = before_g.chains, s_start[t] = tile0 + before_g.tiles;
+    s_keys[t] = x.refused ? kSharedRefused : x.keys;
+    if (t < n_here) s_off[t] = x.lo;
+    if (t + 1 == n_here) s_off[n_here] = x.hi;
     __syncthreads();
-    for (uint32_t i = t; i < (uint32_t)all; i += kThreads) {
-      // (The last group that starts at or before item i: empty ones share its first item.)
-      const uint32_t e = find(s_first, n_here, i);
-      const uint32_t x = i - s_first[e], kvh = x % G;
-      const uint32_t rows = (s_off[e + 1] - s_off[e]) * m, rts = (rows + kSharedRows - 1) / kSharedRows;
-      const uint32_t rt = x / G % rts, piece = x / G / rts;
-      const uint32_t keys = a.n_prefix[g0 + e], nt = tiles_of(keys);
-      const uint32_t t0 = (uint32_t)((uint64_t)nt * piece / s_n[e]);
-      const uint32_t t1 = (uint32_t)((uint64_t)nt * (piece + 1) / s_n[e]);
-      const uint64_t end = min((uint64_t)t1 * p.tile, (uint64_t)keys);
-      SharedItem item;
-      item.key_row = a.prefix_row[g0 + e] + (uint64_t)t0 * p.tile;
-      item.n_keys = (uint32_t)(end - (uint64_t)t0 * p.tile);
-      item.row0 = s_off[e] * m + rt * kSharedRows;
-      item.n_rows = min(kSharedRows, rows - rt * kSharedRows);
-      item.part = s_part[e] + (piece * G + kvh) * rows + rt * kSharedRows;
-      item.kvh = kvh, item.pad = 0;
-      p.item[item0 + i] = item;
+    for (uint32_t i = t; i < here.chains; i += kThreads) {
+      // (Of entries without chains, which share the next one's first, find passes all.)
+      const uint32_t e = find(s_chain, n_here, i), rt = i - s_chain[e], nt = tiles_of(s_keys[e]);
+      const uint32_t seq0 = s_off[e] + rt * tile_seqs, start = s_start[e] + rt * nt;
+      SharedChain c;
+      c.key_row = a.prefix_row[g0 + e];
+      c.n_keys = s_keys[e], c.row0 = seq0 * m;
+      c.n_rows = min(tile_seqs, s_off[e + 1] - seq0) * m;
+      c.start = start, c.first_run = shared_run_of(start, tiles, runs);
+      c.kind = s_off[e + 1] - s_off[e] <= tile_seqs ? kSharedOnce : 0;
+      p.chain[chain0 + i] = c;
     }
     for (uint32_t b = s_off[0] + t; b < s_off[n_here]; b += kThreads) {
-      const uint32_t e = find(s_off, n_here, b), rows = (s_off[e + 1] - s_off[e]) * m;
+      const uint32_t e = find(s_off, n_here, b), keys = s_keys[e];
+      const uint32_t nt = keys == kSharedRefused ? 0 : tiles_of(keys);
+      const uint32_t rt = (b - s_off[e]) / tile_seqs, start = s_start[e] + rt * nt;
       SharedRecord& r = p.record[b];
-      r.prefix = s_part[e] + (b - s_off[e]) * m, r.prefix_n = s_n[e];
-      r.prefix_step = rows * G, r.prefix_head = rows;
+      r.row0 = (s_off[e] + rt * tile_seqs) * m;
+      r.prefix_n = keys == kSharedRefused ? keys : 0;
+      if (nt > 0) {
+        r.prefix_run = shared_run_of(start, tiles, runs);
+        r.prefix_n = shared_run_of(start + nt - 1, tiles, runs) - r.prefix_run + 1;
+      }
     }
-    item0 += all, part0 += parts;
+    put_runs(tile0, tile0 + here.tiles, [&](uint32_t x) {
+      const uint32_t e = find(s_start, n_here, x);
+      return chain0 + s_chain[e] + (x - s_start[e]) / tiles_of(s_keys[e]);
+    });
+    chain0 += here.chains, tile0 += here.tiles;
     __syncthreads();
   }
+  const uint32_t off_0 = a.seq_off[0], off_n = a.seq_off[a.n_groups];
   for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += kThreads) {
     const uint32_t n_here = min((uint32_t)kThreads, a.n_seqs - b0), b = b0 + t;
-    uint32_t n = 0, pieces = 0;
-    if (t < n_here) {
-      n = a.n_keys[b];
-      if (n <= a.max_n_keys) pieces = (tiles_of(n) + per - 1) / per;
-    }
-    uint64_t at_item;
-    const uint64_t all = shared_scan<kWaves>((uint64_t)pieces * G, s_wave, at_item);
-    const uint32_t part = (uint32_t)(part0 + at_item * m);
-    s_first[t] = (uint32_t)at_item, s_n[t] = pieces, s_part[t] = part;
+    const uint32_t n = b0 == 0 ? mine_own : own_keys(b);
+    SharedPair here = t < n_here ? own_pair(n) : SharedPair{0, 0}, none{0, 0};
+    const uint32_t nt = here.tiles;
+    shared_scan<kWaves>(here, none, s_wave, before_g, before_o);
+    const uint32_t start = tile0 + before_g.tiles;
+    s_chain[t] = before_g.chains, s_start[t] = start;
     if (t < n_here) {
       SharedRecord& r = p.record[b];
-      r.own = part;
-      r.own_n = n > a.max_n_keys ? kSharedRefused : n == 0 && a.step ? kSharedIdle : pieces;
-      if (b < a.seq_off[0] || b >= a.seq_off[a.n_groups]) r.prefix_n = 0;
+      if (b < off_0 || b >= off_n) r.prefix_n = 0;
+      r.own_n = n == kSharedRefused ? n : n == 0 && a.step ? kSharedIdle : 0;
+      if (nt > 0) {
+        const uint32_t first = shared_run_of(start, tiles, runs);
+        r.own_run = first;
+        r.own_n = shared_run_of(start + nt - 1, tiles, runs) - first + 1;
+        p.chain[chain0 + before_g.chains] =
+            SharedChain{a.seq_row_off[b], n, b * m, m, start, first, kSharedOwn | kSharedOnce};
+      }
     }
     __syncthreads();
-    for (uint32_t i = t; i < (uint32_t)all; i += kThreads) {
-      const uint32_t e = find(s_first, n_here, i), x = i - s_first[e];
-      const uint32_t kvh = x % G, piece = x / G, keys = a.n_keys[b0 + e], nt = tiles_of(keys);
-      const uint32_t t0 = (uint32_t)((uint64_t)nt * piece / s_n[e]);
-      const uint32_t t1 = (uint32_t)((uint64_t)nt * (piece + 1) / s_n[e]);
-      const uint64_t end = min((uint64_t)t1 * p.tile, (uint64_t)keys);
-      SharedItem item;
-      item.key_row = a.seq_row_off[b0 + e] + (uint64_t)t0 * p.tile;
-      item.n_keys = (uint32_t)(end - (uint64_t)t0 * p.tile);
-      item.row0 = (b0 + e) * m, item.n_rows = m;
-      item.part = s_part[e] + x * m;
-      item.kvh = kvh, item.pad = 0;
-      p.item[item0 + i] = item;
-    }
-    item0 += all, part0 += all * m;
+    put_runs(tile0, tile0 + here.tiles, [&](uint32_t x) {
+      return chain0 + s_chain[find(s_start, n_here, x)];
+    });
+    chain0 += here.chains, tile0 += here.tiles;
     __syncthreads();
   }
-  if (t == 0) *p.n_items = (uint32_t)item0;
 }
 
 // What a sequence sees.
@@ -229,7 +291,7 @@ __device__ __forceinline__ SharedSeq shared_seq(const SharedArgs& a, uint32_t b)
 uint64_t shared_ws_bytes(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix,
                          uint32_t max_n_keys, uint32_t n_heads, uint32_t n_kv_heads,
                          uint32_t head_dim);
-// Whether a call's launches and its numbers of rows and items (32 bits) hold it.
+// Whether a call's launches and its numbers of rows and tiles (32 bits) hold it.
 bool shared_fits(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix, uint32_t max_n_keys,
                  uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
 // fused: the step's raw rows and gains (null: attention alone), q rows q_stride floats

@@ -4,8 +4,9 @@
 // f32 keys and values meet q and the softmax weights on f16 matrix products of two parts each:
 // x = h + l, h = x rounded to f16 and l = x - h likewise (22 bits), and x y = h h' + h l' +
 // l h', all sums in f32. The product left out, l l', is at most 2^-22 of x y. Operands are
-// scaled by powers of two first: q by its row's largest, K by its tile's largest (both
-// undone in the score's factor), V by a factor that moves with its tiles' largest.
+// scaled by powers of two first: q by its row's largest, K and V by factors that stay while the
+// tiles' largest values suit f16 with them (K's and q's are undone in the score's factor, V's
+// at the end).
 //
 // A workgroup takes a run of tiles, 32 keys each (64 of 64-wide heads) that meet up to 128
 // rows of q; four waves of 32 rows, two workgroups a CU. A tile's K and V come through
@@ -14,6 +15,11 @@
 // S^T = K Q^T and O^T += V^T P^T on 32x32x16: a column is a row of q, and P^T is taken from the
 // S^T accumulators as they lie, because V's keys are put in the order in which a lane holds its
 // scores. Waves without rows (a sequence's own keys meet few) only stage.
+//
+// What bounds it: with few rows, reading K and V; with many, how fast a wave gets through its
+// instructions, for a vector instruction of a lone wave takes 7 to 14 cycles and two waves share
+// a SIMD. So the split of the next tile stands among the products of the scores, four
+// instructions to a product, and a tile is split before its largest values are known.
 #include <algorithm>
 
 #include "shared.hpp"
@@ -41,8 +47,23 @@ template <int D>
 struct alignas(16) SharedLds {
   static constexpr int kPart = 8192;  // bytes of a tile's part
   uint8_t k[2][2][kPart], v[2][2][kPart];
-  float top[2][2][kShThreads / 64];  // the largest |k| and |v| of a tile, by wave
+  float top[2][kShThreads / 64];             // the largest |k| and |v| of a tile, by wave
+  alignas(16) uint32_t fit[2][kShThreads / 64];  // how each wave's k and v fit the factors
 };
+// Values with their factor: none (0), too large for f16, all too small for two parts of it.
+constexpr uint32_t kFits = 1, kLarge = 2, kSmall = 4;
+__device__ __forceinline__ uint32_t shared_fit(float top, float up) {  // top: of the lane, >= 0
+  const float x = top * up;
+  const uint64_t large = __ballot(!(x < 65000.f)), fits = __ballot(x >= 1.f);
+  const uint64_t some = __ballot(top > 0.f);
+  return large ? kLarge : fits ? kFits : some ? kSmall : 0;
+}
+__device__ __forceinline__ bool shared_misfit(const uint32_t (&of)[kShThreads / 64]) {
+  // (k's in the low half, v's above.)
+  const uint4 fit = *reinterpret_cast<const uint4*>(of);
+  const uint32_t x = uniform(fit.x | fit.y | fit.z | fit.w), k = x & 0xffff, v = x >> 16;
+  return ((k | v) & kLarge) || k == kSmall || v == kSmall;
+}
 
 // f16(x s) and f16(y s), and what is left of x s and y s (a difference that is formed exactly),
 // rounded likewise; s a power of two.
@@ -65,6 +86,9 @@ __device__ __forceinline__ float wave_max(float v) {
 __device__ __forceinline__ float uniform_f(float v) {  // in a scalar register
   return __builtin_bit_cast(float, uniform(__builtin_bit_cast(uint32_t, v)));
 }
+__device__ __forceinline__ int exponent(float v) {  // of v >= 0: -127 for 0, 128 for infinity
+  return (int)(__builtin_bit_cast(uint32_t, v) >> 23) - 127;
+}
 __device__ __forceinline__ float power_of_two(int e) {  // 2^e, |e| < 127
   return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
 }
@@ -78,6 +102,8 @@ __device__ __forceinline__ uint32_t here(uint32_t v) {
 
 // What of a tile is known when its loads are sent, and goes with it.
 struct SharedTile {
+  uint64_t at;            // floats: its first row in the caches
+  uint32_t once;          // read by this workgroup alone
   uint32_t keys;          // it holds
   uint32_t row0, n_rows;  // they meet
   uint32_t part;          // where the rows' results go
@@ -103,20 +129,33 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
 
   // The chain that tiles are fetched from.
   uint32_t e = uniform(p.run[run].chain), tile = uniform(p.run[run].tile0);
-  const uint32_t end = uniform(p.run[run].tile1);
+  const uint32_t end = uniform(p.run[run + 1].tile0);
   uint64_t key_row;
-  uint32_t n_keys, in_chain, kind;
-  SharedTile next;
+  uint32_t n_keys, in_chain;
+  SharedTile next;  // the last tile that was sent for
   auto open = [&] {
     typedef const __attribute__((address_space(4))) uint32_t* ConstPtr;
     const ConstPtr c = (ConstPtr)(uintptr_t)(p.chain + e);
     key_row = uniform(c[0]) | (uint64_t)uniform(c[1]) << 32;
     n_keys = uniform(c[2]), next.row0 = uniform(c[3]), next.n_rows = uniform(c[4]);
     in_chain = uniform(tile - c[5]);
-    kind = uniform(c[7]);
+    const uint32_t kind = uniform(c[7]);
+    next.once = kind & kSharedOnce;
     next.part = uniform(c[6]) == run ? next.row0 + (kind & kSharedOwn ? rows : 0)
-                            : 2 * rows + run * kSharedRows;
+                                     : 2 * rows + run * kSharedRows;
     next.first = 1;
+  };
+  auto advance = [&] {  // next: one tile on
+    if (next.last) {
+      e++;
+      open();
+    } else {
+      next.first = 0;
+    }
+    next.at = ((key_row + (uint64_t)in_chain * kTile) * G + kvh) * D;
+    next.keys = uniform(min(n_keys - in_chain * kTile, (uint32_t)kTile));
+    next.last = uniform(tile + 1 == end || (in_chain + 1) * kTile >= n_keys ? 1 : 0);
+    tile++, in_chain++;
   };
 
   // Staging: a thread loads chunk c of four rows of K, and of four rows of V that are
@@ -135,22 +174,15 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
   const uint32_t k_off = k_key * stride + 16 * c, v_off = v_key * stride + 16 * c;
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
   u4 rk[4], rv[4];
-  // Sends the loads of the next tile; what goes with it is in `next` then.
-  auto fetch = [&] {
-    if (next.last) {
-      e++;
-      open();
-    }
-    const size_t at = ((key_row + (uint64_t)in_chain * kTile) * G + kvh) * D;
-    next.keys = min(n_keys - in_chain * kTile, (uint32_t)kTile);
+  auto fetch = [&](const SharedTile& x) {
     // (Rows behind the last read as zeros: the descriptors end with the tile's last row.)
-    const uint32_t bytes = (next.keys - 1) * stride + D * 4;
-    const auto ks = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.kcache + at), 0, bytes,
-                                                      0x00020000);
-    const auto vs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.vcache + at), 0, bytes,
-                                                      0x00020000);
+    const uint32_t bytes = (x.keys - 1) * stride + D * 4;
+    const auto ks = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.kcache + x.at), 0,
+                                                      bytes, 0x00020000);
+    const auto vs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.vcache + x.at), 0,
+                                                      bytes, 0x00020000);
     const uint32_t ko = here(k_off), vo = here(v_off);
-    if (kind & kSharedOnce) {  // not to stay in the caches
+    if (x.once) {  // not to stay in the caches
 #pragma unroll
       for (int i = 0; i < 4; i++)
         rk[i] = __builtin_amdgcn_raw_buffer_load_b128(ks, ko + kGroups * i * stride, 0, 2);
@@ -165,11 +197,47 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
       for (int i = 0; i < 4; i++)
         rv[i] = __builtin_amdgcn_raw_buffer_load_b128(vs, vo + i * stride, 0, 0);
     }
-    next.last = uniform(tile + 1 == end || (in_chain + 1) * kTile >= n_keys ? 1 : 0);
-    tile++, in_chain++;
   };
   auto f = [](uint32_t x) { return __builtin_bit_cast(float, x); };
-  auto note_top = [&](int buf) {
+  // The factors of the tile in LDS, 2^k_e and 2^v_e. They stay while a tile's largest values lie
+  // in 2^0 .. 2^16 with them, or are 0: then two parts in f16 are off by 2^-25 of the largest
+  // at most. So a tile need not be seen as a whole before it is split: each wave
+  // notes how its part fits, and the tile is done again if need be.
+  int k_e = 0, v_e = 0, v_low = 0;  // v_low: the least v_e of the chain
+  // An eighth of the tile in registers into LDS.
+  auto stage_part = [&](int buf, int part, float k_up, float v_up) {
+    const int i = part & 3;
+    float x, y, z, w;
+    if (part < 4)
+      x = f(rk[i][0]), y = f(rk[i][1]), z = f(rk[i][2]), w = f(rk[i][3]);
+    else
+      x = f(rv[0][i]), y = f(rv[1][i]), z = f(rv[2][i]), w = f(rv[3][i]);
+    const float up = part < 4 ? k_up : v_up;
+    uint2 hi, lo;
+    hi.x = first_part(x, y, up), hi.y = first_part(z, w, up);
+    lo.x = second_part(x, y, up, hi.x), lo.y = second_part(z, w, up, hi.y);
+    uint8_t* at = part < 4 ? &sh.k[0][0][(k_to + buf * (2 * kPart)) ^ (i << 5)] + 512 * i
+                           : &sh.v[0][0][v_to + buf * (2 * kPart)] + 2048 * i;
+    *reinterpret_cast<uint2*>(at) = hi;
+    *reinterpret_cast<uint2*>(at + kPart) = lo;
+  };
+  auto note_fit = [&](int buf) {
+    float k = 0.f, v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        k = fmaxf(k, fabsf(f(rk[i][j])));
+        v = fmaxf(v, fabsf(f(rv[i][j])));
+      }
+    sh.fit[buf][wave] =
+        shared_fit(k, power_of_two(k_e)) | shared_fit(v, power_of_two(v_e)) << 16;
+  };
+  // The factors from the tile in registers, 2^10 .. 2^11 its largest values with them, and
+  // the tile into LDS; by all waves. (V's is at most 2^60 of the chain's least, so that
+  // accumulators stay finite.) Whether V holds an infinity: its rows are NaN, and the factor
+  // is as before.
+  auto anchor = [&](int buf, bool first) {
     float k = 0.f, v = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -179,45 +247,20 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
         v = fmaxf(v, fabsf(f(rv[i][j])));
       }
     k = wave_max(k), v = wave_max(v);
-    if (lane == 0) sh.top[buf][0][wave] = k, sh.top[buf][1][wave] = v;
-  };
-  // K's factor of the tile in registers, undone (k_down), and V's, 2^v_e (or NaN for a tile with
-  // an infinity, whose rows are NaN then). V's stays while the tile's largest value lies in
-  // 2^7 .. 2^15 with it, so that accumulators seldom change theirs.
-  float k_down = 0.f, v_up = 1.f;
-  int v_e = 0;
-  auto stage = [&](int buf, bool first) {
-    const float4 kt = *reinterpret_cast<const float4*>(sh.top[buf][0]);
-    const float4 vt = *reinterpret_cast<const float4*>(sh.top[buf][1]);
-    const RowScale rs = row_scale(uniform_f(fmaxf(fmaxf(kt.x, kt.y), fmaxf(kt.z, kt.w))));
-    k_down = rs.down;
-    const float top = uniform_f(fmaxf(fmaxf(vt.x, vt.y), fmaxf(vt.z, vt.w)));
-    const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, now = e + v_e;
-    if (first)
-      v_e = min(12 - max(e, -100), 112);
-    else if ((now < 7 || now > 14) && e != -127)  // 2^12; by at most 2^60 up: finite accumulators
-      v_e = max(min(12 - max(e, -100), v_e + 60), -115);
-    v_up = e < 128 ? power_of_two(v_e) : __builtin_nanf("");
+    if (lane == 0) sh.top[0][wave] = k, sh.top[1][wave] = v;
+    lds_barrier();
+    const float4 kt = *reinterpret_cast<const float4*>(sh.top[0]);
+    const float4 vt = *reinterpret_cast<const float4*>(sh.top[1]);
+    const int ke = exponent(uniform_f(fmaxf(fmaxf(kt.x, kt.y), fmaxf(kt.z, kt.w))));
+    const int ve = exponent(uniform_f(fmaxf(fmaxf(vt.x, vt.y), fmaxf(vt.z, vt.w))));
+    if (ke != -127 && ke != 128) k_e = max(10 - max(ke, -100), -115);
+    if (ve != -127 && ve != 128)
+      v_e = max(min(10 - max(ve, -100), first ? 110 : v_low + 60), -115);
+    v_low = first ? v_e : min(v_low, v_e);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float x = f(rk[i][0]), y = f(rk[i][1]), z = f(rk[i][2]), w = f(rk[i][3]);
-      uint2 hi, lo;
-      hi.x = first_part(x, y, rs.up), hi.y = first_part(z, w, rs.up);
-      lo.x = second_part(x, y, rs.up, hi.x), lo.y = second_part(z, w, rs.up, hi.y);
-      uint8_t* at = &sh.k[0][0][(k_to + buf * (2 * kPart)) ^ (i << 5)] + 512 * i;
-      *reinterpret_cast<uint2*>(at) = hi;
-      *reinterpret_cast<uint2*>(at + kPart) = lo;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float x = f(rv[0][j]), y = f(rv[1][j]), z = f(rv[2][j]), w = f(rv[3][j]);
-      uint2 hi, lo;
-      hi.x = first_part(x, y, v_up), hi.y = first_part(z, w, v_up);
-      lo.x = second_part(x, y, v_up, hi.x), lo.y = second_part(z, w, v_up, hi.y);
-      uint8_t* at = &sh.v[0][0][v_to + buf * (2 * kPart)] + 2048 * j;
-      *reinterpret_cast<uint2*>(at) = hi;
-      *reinterpret_cast<uint2*>(at + kPart) = lo;
-    }
+    for (int i = 0; i < 8; i++) stage_part(buf, i, power_of_two(k_e), power_of_two(v_e));
+    lds_barrier();
+    return ve == 128;
   };
 
   // This wave's rows (lanes behind the last repeat it), q in two parts: dims 16 s + 8 h ..
@@ -250,24 +293,40 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
 
   floatx16v o[kOT];
   float ref = -INFINITY, l = 0.f;
-  auto block = [&](int buf, int kb, float c_t, uint32_t keys) {
-    floatx16v s = {};
+  floatx16v scores[kBlocks];
+  // The scores of the tile in LDS and, among their products, the next tile's way there.
+  auto products = [&](int buf) {
+    const int to = buf ^ 1;
+    const float k_up = power_of_two(k_e), v_up = power_of_two(v_e);
 #pragma unroll
-    for (int i = 0; i < kSteps; i++) {
-      const uint8_t* at = &sh.k[0][0][(k_from + buf * (2 * kPart)) ^ (i << 5)] + kb * (64 * D);
+    for (int i = 0; i < 8; i++) {
+      const int kb = i / kSteps, st = i % kSteps;
+      floatx16v& s = scores[kb];
+      if (st == 0) s = floatx16v{};
+      const uint8_t* at = &sh.k[0][0][(k_from + buf * (2 * kPart)) ^ (st << 5)] + kb * (64 * D);
       const halfx8 kh = *reinterpret_cast<const halfx8*>(at);
       const halfx8 kl = *reinterpret_cast<const halfx8*>(at + kPart);
-      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[i].h, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[i].h, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[i].h, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[st].h, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[st].h, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[st].h, s, 0, 0, 0);
+      stage_part(to, i, k_up, v_up);
     }
+    note_fit(to);
     // (K's operands two steps ahead of the products.)
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-    for (int i = 0; i < kSteps; i++) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+    for (int i = 0; i < 8; i++) {
+#pragma unroll
+      for (int j = 0; j < 3; j++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
+  };
+  auto block = [&](int buf, int kb, float c_t, uint32_t keys) {
+    floatx16v& s = scores[kb];
     if (keys < kTile) {
 #pragma unroll
       for (int i = 0; i < 16; i++)
@@ -301,9 +360,6 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     }
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
-      // (Half of V's operands may be read ahead, during the weights; all of them are too many
-      // registers.)
-      if (ks > 0) asm volatile("" ::: "memory");
 #pragma unroll
       for (int x = 0; x < kOT; x++) {
         const uint8_t* at =
@@ -314,6 +370,13 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
         o[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[ks].h, o[x], 0, 0, 0);
         o[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[ks].h, o[x], 0, 0, 0);
       }
+    }
+    // (V's operands likewise; the first during the weights.)
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * kOT; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
   };
   // The rows' results so far: accumulator i of block x is row 8 (i / 4) + 4 h + i % 4 of V's
@@ -343,56 +406,71 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     }
   };
 
+  // Two waves share a SIMD, and where both could issue the older one does: its run was done in
+  // 388 us of 529, the other's in 470 (128 sequences, 128k keys). So the wave in the second place
+  // goes first in every other tile: 548 -> 537 us, and 126 -> 120 of 64-wide heads.
+  const bool second = __builtin_amdgcn_s_getreg(4 | 0 << 6 | 3 << 11) & 1;  // HW_ID's wave id
   const uint32_t n = end - tile;
-  next.last = 0;
   open();
-  fetch();
-  note_top(0);
+  next.last = 0;
+  advance();
+  next.first = 1;
+  fetch(next);
   SharedTile staged = next;
-  lds_barrier();
-  stage(0, true);
-  float k_now = k_down, v_now = v_up;  // of the tile in LDS
-  int e_now = v_e, unit;               // unit: accumulators hold O^T 2^unit
+  bool infinite = anchor(0, true);
   if (n > 1) {
-    next.first = 0;
-    fetch();
-    note_top(1);
+    advance();
+    fetch(next);
   }
-  lds_barrier();
   for (uint32_t t = 0; t < n;) {  // chains
     const uint32_t n_rows = staged.n_rows, part = staged.part;
     const bool busy = wave * 32u < n_rows;
     if (busy) load_q(staged.row0, n_rows);
-    ref = -INFINITY, l = 0.f, unit = e_now;
+    ref = -INFINITY, l = 0.f;
 #pragma unroll
     for (int x = 0; x < kOT; x++) o[x] = floatx16v{};
+    v_low = v_e;
+    int unit = v_e;  // accumulators hold O^T 2^unit
     uint32_t last;
     do {  // their tiles
       const int buf = t & 1;
-      const uint32_t keys = staged.keys;
-      const float k_t = k_now, v_t = v_now;
-      const int e_t = e_now;
-      last = staged.last;
-      if (t + 1 < n) {
-        stage(buf ^ 1, next.first);
-        staged = next;
-        k_now = k_down, v_now = v_up, e_now = v_e;
-        if (t + 2 < n) {
-          next.first = 0;
-          fetch();
-        }
+      if (second && (t & 1))
+        __builtin_amdgcn_s_setprio(1);
+      else
+        __builtin_amdgcn_s_setprio(0);
+      const SharedTile now = staged;
+      last = now.last;
+      if (t + 1 < n) staged = next;
+      if (t > 0 && shared_misfit(sh.fit[buf])) {
+        fetch(now);
+        infinite = anchor(buf, now.first);
+        if (t + 1 < n) fetch(staged);
       }
+      // (Behind the run's last tile what is staged is not read.)
       if (busy) {
-        if (e_t != unit || !(v_t > 0.f)) {  // uniform
-          const float alpha = v_t > 0.f ? ldexpf(1.f, e_t - unit) : v_t;
+        products(buf);
+      } else {
 #pragma unroll
-          for (int x = 0; x < kOT; x++) o[x] *= alpha;
-          unit = e_t;
-        }
-#pragma unroll
-        for (int kb = 0; kb < kBlocks; kb++) block(buf, kb, c_s * k_t, keys);
+        for (int i = 0; i < 8; i++) stage_part(buf ^ 1, i, power_of_two(k_e), power_of_two(v_e));
+        note_fit(buf ^ 1);
       }
-      if (t + 2 < n) note_top(buf);
+      if (t + 2 < n) {
+        advance();
+        fetch(next);
+      }
+      if (v_e != unit || infinite) {  // (a chain's first tile meets zeros)
+        const float alpha =
+            infinite ? __builtin_nanf("") : now.first ? 0.f : ldexpf(1.f, v_e - unit);
+#pragma unroll
+        for (int x = 0; x < kOT; x++) o[x] *= alpha;
+        unit = v_e;
+        infinite = false;
+      }
+      const float c_t = c_s * power_of_two(-k_e);
+      if (busy) {
+#pragma unroll
+        for (int kb = 0; kb < kBlocks; kb++) block(buf, kb, c_t, now.keys);
+      }
       lds_barrier();
       t++;
     } while (!last);
@@ -458,7 +536,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a, SharedP
       make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
 }
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 256;
 __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedArgs a, SharedPlan p) {
   shared_plan<kPlanThreads>(a, p);
 }
@@ -470,22 +548,23 @@ constexpr uint32_t kSharedSlots = 512;  // workgroups: two a CU
 
 static SharedPlan plan_of(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix,
                           uint32_t max_n_keys, uint32_t n_heads, uint32_t n_kv_heads,
-                          uint32_t head_dim, uint64_t* tiles_out = nullptr) {
+                          uint32_t head_dim, uint64_t* work_out = nullptr) {
   SharedPlan p{};
   p.tile = 4096 / head_dim;
   const uint64_t tile_seqs = kSharedRows / (n_heads / n_kv_heads);
   const uint64_t row_tiles = std::min(n_groups, n_seqs) + n_seqs / tile_seqs;
   auto tiles_of = [&](uint64_t keys) { return (keys + p.tile - 1) / p.tile; };
   const uint64_t tiles = row_tiles * tiles_of(max_prefix) + n_seqs * tiles_of(max_n_keys);
-  p.max_runs = (uint32_t)std::min((uint64_t)std::max(1u, kSharedSlots / n_kv_heads),
-                                  (tiles + kSharedLeast - 1) / kSharedLeast);
   p.chains = (uint32_t)(row_tiles + n_seqs);
-  if (tiles_out) *tiles_out = tiles;
+  const uint64_t work = tiles + p.chains;
+  p.max_runs = (uint32_t)std::min((uint64_t)std::max(1u, kSharedSlots / n_kv_heads),
+                                  std::max((uint64_t)1, work / kSharedLeast));
+  if (work_out) *work_out = work;
   return p;
 }
 
 static uint64_t list_bytes(const SharedPlan& p, uint32_t n_seqs) {
-  return 256 + ws_align(p.max_runs * sizeof(SharedRun)) +
+  return 256 + ws_align((p.max_runs + 1ull) * sizeof(SharedRun)) +
          ws_align((uint64_t)p.chains * sizeof(SharedChain)) +
          ws_align((uint64_t)n_seqs * sizeof(SharedRecord));
 }
@@ -505,10 +584,10 @@ uint64_t shared_ws_bytes(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix
 
 bool shared_fits(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix, uint32_t max_n_keys,
                  uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
-  uint64_t tiles;
+  uint64_t work;
   const SharedPlan p = plan_of(n_groups, n_seqs, max_prefix, max_n_keys, n_heads, n_kv_heads,
-                               head_dim, &tiles);
-  return tiles <= 0xfffffffeull && (uint64_t)p.max_runs * n_kv_heads <= kMaxGroups &&
+                               head_dim, &work);
+  return work <= 0xfffffffeull && (uint64_t)p.max_runs * n_kv_heads <= kMaxGroups &&
          shared_parts(n_seqs * (n_heads / n_kv_heads), p.max_runs) <= 0xffffffffull &&
          (uint64_t)n_seqs * n_heads <= kMaxGroups;
 }
@@ -521,7 +600,8 @@ static hipError_t launch(const SharedArgs& a, const DecodeFused* fused, uint32_t
   uint8_t* w = static_cast<uint8_t*>(ws);
   p.n_runs = reinterpret_cast<uint32_t*>(w);
   p.run = reinterpret_cast<SharedRun*>(w + 256);
-  p.chain = reinterpret_cast<SharedChain*>(w + 256 + ws_align(p.max_runs * sizeof(SharedRun)));
+  p.chain = reinterpret_cast<SharedChain*>(w + 256 +
+                                           ws_align((p.max_runs + 1ull) * sizeof(SharedRun)));
   p.record = reinterpret_cast<SharedRecord*>(
       reinterpret_cast<uint8_t*>(p.chain) + ws_align((uint64_t)p.chains * sizeof(SharedChain)));
   w += list_bytes(p, a.n_seqs);

@@ -19,8 +19,10 @@ struct SharedArgs {
 // heads of a kv head, of every sequence of a group (a row is sequence * m + head of the kv
 // head), in row tiles of up to 128 rows of whole sequences, and the m of one sequence for its
 // own keys. A chain is a row tile and its keys, in tiles. The tiles of all chains, one after the
-// other, are cut into runs of the same length: a run is one workgroup's work for one kv
-// head, whatever the lengths of the chains in it.
+// other, are cut into runs of the same work: a run is one workgroup's for one kv head, whatever
+// the lengths of the chains in it. Work is counted in tiles, and each chain is one more: to
+// read q and to write the results takes about as long (64 sequences of one own key each, a tile
+// a chain: 151 us for such a run, and 112 for as many tiles of a prefix).
 constexpr uint32_t kSharedRows = 128;
 struct alignas(16) SharedChain {
   uint64_t key_row;               // of the caches
@@ -30,8 +32,8 @@ struct alignas(16) SharedChain {
   uint32_t kind;                  // kSharedOwn: a sequence's own keys; kSharedOnce: read once
 };
 constexpr uint32_t kSharedOwn = 1, kSharedOnce = 2;
-struct alignas(16) SharedRun {
-  uint32_t chain, tile0, tile1, pad;
+struct alignas(8) SharedRun {
+  uint32_t chain, tile0;  // it ends where the next begins
 };
 // A sequence's partial results: prefix_n of its prefix (the first by run prefix_run, for a row
 // tile whose first row is row0) and own_n of its own keys.
@@ -45,7 +47,7 @@ struct SharedPlan {
   uint32_t max_runs;  // of a kv head
   uint32_t chains;    // at most
   uint32_t* n_runs;   // of a kv head
-  SharedRun* run;
+  SharedRun* run;     // and one more, behind the last
   SharedChain* chain;
   SharedRecord* record;
   float2* ml;         // (reference, sum) of a partial result's row
@@ -59,15 +61,15 @@ __host__ __device__ __forceinline__ uint64_t shared_parts(uint32_t rows, uint32_
   return 2ull * rows + (uint64_t)runs * kSharedRows;
 }
 
-constexpr uint32_t kSharedLeast = 2;  // tiles of a run at least
+constexpr uint32_t kSharedLeast = 2;  // work of a run: a tile at least
 
-// The run that holds tile x of `tiles`, cut into `runs`: run r has the tiles from tiles * r / runs on.
-__device__ __forceinline__ uint32_t shared_run_of(uint32_t x, uint32_t tiles, uint32_t runs) {
+// The run that holds x of the work, cut into `runs`: run r begins at work * r / runs.
+__device__ __forceinline__ uint32_t shared_run_of(uint32_t x, uint32_t work, uint32_t runs) {
   const uint64_t n = ((uint64_t)x + 1) * runs - 1;
-  return n >> 32 ? (uint32_t)(n / tiles) : (uint32_t)n / tiles;
+  return n >> 32 ? (uint32_t)(n / work) : (uint32_t)n / work;
 }
-__device__ __forceinline__ uint32_t shared_run_start(uint32_t r, uint32_t tiles, uint32_t runs) {
-  const uint64_t n = (uint64_t)tiles * r;
+__device__ __forceinline__ uint32_t shared_run_start(uint32_t r, uint32_t work, uint32_t runs) {
+  const uint64_t n = (uint64_t)work * r;
   return n >> 32 ? (uint32_t)(n / runs) : (uint32_t)n / runs;
 }
 
@@ -168,23 +170,28 @@ __device__ __forceinline__ void shared_plan(const SharedArgs& a, const SharedPla
     return;
   }
   const uint32_t tiles = groups.tiles + owns.tiles;
-  const uint32_t runs = min(p.max_runs, (tiles + kSharedLeast - 1) / kSharedLeast);
-  if (t == 0) *p.n_runs = runs;
+  const uint32_t work = tiles + groups.chains + owns.chains;
+  const uint32_t runs = min(p.max_runs, work / kSharedLeast);
+  if (t == 0) *p.n_runs = runs, p.run[runs] = SharedRun{0, tiles};
+  // Tile x (among all) of a chain that c others precede lies at x + c + 1 of the work.
+  auto run_of = [&](uint32_t x, uint32_t c) {
+    return shared_run_of(x + c + 1, work, runs);
+  };
 
-  // The last entry of a rising list of n that is not above x.
-  auto find = [&](const uint32_t* list, uint32_t n, uint32_t x) {
+  // The last of n entries that does not begin above x.
+  auto find = [&](uint32_t n, uint32_t x, auto begin) {
     uint32_t lo = 0, hi = n;
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
-      if (list[mid] <= x) lo = mid; else hi = mid;
+      if (begin(mid) <= x) lo = mid; else hi = mid;
     }
     return lo;
   };
-  auto put_runs = [&](uint32_t from, uint32_t to, auto chain_at) {  // those that start there
+  // Runs that begin in a range of the work: the chain there, and how many tiles of it are before.
+  auto put_runs = [&](uint32_t from, uint32_t to, auto chain_at) {
     for (uint32_t r = t; r < runs; r += kThreads) {
-      const uint32_t x = shared_run_start(r, tiles, runs);
-      if (x >= from && x < to)
-        p.run[r] = SharedRun{chain_at(x), x, shared_run_start(r + 1, tiles, runs), 0};
+      const uint32_t x = shared_run_start(r, work, runs);
+      if (x >= from && x < to) p.run[r] = chain_at(x);
     }
   };
   uint32_t chain0 = 0, tile0 = 0;
@@ -200,31 +207,37 @@ __device__ __forceinline__ void shared_plan(const SharedArgs& a, const SharedPla
     __syncthreads();
     for (uint32_t i = t; i < here.chains; i += kThreads) {
       // (Of entries without chains, which share the next one's first, find passes all.)
-      const uint32_t e = find(s_chain, n_here, i), rt = i - s_chain[e], nt = tiles_of(s_keys[e]);
+      const uint32_t e = find(n_here, i, [&](uint32_t j) { return s_chain[j]; });
+      const uint32_t rt = i - s_chain[e], nt = tiles_of(s_keys[e]);
       const uint32_t seq0 = s_off[e] + rt * tile_seqs, start = s_start[e] + rt * nt;
       SharedChain c;
       c.key_row = a.prefix_row[g0 + e];
       c.n_keys = s_keys[e], c.row0 = seq0 * m;
       c.n_rows = min(tile_seqs, s_off[e + 1] - seq0) * m;
-      c.start = start, c.first_run = shared_run_of(start, tiles, runs);
+      c.start = start, c.first_run = run_of(start, chain0 + i);
       c.kind = s_off[e + 1] - s_off[e] <= tile_seqs ? kSharedOnce : 0;
       p.chain[chain0 + i] = c;
     }
     for (uint32_t b = s_off[0] + t; b < s_off[n_here]; b += kThreads) {
-      const uint32_t e = find(s_off, n_here, b), keys = s_keys[e];
+      const uint32_t e = find(n_here, b, [&](uint32_t j) { return s_off[j]; });
+      const uint32_t keys = s_keys[e];
       const uint32_t nt = keys == kSharedRefused ? 0 : tiles_of(keys);
       const uint32_t rt = (b - s_off[e]) / tile_seqs, start = s_start[e] + rt * nt;
       SharedRecord& r = p.record[b];
       r.row0 = (s_off[e] + rt * tile_seqs) * m;
       r.prefix_n = keys == kSharedRefused ? keys : 0;
       if (nt > 0) {
-        r.prefix_run = shared_run_of(start, tiles, runs);
-        r.prefix_n = shared_run_of(start + nt - 1, tiles, runs) - r.prefix_run + 1;
+        const uint32_t before = chain0 + s_chain[e] + rt;
+        r.prefix_run = run_of(start, before);
+        r.prefix_n = run_of(start + nt - 1, before) - r.prefix_run + 1;
       }
     }
-    put_runs(tile0, tile0 + here.tiles, [&](uint32_t x) {
-      const uint32_t e = find(s_start, n_here, x);
-      return chain0 + s_chain[e] + (x - s_start[e]) / tiles_of(s_keys[e]);
+    const uint32_t from = tile0 + chain0;
+    put_runs(from, from + here.tiles + here.chains, [&](uint32_t x) {
+      auto begin = [&](uint32_t j) { return s_start[j] + chain0 + s_chain[j]; };
+      const uint32_t e = find(n_here, x, begin), nt = tiles_of(s_keys[e]);
+      const uint32_t y = x - begin(e), rt = y / (nt + 1), i = y % (nt + 1);
+      return SharedRun{chain0 + s_chain[e] + rt, s_start[e] + rt * nt + (i > 0 ? i - 1 : 0)};
     });
     chain0 += here.chains, tile0 += here.tiles;
     __syncthreads();
@@ -243,16 +256,19 @@ __device__ __forceinline__ void shared_plan(const SharedArgs& a, const SharedPla
       if (b < off_0 || b >= off_n) r.prefix_n = 0;
       r.own_n = n == kSharedRefused ? n : n == 0 && a.step ? kSharedIdle : 0;
       if (nt > 0) {
-        const uint32_t first = shared_run_of(start, tiles, runs);
+        const uint32_t before = chain0 + before_g.chains, first = run_of(start, before);
         r.own_run = first;
-        r.own_n = shared_run_of(start + nt - 1, tiles, runs) - first + 1;
+        r.own_n = run_of(start + nt - 1, before) - first + 1;
         p.chain[chain0 + before_g.chains] =
             SharedChain{a.seq_row_off[b], n, b * m, m, start, first, kSharedOwn | kSharedOnce};
       }
     }
     __syncthreads();
-    put_runs(tile0, tile0 + here.tiles, [&](uint32_t x) {
-      return chain0 + s_chain[find(s_start, n_here, x)];
+    const uint32_t from = tile0 + chain0;
+    put_runs(from, from + here.tiles + here.chains, [&](uint32_t x) {
+      auto begin = [&](uint32_t j) { return s_start[j] + chain0 + s_chain[j]; };
+      const uint32_t e = find(n_here, x, begin), i = x - begin(e);
+      return SharedRun{chain0 + s_chain[e], s_start[e] + (i > 0 ? i - 1 : 0)};
     });
     chain0 += here.chains, tile0 += here.tiles;
     __syncthreads();

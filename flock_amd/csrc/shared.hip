@@ -541,10 +541,13 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedArgs a,
   shared_plan<kPlanThreads>(a, p);
 }
 
-#ifndef MERGE_ROWS
-#define MERGE_ROWS 4096
-#endif
-constexpr uint32_t kSharedSlots = 512;  // workgroups: two a CU
+// Workgroups: two a CU, all at once. Calls with 256 / 512 / 1024, us: 64 x 8k step 77 / 59 / 75,
+// 16 x 32k 91 / 73 / 80, 128 x 128k 654 / 547 / 564.
+constexpr uint32_t kSharedSlots = 512;
+// Rows from which a row's pieces are joined by one group of threads: with more rows each has fewer
+// pieces, and the GPU is full without dividing them. Whole calls, us, divided / not: 256 rows
+// 73 / 78, 1024 59.1 / 60.0, 2048 556 / 555, 6400 129 / 121, 8192 84 / 76.
+constexpr uint32_t kMergeRows = 4096;
 
 static SharedPlan plan_of(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix,
                           uint32_t max_n_keys, uint32_t n_heads, uint32_t n_kv_heads,
@@ -626,8 +629,7 @@ static hipError_t launch(const SharedArgs& a, const DecodeFused* fused, uint32_t
     const uint32_t per = 1024 / (D * groups);
     hipLaunchKernelGGL(kernel, dim3((rows + per - 1) / per), dim3(256), 0, st, a, p);
   };
-  // (With more rows each has fewer pieces, and the GPU is full without dividing them.)
-  if (rows <= MERGE_ROWS)
+  if (rows <= kMergeRows)
     merge(shared_merge_kernel<D, 1024 / D>, 1024 / D);
   else
     merge(shared_merge_kernel<D, 1>, 1);

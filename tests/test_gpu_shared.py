@@ -195,7 +195,7 @@ def test_scales(case, rng):
 
 def test_values_of_growing_size(rng):
     """Later keys' values far above earlier ones', and the other way round. Keys and values
-    are off by 2^-22 of themselves or 2^-39 of the largest near them, so that a row's error is
+    are off by 2^-22 of themselves or 2^-25 of the largest near them, so that a row's error is
     within the usual bound of its largest value."""
     for order in (1, -1):
         batch = Batch(rng, [1500], [[90, 0]], q_scale=1.5)
@@ -206,6 +206,38 @@ def test_values_of_growing_size(rng):
         scale = (2.0 ** np.linspace(-20, 4, 1500)).astype(np.float32)[::order]
         batch.k[batch.prefix_row[0]:][:1500] *= scale[:, None, None]
         batch.check()
+
+
+@pytest.mark.parametrize("H,G,d", [(64, 64, 64), (128, 64, 128)])
+def test_sizes_that_jump_from_chain_to_chain(H, G, d, rng):
+    """Few runs of many chains (a kv head has eight), whose keys and values have sizes of their
+    own: 0, and 2^-90 to 2^90 apart from one to the next, and from tile to tile in one."""
+    k_scale = [0, 40, -20, 90, -90, 0, 3, -60]
+    v_scale = [0, -40, 60, -100, 90, 0, -3, 30]
+    batch = Batch(rng, [70, 33, 300, 64, 5, 129, 1, 200],
+                  [[3, 70], [1], [40, 0, 5], [33], [], [64, 2], [90], [7, 7, 7]], H, G, d)
+    for g in range(8):
+        seqs = range(batch.off[g], batch.off[g + 1])
+        spans = [(batch.prefix_row[g], batch.prefix[g])]
+        spans += [(batch.own_row[b], batch.n_keys[b]) for b in seqs]
+        for at, n in spans:
+            batch.k[at:at + n] *= np.float32(2.0 ** k_scale[g])
+            batch.v[at:at + n] *= np.float32(2.0 ** v_scale[g])
+        for b in seqs:
+            batch.q[b] *= np.float32(2.0 ** -k_scale[g])
+    at = batch.prefix_row[2]
+    batch.k[at + 64:at + 128] = 0
+    batch.v[at + 64:at + 128] = 0
+    batch.v[at + 192:at + 256] *= np.float32(2.0 ** -100)
+    batch.k[at + 128:at + 160] *= np.float32(2.0 ** -30)
+    batch.check()
+    # An infinite value reaches its sequence, none behind it.
+    batch.v[batch.own_row[1] + 5, :, 0] = math.inf
+    got = batch.run()
+    assert not np.isfinite(got[1]).all(-1).any()
+    rest = np.arange(batch.S) != 1
+    o, tol = batch.want(np.flatnonzero(rest))
+    assert (np.abs(got - o) <= tol)[rest].all()
 
 
 def test_one_key_takes_all(rng):

@@ -100,6 +100,7 @@ SIGNATURES: dict[str, tuple] = {
         [_p, _p, _p, _p, _p, _p, _f32, _i32, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _p, _u64]),
     "flk_embed": (_i32, [_p, _p, _p, _u32, _u32, _u32, _p]),
     "flk_advance": (_i32, [_p, _u32, _p, _p, _u32]),
+    "flk_advance_seqs": (_i32, [_p, _p, _p, _p, _p, _u32, _p, _p, _p, _p, _u32, _u32]),
     "flk_stream_create": (_i32, [ctypes.POINTER(_p)]),
     "flk_stream_destroy": (_i32, [_p]),
     "flk_capture_begin": (_i32, []),

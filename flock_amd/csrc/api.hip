@@ -889,6 +889,11 @@ static int32_t check_words(const void* p, const char* name) {
     FLK_NONNULL(p);                           \
     if (int32_t rc_ = check_words((p), #p)) return rc_; \
   } while (0)
+// One that may be null.
+#define FLK_MAYBE_WORDS(p)                    \
+  do {                                        \
+    if (int32_t rc_ = check_words((p), #p)) return rc_; \
+  } while (0)
 
 static int32_t check_pages(uint32_t n_pages, uint32_t page) {
   if (page != 32 && page != 64 && page != 128 && page != 256)
@@ -1252,9 +1257,6 @@ static int32_t token_args(const float* logits, uint64_t ld, uint32_t n_rows, uin
   return FLK_OK;
 }
 
-// An optional device array of 32-bit words.
-#define FLK_MAYBE_WORDS(p)                                do {                                                      if (int32_t rc_ = check_words((p), #p)) return rc_;   } while (0)
-
 int32_t flk_token_logprobs(const float* logits, uint64_t ld, const uint32_t* tokens,
                            float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs,
                            uint32_t n_rows, uint32_t n_vocab, uint32_t n_top, void* ws,
@@ -1298,4 +1300,30 @@ int32_t flk_sample(const float* logits, uint64_t ld, const float* temperature,
   a.uniform = uniform;
   a.token = token, a.logprob = logprob;
   return hip_status(launch_tokens(a, ws, g_stream), "flk_sample");
+}
+
+int32_t flk_advance_seqs(uint32_t* n_keys, uint32_t* cursor, const uint32_t* token,
+                         const float* logprob, const uint32_t* stops, uint32_t n_stops,
+                         uint32_t* token_log, float* logprob_log, const float* uniform_log,
+                         float* uniform, uint32_t n_seqs, uint32_t log_len) {
+  FLK_WORDS(n_keys);
+  FLK_WORDS(cursor);
+  FLK_WORDS(token);
+  FLK_WORDS(token_log);
+  FLK_MAYBE_WORDS(logprob);
+  FLK_MAYBE_WORDS(logprob_log);
+  FLK_MAYBE_WORDS(stops);
+  FLK_MAYBE_WORDS(uniform_log);
+  FLK_MAYBE_WORDS(uniform);
+  if ((logprob == nullptr) != (logprob_log == nullptr))
+    return fail(FLK_ERR_ARG, "advance_seqs: logprob and logprob_log go together");
+  if ((uniform == nullptr) != (uniform_log == nullptr))
+    return fail(FLK_ERR_ARG, "advance_seqs: uniform and uniform_log go together");
+  if ((n_stops != 0) != (stops != nullptr))
+    return fail(FLK_ERR_ARG, "advance_seqs: %u stops, stops %s", n_stops,
+                stops ? "given" : "null");
+  if (n_seqs == 0) return fail(FLK_ERR_ARG, "n_seqs must be >= 1");
+  const AdvanceSeqs a{n_keys,      cursor,      token,   logprob, stops,  n_stops, token_log,
+                      logprob_log, uniform_log, uniform, n_seqs,  log_len};
+  return hip_status(launch_advance_seqs(a, g_stream), "flk_advance_seqs");
 }

@@ -402,6 +402,19 @@ hipError_t launch_elementwise(int op, const float* a, const float* b, float* o, 
 hipError_t launch_embed(const int8_t* qs, const uint16_t* scales, const uint32_t* ids,
                         uint32_t n_tokens, uint32_t vocab, uint32_t hidden, float* out,
                         hipStream_t st);
+struct AdvanceSeqs {
+  uint32_t *n_keys, *cursor;
+  const uint32_t* token;
+  const float* logprob;
+  const uint32_t* stops;
+  uint32_t n_stops;
+  uint32_t* token_log;
+  float* logprob_log;
+  const float* uniform_log;
+  float* uniform;
+  uint32_t n_seqs, log_len;
+};
+hipError_t launch_advance_seqs(const AdvanceSeqs& a, hipStream_t st);
 hipError_t launch_advance(uint32_t* state, uint32_t delta, const uint32_t* value, uint32_t* log,
                           uint32_t log_len, hipStream_t st);
 

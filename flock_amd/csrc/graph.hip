@@ -62,4 +62,29 @@ hipError_t launch_advance(uint32_t* state, uint32_t delta, const uint32_t* value
   return hipGetLastError();
 }
 
+// One workgroup: its time is the launch's, and the cursor moves when all have read it.
+__global__ __launch_bounds__(256) void advance_seqs_kernel(AdvanceSeqs a) {
+  const uint32_t c = *a.cursor;
+  __syncthreads();
+  if (threadIdx.x == 0) *a.cursor = c + 1;
+  for (uint32_t b = threadIdx.x; b < a.n_seqs; b += 256) {
+    const uint32_t t = a.token[b], n = a.n_keys[b];
+    bool stop = t == 0xffffffffu;
+    for (uint32_t i = 0; i < a.n_stops; i++) stop |= t == a.stops[i];
+    a.n_keys[b] = n == 0 || stop ? 0 : n + 1;
+    if (c < a.log_len) {
+      const size_t at = (size_t)c * a.n_seqs + b;
+      a.token_log[at] = t;
+      if (a.logprob_log != nullptr) a.logprob_log[at] = a.logprob[b];
+    }
+    if (a.uniform != nullptr && c < a.log_len && c + 1 < a.log_len)
+      a.uniform[b] = a.uniform_log[(size_t)(c + 1) * a.n_seqs + b];
+  }
+}
+
+hipError_t launch_advance_seqs(const AdvanceSeqs& a, hipStream_t st) {
+  hipLaunchKernelGGL(advance_seqs_kernel, dim3(1), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
 }  // namespace flk

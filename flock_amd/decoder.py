@@ -229,6 +229,28 @@ class DecoderLayer:
         """Where encode_dev writes (fixed, so a captured step can chain layers)."""
         return self.out_dev
 
+    def encode_shared(self, src, batch, out) -> None:
+        """One decode step of ``batch.n_seqs`` sequences that share a prefix (ops.decode_layer_shared),
+        rows of ``src`` to rows of ``out``. Their lengths and places in this layer's caches
+        are the batch's device arrays, so a captured step replays as they change; no host
+        bookkeeping."""
+        cfg, b, g = self.cfg, self.buf, self.g
+        H, Hkv, d, n = cfg.nHeads, cfg.nKvHeads, cfg.headDim, batch.n_seqs
+        if n > cfg.maxPrefill:
+            raise ValueError(f"{n} sequences exceed maxPrefill {cfg.maxPrefill}")
+        qkv, row = b["qkv"].ptr, (H + 2 * Hkv) * d
+        ops.q8_matvec_ex(self.w_qkv, src, b["qkv"], n, norm_gain=g["attn_norm.weight"],
+                         eps=cfg.eps)
+        ops.decode_layer_shared(qkv, qkv + H * d * 4, qkv + (H + Hkv) * d * 4,
+                                g["attn_q_norm.weight"], g["attn_k_norm.weight"], b["invFreq"],
+                                cfg.eps, cfg.ropePairing, b["qn"], b["kcache"], b["vcache"],
+                                batch.prefix_row, batch.n_prefix, batch.seq_off,
+                                batch.seq_row_off, batch.n_keys, b["attn"], batch.n_groups, n,
+                                batch.max_prefix, batch.max_n_keys, H, Hkv, d, batch.ws,
+                                in_stride=row)
+        ops.q8_matvec_ex(self.w_o, b["attn"], b["h2"], n, res=src)
+        self._ffn(n, out)
+
     # ----------------------------------------------------------------- prefill
     def encodePrefill(self, nTokens: int, hidden=None, offset: int | None = None,
                       src=None) -> None:

@@ -110,6 +110,7 @@ export const hip = Deno.dlopen(Deno.env.get("FLOCK_ATTN_LIB") ?? "libflock_attn.
   },
   flk_embed: { parameters: [P, P, P, U32, U32, U32, P], result: I32 },
   flk_advance: { parameters: [P, U32, P, P, U32], result: I32 },
+  flk_advance_seqs: { parameters: [P, P, P, P, P, U32, P, P, P, P, U32, U32], result: I32 },
   flk_stream_create: { parameters: ["buffer"], result: I32 },
   flk_stream_destroy: { parameters: [P], result: I32 },
   flk_capture_begin: { parameters: [], result: I32 },

@@ -1,4 +1,4 @@
-"""Greedy decoding of a whole Qwen3 model on libflock_attn (kernels/model.ts).
+"""Decoding of a whole Qwen3 model on libflock_attn (kernels/model.ts).
 
 ``Model`` follows model.ts's engine: token ids -> embedding gather (embed.wgsl,
 over the tied token_embd) -> the decoder layers -> output norm -> LM head ->
@@ -11,6 +11,10 @@ one-token step is captured once into a HIP graph and replayed: the position,
 the token the embedding reads (the previous step's argmax) and the log of
 generated ids all live in device memory, so a token costs one graph launch
 and no host round trip; the host reads the whole log at the end.
+
+Extensions (the reference decodes one sequence, greedily): ``answers`` draws several
+answers to one prompt together, the prompt's keys stored and read once for all of
+them, and ``score`` gives the log probabilities of given ids.
 """
 from __future__ import annotations
 
@@ -19,6 +23,61 @@ import numpy as np
 from ._lib import CacheFullError
 from . import ops
 from .decoder import DecoderConfig, DecoderLayer
+
+
+SCORE_ROWS = 128  # of logits at a time
+
+
+class _Answers:
+    """n answers of up to T ids: what a step of them reads and writes on the device, and
+    the captured step. Sequence b's own keys are the T rows behind the prompt's and those of
+    the b sequences before it, in every layer's cache."""
+
+    def __init__(self, model: "Model", n: int, T: int, n_stops: int):
+        cfg, V = model.cfg, model.vocab
+        B, f = ops.DeviceBuffer, 4
+        self.key, self.max_top_k = (n, T, n_stops), min(64, V)
+        self.n_groups, self.n_seqs, self.max_prefix, self.max_n_keys = 1, n, cfg.maxKeys, T
+        self.prefix_row = B.from_array(np.zeros(1, np.uint64))
+        self.n_prefix = B(4)
+        self.seq_off = B.from_array(np.array([0, n], np.uint32))
+        self.seq_row_off, self.n_keys = B(8 * n), B(4 * n)
+        self.ws = B(ops.decode_shared_ws_bytes(1, n, cfg.maxKeys, T, cfg.nHeads, cfg.nKvHeads,
+                                               cfg.headDim))
+        self.x, self.logits = B(n * cfg.hidden * f), B(n * V * f)
+        self.token, self.logprob, self.uniform = B(4 * n), B(4 * n), B(4 * n)
+        self.temperature, self.top_k = B(4 * n), B(4 * n)
+        self.top_p, self.min_p = B(4 * n), B(4 * n)
+        self.token_ws = B(max(256, ops.tokens_ws_bytes(n, V, self.max_top_k)))
+        self.stops = B(4 * n_stops) if n_stops else None
+        self.cursor = B(4)
+        self.token_log, self.logprob_log, self.uniform_log = (B(4 * T * n) for _ in range(3))
+        self.stream = ops.Stream()
+        ops.set_stream(self.stream)
+        try:
+            with ops.Graph() as g:
+                ops.embed(model.embd, self.token, n, self.x)
+                for layer in model.layers:
+                    layer.encode_shared(self.x, self, self.x)
+                ops.q8_matvec_ex(model.embd, self.x, self.logits, n, norm_gain=model.g_out,
+                                 eps=cfg.eps)
+                ops.sample(self.logits, self.uniform, self.token, n, V, self.max_top_k,
+                           self.token_ws, temperature=self.temperature, top_k=self.top_k,
+                           top_p=self.top_p, min_p=self.min_p, logprob=self.logprob)
+                ops.advance_seqs(self.n_keys, self.cursor, self.token, self.token_log, n, T,
+                                 logprob=self.logprob, logprob_log=self.logprob_log,
+                                 stops=self.stops, n_stops=n_stops,
+                                 uniform_log=self.uniform_log, uniform=self.uniform)
+        finally:
+            ops.set_stream(None)
+        self.graph = g
+
+    def free(self) -> None:
+        self.graph.free()
+        self.stream.free()
+        for x in vars(self).values():
+            if isinstance(x, ops.DeviceBuffer):
+                x.free()
 
 
 class Model:
@@ -42,6 +101,8 @@ class Model:
         self.nKeys = 0
         self.graph = None
         self._stream = None
+        self._answers = None
+        self._score = None
 
     # ------------------------------------------------------------- host steps
     def reset(self) -> None:
@@ -62,8 +123,15 @@ class Model:
         if self.nKeys + ids.size > self.cfg.maxKeys:
             raise CacheFullError(-2, f"KV cache would exceed {self.cfg.maxKeys} keys "
                                      f"({self.nKeys} + {ids.size})")
+        for n, src in self._feed(ids):
+            pass
+        self._head(ops.ptr(src) + (n - 1) * self.cfg.hidden * 4)
+        ops.sync()
+        return int(self.tok_idx.download(1, np.uint32)[0])
+
+    def _feed(self, ids):
+        """Feed ids in chunks of maxPrefill; yields each chunk's size and output rows."""
         P = max(1, self.cfg.maxPrefill)
-        hid = self.cfg.hidden
         for off in range(0, ids.size, P):
             chunk = ids[off:off + P]
             n = chunk.size
@@ -77,9 +145,41 @@ class Model:
                     layer.encodePrefill(n, src=src)
                 src = layer.outputBuffer()
             self.nKeys += n
-        self._head(ops.ptr(src) + (n - 1) * hid * 4)
-        ops.sync()
-        return int(self.tok_idx.download(1, np.uint32)[0])
+            yield n, src
+
+    def score(self, ids) -> np.ndarray:
+        """Feed ``ids`` at positions nKeys.. as step does; the log probability of
+        each but the first, given all before it."""
+        ids = np.ascontiguousarray(ids, np.uint32).ravel()
+        if ids.size < 2:
+            raise ValueError("score needs two token ids or more")
+        if ids.max() >= self.vocab:
+            raise ValueError(f"id {ids.max()} of a vocabulary of {self.vocab}")
+        if self.nKeys + ids.size > self.cfg.maxKeys:
+            raise CacheFullError(-2, f"KV cache would exceed {self.cfg.maxKeys} keys "
+                                     f"({self.nKeys} + {ids.size})")
+        B, hid, V = ops.DeviceBuffer, self.cfg.hidden, self.vocab
+        if self._score is None:
+            P = max(1, self.cfg.maxPrefill)
+            R = min(P, SCORE_ROWS)
+            self._score = (B(R * V * 4), B(4 * P), B(4 * P),
+                           B(max(256, ops.tokens_ws_bytes(R, V, 0))))
+        logits, tokens, logprob, ws = self._score
+        out, off = [], 0
+        for n, src in self._feed(ids):
+            m = min(n, ids.size - 1 - off)  # rows with an id to score
+            if m == 0:
+                break
+            tokens.upload(ids[off + 1:off + 1 + m])
+            for r in range(0, m, SCORE_ROWS):
+                rows = min(SCORE_ROWS, m - r)
+                ops.q8_matvec_ex(self.embd, ops.ptr(src) + r * hid * 4, logits, rows,
+                                 norm_gain=self.g_out, eps=self.cfg.eps)
+                ops.token_logprobs(logits, tokens.ptr + 4 * r, logprob.ptr + 4 * r, rows, V, ws)
+            ops.sync()
+            out.append(logprob.download(m))
+            off += n
+        return np.concatenate(out)
 
     # --------------------------------------------------------- captured steps
     def _capture(self) -> None:
@@ -139,7 +239,84 @@ class Model:
         ops.set_stream(None)
         return out
 
+    def answers(self, prompt, n: int, maxTokens: int, eos=(), temperature: float = 1.0,
+                top_k: int = 64, top_p: float = 1.0, min_p: float = 0.0, seed=None) -> list:
+        """n answers to ``prompt`` (fed at positions nKeys..), drawn together: a list of
+        (ids, their log probabilities), each up to maxTokens long and ending before an id in
+        ``eos``. Tokens come from the top_k (up to 64) largest logits as ops.sample draws
+        them, temperature 0 takes the largest; log probabilities are the model's own, whatever
+        the settings. ``seed`` fixes the random numbers.
+
+        A step is one replay of a captured step of all answers: their queries meet the
+        prompt's keys together. The prompt's last id is each answer's first input, so
+        the cache holds the prompt but for that id afterwards, and no answer."""
+        prompt = np.ascontiguousarray(prompt, np.uint32).ravel()
+        if prompt.size == 0:
+            raise ValueError("answers need at least one token id")
+        if n < 1 or n > max(1, self.cfg.maxPrefill):
+            raise ValueError(f"{n} answers: 1 .. maxPrefill ({self.cfg.maxPrefill}) at a time")
+        if not 1 <= top_k <= 64:
+            raise ValueError(f"top_k must be 1 .. 64, got {top_k}")
+        if not 0 <= temperature < np.inf:
+            raise ValueError(f"temperature must be finite and >= 0, got {temperature}")
+        if not top_p > 0 or not 0 <= min_p <= 1:
+            raise ValueError(f"top_p must be > 0 and min_p 0 .. 1, got {top_p} and {min_p}")
+        if maxTokens < 1:
+            return [([], []) for _ in range(n)]
+        held = self.nKeys + prompt.size - 1
+        if held + n * maxTokens > self.cfg.maxKeys:
+            raise CacheFullError(-2, f"KV cache would exceed {self.cfg.maxKeys} keys "
+                                     f"({held} + {n} x {maxTokens})")
+        for _ in self._feed(prompt[:-1]):
+            pass
+        ops.sync()  # (the captured step is on a stream of its own)
+        eos = sorted(set(int(e) for e in eos))
+        key = (n, maxTokens, len(eos))
+        if self._answers is None or self._answers.key != key:
+            if self._answers is not None:
+                self._answers.free()
+                self._answers = None
+            self._answers = _Answers(self, *key)
+        a, u32, f32 = self._answers, np.uint32, np.float32
+        a.n_prefix.upload(np.array([held], u32))
+        a.seq_row_off.upload(held + maxTokens * np.arange(n, dtype=np.uint64))
+        a.n_keys.upload(np.ones(n, u32))
+        a.cursor.upload(np.zeros(1, u32))
+        a.token.upload(np.full(n, prompt[-1], u32))
+        for buf, x, t in ((a.temperature, temperature, f32), (a.top_k, min(top_k, a.max_top_k), u32),
+                          (a.top_p, top_p, f32), (a.min_p, min_p, f32)):
+            buf.upload(np.full(n, x, t))
+        if eos:
+            a.stops.upload(np.array(eos, u32))
+        uniform = np.random.default_rng(seed).random((maxTokens, n), f32)
+        a.uniform_log.upload(uniform)
+        a.uniform.upload(uniform[0])
+        done = 0
+        ops.set_stream(a.stream)
+        try:
+            while done < maxTokens:
+                for _ in range(min(32, maxTokens - done)):
+                    a.graph.launch()
+                    done += 1
+                ops.sync()
+                if not a.n_keys.download(n, u32).any():
+                    break
+        finally:
+            ops.set_stream(None)
+        ids = a.token_log.download(done * n, u32).reshape(done, n)
+        logprob = a.logprob_log.download(done * n).reshape(done, n)
+        out = []
+        for b in range(n):
+            stop = np.flatnonzero(np.isin(ids[:, b], eos + [0xffffffff]))
+            end = stop[0] if stop.size else done
+            out.append(([int(t) for t in ids[:end, b]], [float(x) for x in logprob[:end, b]]))
+        return out
+
     def free(self) -> None:
+        if self._answers is not None:
+            self._answers.free()
+        for x in self._score or ():
+            x.free()
         if self.graph is not None:
             self.graph.free()
         if self._stream is not None:

@@ -516,6 +516,16 @@ def advance(state, delta: int = 1, value=None, log=None, log_len: int = 0) -> No
     check(lib().flk_advance(ptr(state), delta, ptr(value), ptr(log), log_len), "flk_advance")
 
 
+def advance_seqs(n_keys, cursor, token, token_log, n_seqs: int, log_len: int, logprob=None,
+                 logprob_log=None, stops=None, n_stops: int = 0, uniform_log=None,
+                 uniform=None) -> None:
+    """The end of a captured step of n_seqs sequences (flk_advance_seqs): lengths go up (to 0
+    at a stop), the tokens into the log, the next step's uniform numbers out of theirs."""
+    check(lib().flk_advance_seqs(ptr(n_keys), ptr(cursor), ptr(token), ptr(logprob), ptr(stops),
+                                 n_stops, ptr(token_log), ptr(logprob_log), ptr(uniform_log),
+                                 ptr(uniform), n_seqs, log_len), "flk_advance_seqs")
+
+
 class Stream:
     """A library-created stream of default priority (capturable)."""
 

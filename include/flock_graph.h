@@ -49,6 +49,21 @@ int32_t flk_embed(const int8_t* qs, const uint16_t* scales, const uint32_t* ids,
 int32_t flk_advance(uint32_t* state, uint32_t delta, const uint32_t* value, uint32_t* log,
                     uint32_t log_len);
 
+/* The same at the end of a captured step of n_seqs sequences (flk_decode_layer_ragged,
+ * flk_decode_layer_shared) that draws its tokens (flk_sample). All DEVICE arrays; a log
+ * has log_len steps of n_seqs entries, and c = *cursor is the step:
+ *   n_keys        n_keys[b] += 1; to 0 (idle) where token[b] is among the n_stops ids `stops`,
+ *                 or 0xffffffff; idle ones stay so
+ *   token_log     step c's entries become token and logprob, if c < log_len. logprob and
+ *   logprob_log   logprob_log may both be NULL
+ *   uniform       becomes step c + 1's entries of uniform_log, if c + 1 < log_len. Both may be
+ *                 NULL
+ *   cursor        *cursor += 1 */
+int32_t flk_advance_seqs(uint32_t* n_keys, uint32_t* cursor, const uint32_t* token,
+                         const float* logprob, const uint32_t* stops, uint32_t n_stops,
+                         uint32_t* token_log, float* logprob_log, const float* uniform_log,
+                         float* uniform, uint32_t n_seqs, uint32_t log_len);
+
 /* A stream of default priority for capture and replay (the null stream
  * cannot be captured); destroy it when done. */
 int32_t flk_stream_create(void** stream);

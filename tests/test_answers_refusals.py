@@ -132,3 +132,17 @@ def test_samples():
         assert need <= ops.tokens_ws_bytes(rows, 151936, 20) <= ops.tokens_ws_bytes(
             rows + 1, 151936, 20)
     assert ops.tokens_ws_bytes(0, 100, 5) == 0 and ops.tokens_ws_bytes(1, 100, 65) == 0
+
+
+def advance(nk=P, cursor=P, token=P, log=P, n=3, T=4, lp=P, lp_log=P, stops=P, n_stops=2, u_log=P,
+            u=P):
+    ops.advance_seqs(nk, cursor, token, log, n, T, logprob=lp, logprob_log=lp_log, stops=stops,
+                     n_stops=n_stops, uniform_log=u_log, uniform=u)
+
+
+def test_advance_seqs():
+    for name in ("nk", "cursor", "token", "log", "lp", "lp_log", "stops", "u_log", "u"):
+        refused(ARG, advance, **{name: None})
+        refused(ARG, advance, **{name: P + 1})
+    refused(ARG, advance, n_stops=0)
+    refused(ARG, advance, n=0)

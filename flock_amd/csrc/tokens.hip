@@ -1,5 +1,7 @@
 // Log probabilities of given tokens with entropy and top alternatives, and sampling from
-// the alternatives. HBM-bound: a row of logits is read once.
+// the alternatives. HBM-bound: a row of logits is read once. 2048 rows of 151936: 212 us, 5.9
+// TB/s; 256 with 50 alternatives 32 us, 4.8 TB/s; with fewer rows two launches and the
+// latency of the alternatives' second look count (64 rows: 14 + 4.6 us, one row 7.5 + 5.4).
 //
 // For a row x with largest value m (held c times) and R = sum of exp(x - m) over the
 // others, log sum exp x = m + log(c + R); with c and R apart, log1p keeps the small
@@ -466,6 +468,10 @@ __global__ __launch_bounds__(kTokenThreads) void token_join_kernel(TokenArgs a, 
   finish(a, row, wave_join(s), list, lane);
 }
 
+// Rows are cut where a workgroup each would leave CUs idle, into parts of two chunks a wave at
+// least. Calls, us, cut into 256 / 512 / 1024 workgroups: 64 rows of 151936 18.8 / 17.6 / 24.7,
+// 100 of 50021 16.1 / 15.2 / 19.2; 256 rows of 151936, uncut / in four 32.4 / 40.7. One row, its
+// parts of one chunk a wave at least / two / four: 14.2 / 13.1 / 13.5.
 constexpr uint32_t kTokenGroups = 512, kTokenLeast = 2;
 static uint32_t token_splits(uint32_t n_rows, uint32_t n_vocab) {
   const uint32_t part = kChunk * kTokenWaves * kTokenLeast;

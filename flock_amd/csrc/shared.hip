@@ -123,7 +123,9 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
   __shared__ SharedLds<D> sh;
   const uint32_t G = a.n_kv_heads, m = a.n_heads / G;
   const uint32_t kvh = blockIdx.x % G, run = blockIdx.x / G;
-  if (run >= uniform(*p.n_runs)) return;
+  uint32_t e = uniform(p.run[run].chain), tile = uniform(p.run[run].tile0);
+  const uint32_t end = uniform(p.run[run + 1].tile0);
+  if (tile == end) return;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
@@ -131,8 +133,6 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
   const size_t part0 = kvh * shared_parts(rows, p.max_runs);
 
   // The chain that tiles are fetched from.
-  uint32_t e = uniform(p.run[run].chain), tile = uniform(p.run[run].tile0);
-  const uint32_t end = uniform(p.run[run + 1].tile0);
   uint64_t key_row;
   uint32_t n_keys, in_chain;
   SharedTile next;  // the last tile that was sent for
@@ -420,6 +420,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
   next.first = 1;
   fetch(next);
   SharedTile staged = next;
+  if (wave * 32u < staged.n_rows) load_q(staged.row0, staged.n_rows);
   bool infinite = anchor(0, true);
   if (n > 1) {
     advance();
@@ -428,7 +429,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
   for (uint32_t t = 0; t < n;) {  // chains
     const uint32_t n_rows = staged.n_rows, part = staged.part;
     const bool busy = wave * 32u < n_rows;
-    if (busy) load_q(staged.row0, n_rows);
+    if (busy && t > 0) load_q(staged.row0, n_rows);
     ref = -INFINITY, l = 0.f;
 #pragma unroll
     for (int x = 0; x < kOT; x++) o[x] = floatx16v{};
@@ -570,7 +571,7 @@ static SharedPlan plan_of(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefi
 }
 
 static uint64_t list_bytes(const SharedPlan& p, uint32_t n_seqs) {
-  return 256 + ws_align((p.max_runs + 1ull) * sizeof(SharedRun)) +
+  return ws_align((p.max_runs + 1ull) * sizeof(SharedRun)) +
          ws_align((uint64_t)p.chains * sizeof(SharedChain)) +
          ws_align((uint64_t)n_seqs * sizeof(SharedRecord));
 }
@@ -604,10 +605,8 @@ static hipError_t launch(const SharedArgs& a, const DecodeFused* fused, uint32_t
   SharedPlan p = plan_of(a.n_groups, a.n_seqs, a.max_prefix, a.max_n_keys, a.n_heads,
                          a.n_kv_heads, a.head_dim);
   uint8_t* w = static_cast<uint8_t*>(ws);
-  p.n_runs = reinterpret_cast<uint32_t*>(w);
-  p.run = reinterpret_cast<SharedRun*>(w + 256);
-  p.chain = reinterpret_cast<SharedChain*>(w + 256 +
-                                           ws_align((p.max_runs + 1ull) * sizeof(SharedRun)));
+  p.run = reinterpret_cast<SharedRun*>(w);
+  p.chain = reinterpret_cast<SharedChain*>(w + ws_align((p.max_runs + 1ull) * sizeof(SharedRun)));
   p.record = reinterpret_cast<SharedRecord*>(
       reinterpret_cast<uint8_t*>(p.chain) + ws_align((uint64_t)p.chains * sizeof(SharedChain)));
   w += list_bytes(p, a.n_seqs);

@@ -46,8 +46,7 @@ struct SharedPlan {
   uint32_t tile;      // keys of a tile
   uint32_t max_runs;  // of a kv head
   uint32_t chains;    // at most
-  uint32_t* n_runs;   // of a kv head
-  SharedRun* run;     // and one more, behind the last
+  SharedRun* run;     // max_runs and one more; those behind the last have no tiles
   SharedChain* chain;
   SharedRecord* record;
   float2* ml;         // (reference, sum) of a partial result's row
@@ -166,13 +165,13 @@ __device__ __forceinline__ void shared_plan(const SharedArgs& a, const SharedPla
   if (s_bad) {  // (seen by all: the sums' barriers)
     for (uint32_t b = t; b < a.n_seqs; b += kThreads)
       p.record[b] = SharedRecord{0, kSharedRefused, 0, 0, kSharedRefused, {0, 0, 0}};
-    if (t == 0) *p.n_runs = 0;
+    for (uint32_t r = t; r <= p.max_runs; r += kThreads) p.run[r] = SharedRun{0, 0};
     return;
   }
   const uint32_t tiles = groups.tiles + owns.tiles;
   const uint32_t work = tiles + groups.chains + owns.chains;
   const uint32_t runs = min(p.max_runs, work / kSharedLeast);
-  if (t == 0) *p.n_runs = runs, p.run[runs] = SharedRun{0, tiles};
+  for (uint32_t r = runs + t; r <= p.max_runs; r += kThreads) p.run[r] = SharedRun{0, tiles};
   // Tile x (among all) of a chain that c others precede lies at x + c + 1 of the work.
   auto run_of = [&](uint32_t x, uint32_t c) {
     return shared_run_of(x + c + 1, work, runs);

@@ -57,7 +57,7 @@ struct alignas(16) SharedLds {
 constexpr uint32_t kFits = 1, kLarge = 2, kSmall = 4;
 __device__ __forceinline__ uint32_t shared_fit(float top, float up) {  // top: of the lane, >= 0
   const float x = top * up;
-  const uint64_t large = __ballot(!(x < 65000.f)), fits = __ballot(x >= 1.f);
+  const uint64_t large = __ballot(!(x < 65000.f)), fits = __ballot(x >= 256.f);
   const uint64_t some = __ballot(top > 0.f);
   return large ? kLarge : fits ? kFits : some ? kSmall : 0;
 }
@@ -203,8 +203,8 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
   };
   auto f = [](uint32_t x) { return __builtin_bit_cast(float, x); };
   // The factors of the tile in LDS, 2^k_e and 2^v_e. They stay while a tile's largest values lie
-  // in 2^0 .. 2^16 with them, or are 0: then two parts in f16 are off by 2^-25 of the largest
-  // at most. So a tile need not be seen as a whole before it is split: each wave
+  // in 2^8 .. 2^16 with them, or are 0: then two parts in f16 are off by 2^-25 at most, 2^-33
+  // of the largest. So a tile need not be seen as a whole before it is split: each wave
   // notes how its part fits, and the tile is done again if need be.
   int k_e = 0, v_e = 0, v_low = 0;  // v_low: the least v_e of the chain
   // An eighth of the tile in registers into LDS.
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     sh.fit[buf][wave] =
         shared_fit(k, power_of_two(k_e)) | shared_fit(v, power_of_two(v_e)) << 16;
   };
-  // The factors from the tile in registers, 2^10 .. 2^11 its largest values with them, and
+  // The factors from the tile in registers, 2^11 .. 2^12 its largest values with them, and
   // the tile into LDS; by all waves. (V's is at most 2^60 of the chain's least, so that
   // accumulators stay finite.) Whether V holds an infinity: its rows are NaN, and the factor
   // is as before.
@@ -256,9 +256,9 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     const float4 vt = *reinterpret_cast<const float4*>(sh.top[1]);
     const int ke = exponent(uniform_f(fmaxf(fmaxf(kt.x, kt.y), fmaxf(kt.z, kt.w))));
     const int ve = exponent(uniform_f(fmaxf(fmaxf(vt.x, vt.y), fmaxf(vt.z, vt.w))));
-    if (ke != -127 && ke != 128) k_e = max(10 - max(ke, -100), -115);
+    if (ke != -127 && ke != 128) k_e = max(11 - max(ke, -100), -115);
     if (ve != -127 && ve != 128)
-      v_e = max(min(10 - max(ve, -100), first ? 110 : v_low + 60), -115);
+      v_e = max(min(11 - max(ve, -100), first ? 110 : v_low + 60), -115);
     v_low = first ? v_e : min(v_low, v_e);
 #pragma unroll
     for (int i = 0; i < 8; i++) stage_part(buf, i, power_of_two(k_e), power_of_two(v_e));
@@ -392,8 +392,9 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     if (row >= n_rows) return;
     const size_t at = part0 + part + row;
     if (ln < 32) p.ml[at] = make_float2(ref, sum);
-    // (One after the other: their product may overflow.)
-    const float inv = 1.f / sum, down = power_of_two(-unit);
+    // (One after the other: their product may overflow. The sum is 0 where every score is below
+    // f32's range: weight 0 beside other keys.)
+    const float inv = sum == 0.f ? 0.f : 1.f / sum, down = power_of_two(-unit);
     float* dst = p.acc + at * D + 16 * (ln >> 5);
 #pragma unroll
     for (int i = 0; i < D / 8; i++) {

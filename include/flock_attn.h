@@ -276,11 +276,12 @@ int32_t flk_decode_layer_ragged(const float* q_raw, const float* k_raw, const fl
  * sequence, or the group's), and seq_off that falls or passes n_seqs (every row).
  *
  * q, keys, values and softmax weights enter the matrix products as two f16 parts each
- * (22 bits, relative to the element or to 2^-3 of the largest of the 32 or 64 keys
+ * (22 bits, relative to the element or to 2^-11 of the largest of the 32 or 64 keys
  * that are read together, whichever is more), the sums are f32: results are as near to
  * exact ones as those of f32 products. Any finite sizes do; where they jump by more than
- * 2^10 from some keys to the next a call may take longer. A sequence that sees a NaN or
- * an infinity among its keys or values has NaN in every dim of the heads concerned.
+ * 2^3 from some keys to the next a call may take longer. A sequence that sees a NaN or
+ * an infinity among its keys or values has NaN in the dims that they reach, and may have
+ * it in others of the same head.
  * Results are the same bits on every call. ws: flk_decode_shared_ws_bytes of the same arguments, 256-byte
  * aligned; calls that share one must be ordered on one stream. */
 uint64_t flk_decode_shared_ws_bytes(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefix,

@@ -195,7 +195,7 @@ def test_scales(case, rng):
 
 def test_values_of_growing_size(rng):
     """Later keys' values far above earlier ones', and the other way round. Keys and values
-    are off by 2^-22 of themselves or 2^-25 of the largest near them, so that a row's error is
+    are off by 2^-22 of themselves or 2^-33 of the largest near them, so that a row's error is
     within the usual bound of its largest value."""
     for order in (1, -1):
         batch = Batch(rng, [1500], [[90, 0]], q_scale=1.5)
@@ -245,6 +245,24 @@ def test_one_key_takes_all(rng):
     batch = Batch(rng, [3000], [[40, 900]], q_scale=4.0, k_scale=4.0)
     batch.k[batch.prefix_row[0] + 2990] = batch.k[batch.prefix_row[0] + 5] * 3
     batch.check()
+
+
+def test_scores_below_the_range_of_f32_have_no_weight(rng):
+    """Own keys (a part of their own) and some of the prefix so far below that their scores
+    overflow: the rest is what counts. Beside keys 2^136 times as large, which keys 0 .. 31 of
+    the prefix are (one tile), operands are off by 2^-33 of those, here by all of
+    themselves: scores of 0 instead of their own, for all but keys 32 .. 39."""
+    batch = Batch(rng, [40], [[3, 70]], q_scale=0.0)
+    batch.q[:] = 1e20
+    batch.k[batch.prefix_row[0]:][:40] *= np.float32(1e-21)
+    for at, n in [(batch.own_row[0], 3), (batch.own_row[1], 70), (batch.prefix_row[0] + 7, 5)]:
+        batch.k[at:at + n] = -1e20
+    got = batch.run()
+    rows = [batch.prefix_row[0] + i for i in range(40) if not 7 <= i < 12]
+    batch.rows = lambda b: rows
+    batch.k[batch.prefix_row[0]:][:32] = 0
+    o, tol = batch.want()
+    assert (np.abs(got - o) <= tol).all()
 
 
 @pytest.mark.parametrize("bad", [NAN, math.inf, -math.inf])

@@ -150,6 +150,19 @@ def test_attention(i, rng):
     assert np.array_equal(a, batch.run(in_place=True))
 
 
+@pytest.mark.parametrize("n,H,G,d", [(257, 2, 1, 64), (700, 2, 2, 128)])
+def test_more_groups_than_the_plan_has_threads(n, H, G, d, rng):
+    """Empty groups and groups without a prefix among them, long ones at the ends of the plan's
+    rounds; sequences in several rounds too."""
+    prefix = [int(x) for x in rng.integers(0, 70, n)]
+    own = [[int(x) for x in rng.integers(0, 40, rng.integers(0, 4))] for _ in range(n)]
+    for g in (0, 255, 256, n - 1):
+        prefix[g], own[g] = 600, [5] * 130
+    batch = Batch(rng, prefix, own, H, G, d, gap=1, before=[0, 3], after=[9])
+    a = batch.check()
+    assert np.array_equal(a, batch.run())
+
+
 def test_sequences_outside_every_group(rng):
     Batch(rng, [90, 70], [[4], [5, 6]], before=[30, 0], after=[1, 77]).check()
 

@@ -566,8 +566,7 @@ static SharedPlan plan_of(uint32_t n_groups, uint32_t n_seqs, uint32_t max_prefi
   const uint64_t tiles = row_tiles * tiles_of(max_prefix) + n_seqs * tiles_of(max_n_keys);
   p.chains = (uint32_t)(row_tiles + n_seqs);
   const uint64_t work = tiles + p.chains;
-  p.max_runs = (uint32_t)std::min((uint64_t)std::max(1u, kSharedSlots / n_kv_heads),
-                                  std::max((uint64_t)1, work / kSharedLeast));
+  p.max_runs = (uint32_t)std::min((uint64_t)std::max(1u, kSharedSlots / n_kv_heads), work);
   if (work_out) *work_out = work;
   return p;
 }

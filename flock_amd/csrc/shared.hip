@@ -472,7 +472,9 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
         unit = v_e;
         infinite = false;
       }
-      const float c_t = c_s * power_of_two(-k_e);
+      // (Not 0: masked scores are -infinity, and the others times the least normal number are
+      // next to 0 as well.)
+      const float c_t = fmaxf(c_s * power_of_two(-k_e), 1.17549435e-38f);
       if (busy) {
 #pragma unroll
         for (int kb = 0; kb < kBlocks; kb++) block(buf, kb, c_t, now.keys);

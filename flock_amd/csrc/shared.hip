@@ -472,9 +472,10 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
         unit = v_e;
         infinite = false;
       }
-      // (Not 0: masked scores are -infinity, and the others times the least normal number are
-      // next to 0 as well.)
-      const float c_t = fmaxf(c_s * power_of_two(-k_e), 1.17549435e-38f);
+      // (Neither 0 nor infinite: masked scores are -infinity, others may be 0. The least normal
+      // number leaves scores next to 0 too; with the largest those that are not lost beside the
+      // tile's largest keys overflow as well.)
+      const float c_t = fminf(fmaxf(c_s * power_of_two(-k_e), 1.17549435e-38f), 3.40282347e38f);
       if (busy) {
 #pragma unroll
         for (int kb = 0; kb < kBlocks; kb++) block(buf, kb, c_t, now.keys);

@@ -20,3 +20,13 @@ SHAPES = [([200], [[40, 0, 3]], 16, 8, 128), ([100, 30], [[70], [1]], 8, 4, 64)]
 def test_scores_next_to_zero(shape, q_scale, k_scale, rng):
     """Weights that are all the same, of key counts that fill no tile: the mean of the values."""
     Batch(rng, *shape, q_scale=q_scale, k_scale=k_scale).check()
+
+
+@pytest.mark.parametrize("size", [1e18, 1e25, 1e37])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_huge_rows_that_do_not_meet(shape, size, rng):
+    """q has even dims alone and the keys odd ones: every score is 0, whatever the sizes."""
+    batch = Batch(rng, *shape, q_scale=size, k_scale=size)
+    batch.q[..., 1::2] = 0
+    batch.k[..., ::2] *= 0  # (rows that nobody sees stay NaN)
+    batch.check()

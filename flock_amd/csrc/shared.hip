@@ -61,10 +61,13 @@ __device__ __forceinline__ uint32_t shared_fit(float top, float up) {  // top: o
   const uint64_t some = __ballot(top > 0.f);
   return large ? kLarge : fits ? kFits : some ? kSmall : 0;
 }
-__device__ __forceinline__ bool shared_misfit(const uint32_t (&of)[kShThreads / 64]) {
-  // (k's in the low half, v's above.)
+// Those of a tile: k's in the low half, v's above.
+__device__ __forceinline__ uint32_t shared_fits_of(const uint32_t (&of)[kShThreads / 64]) {
   const uint4 fit = *reinterpret_cast<const uint4*>(of);
-  const uint32_t x = uniform(fit.x | fit.y | fit.z | fit.w), k = x & 0xffff, v = x >> 16;
+  return uniform(fit.x | fit.y | fit.z | fit.w);
+}
+__device__ __forceinline__ bool shared_misfit(uint32_t fits) {
+  const uint32_t k = fits & 0xffff, v = fits >> 16;
   return ((k | v) & kLarge) || k == kSmall || v == kSmall;
 }
 
@@ -110,7 +113,7 @@ struct SharedTile {
   uint32_t keys;          // it holds
   uint32_t row0, n_rows;  // they meet
   uint32_t part;          // where the rows' results go
-  uint32_t first, last;   // of the run's tiles of its chain: 1
+  uint32_t last;          // of the run's tiles of its chain: 1
 };
 
 template <int D>
@@ -146,14 +149,11 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     next.once = kind & kSharedOnce;
     next.part = uniform(c[6]) == run ? next.row0 + (kind & kSharedOwn ? rows : 0)
                                      : 2 * rows + run * kSharedRows;
-    next.first = 1;
   };
   auto advance = [&] {  // next: one tile on
     if (next.last) {
       e++;
       open();
-    } else {
-      next.first = 0;
     }
     next.at = ((key_row + (uint64_t)in_chain * kTile) * G + kvh) * D;
     next.keys = uniform(min(n_keys - in_chain * kTile, (uint32_t)kTile));
@@ -206,7 +206,11 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
   // in 2^8 .. 2^16 with them, or are 0: then two parts in f16 are off by 2^-25 at most, 2^-33
   // of the largest. So a tile need not be seen as a whole before it is split: each wave
   // notes how its part fits, and the tile is done again if need be.
-  int k_e = 0, v_e = 0, v_low = 0;  // v_low: the least v_e of the chain
+  int k_e = 0, v_e = 0;
+  // The least v_e of the chain's tiles so far that held values other than 0; kNoValues: none did,
+  // and the accumulators are 0.
+  constexpr int kNoValues = 50;
+  int v_low = kNoValues;
   // An eighth of the tile in registers into LDS.
   auto stage_part = [&](int buf, int part, float k_up, float v_up) {
     const int i = part & 3;
@@ -238,10 +242,10 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
   };
   // The factors from the tile in registers, 2^11 .. 2^12 its largest values with them, and
   // the tile into LDS; by all waves. (V's is at most 2^60 of the chain's least, so that
-  // accumulators stay finite.) Whether V holds an infinity: its rows are NaN, and the factor
-  // is as before. (Where every tile's sizes jump by 2^4, a call takes 119 us for 68, 16 sequences
+  // accumulators stay finite.) The exponent of V's largest: at 128 it holds an infinity, its
+  // rows are NaN, and the factor is as before. (Where every tile's sizes jump by 2^4, a call takes 119 us for 68, 16 sequences
   // over 32k keys, or 767 for 541, 128 over 128k.)
-  auto anchor = [&](int buf, bool first) {
+  auto anchor = [&](int buf) {
     float k = 0.f, v = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -258,13 +262,11 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     const int ke = exponent(uniform_f(fmaxf(fmaxf(kt.x, kt.y), fmaxf(kt.z, kt.w))));
     const int ve = exponent(uniform_f(fmaxf(fmaxf(vt.x, vt.y), fmaxf(vt.z, vt.w))));
     if (ke != -127 && ke != 128) k_e = max(11 - max(ke, -100), -115);
-    if (ve != -127 && ve != 128)
-      v_e = max(min(11 - max(ve, -100), first ? 110 : v_low + 60), -115);
-    v_low = first ? v_e : min(v_low, v_e);
+    if (ve != -127 && ve != 128) v_e = max(min(11 - max(ve, -100), v_low + 60), -115);
 #pragma unroll
     for (int i = 0; i < 8; i++) stage_part(buf, i, power_of_two(k_e), power_of_two(v_e));
     lds_barrier();
-    return ve == 128;
+    return ve;
   };
 
   // This wave's rows (lanes behind the last repeat it), q in two parts: dims 16 s + 8 h ..
@@ -419,11 +421,10 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
   open();
   next.last = 0;
   advance();
-  next.first = 1;
   fetch(next);
   SharedTile staged = next;
   if (wave * 32u < staged.n_rows) load_q(staged.row0, staged.n_rows);
-  bool infinite = anchor(0, true);
+  const int top_v = anchor(0);
   if (n > 1) {
     advance();
     fetch(next);
@@ -435,7 +436,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     ref = -INFINITY, l = 0.f;
 #pragma unroll
     for (int x = 0; x < kOT; x++) o[x] = floatx16v{};
-    v_low = v_e;
+    v_low = kNoValues;
     int unit = v_e;  // accumulators hold O^T 2^unit
     uint32_t last;
     do {  // their tiles
@@ -447,10 +448,16 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
       const SharedTile now = staged;
       last = now.last;
       if (t + 1 < n) staged = next;
-      if (t > 0 && shared_misfit(sh.fit[buf])) {
-        fetch(now);
-        infinite = anchor(buf, now.first);
-        if (t + 1 < n) fetch(staged);
+      bool values = top_v != -127, infinite = top_v == 128;
+      if (t > 0) {
+        const uint32_t fits = shared_fits_of(sh.fit[buf]);
+        values = fits >> 16;
+        infinite = false;
+        if (shared_misfit(fits)) {
+          fetch(now);
+          infinite = anchor(buf) == 128;
+          if (t + 1 < n) fetch(staged);
+        }
       }
       // (Behind the run's last tile what is staged is not read.)
       if (busy) {
@@ -464,14 +471,15 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
         advance();
         fetch(next);
       }
-      if (v_e != unit || infinite) {  // (a chain's first tile meets zeros)
-        const float alpha =
-            infinite ? __builtin_nanf("") : now.first ? 0.f : ldexpf(1.f, v_e - unit);
+      if (v_e != unit || infinite) {
+        const float alpha = infinite             ? __builtin_nanf("")
+                            : v_low == kNoValues ? 0.f
+                                                 : ldexpf(1.f, v_e - unit);
 #pragma unroll
         for (int x = 0; x < kOT; x++) o[x] *= alpha;
         unit = v_e;
-        infinite = false;
       }
+      if (values) v_low = min(v_low, v_e);
       // (Neither 0 nor infinite: masked scores are -infinity, others may be 0. The least normal
       // number leaves scores next to 0 too; with the largest those that are not lost beside the
       // tile's largest keys overflow as well.)

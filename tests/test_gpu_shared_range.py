@@ -30,3 +30,18 @@ def test_huge_rows_that_do_not_meet(shape, size, rng):
     batch.q[..., 1::2] = 0
     batch.k[..., ::2] *= 0  # (rows that nobody sees stay NaN)
     batch.check()
+
+
+@pytest.mark.parametrize("H,d,tile", [(64, 64, 64), (64, 128, 32)])
+def test_values_that_begin_with_zeros(H, d, tile, rng):
+    """Prefixes of large values and, behind each in the same run, one whose first tile of values
+    is zeros and the second tiny: a run holds two chains (64 kv heads have 8 runs each, and a
+    chain of two tiles counts as three)."""
+    batch = Batch(rng, [2 * tile] * 16, [[0]] * 16, H, 64, d)
+    for g, at in enumerate(batch.prefix_row):
+        if g % 2 == 0:
+            batch.v[at:at + 2 * tile] *= np.float32(2.0 ** 90)
+        else:
+            batch.v[at:at + tile] = 0
+            batch.v[at + tile:at + 2 * tile] *= np.float32(2.0 ** (-100 if g % 4 == 1 else 100))
+    batch.check()

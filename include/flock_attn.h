@@ -275,11 +275,17 @@ int32_t flk_decode_layer_ragged(const float* q_raw, const float* k_raw, const fl
  * see is refused on the device, with NaN rows: a count beyond its bound (the
  * sequence, or the group's), and seq_off that falls or passes n_seqs (every row).
  *
- * q, keys, values and softmax weights enter the matrix products as two f16 parts each
- * (22 bits, relative to the element or to 2^-11 of the largest of the 32 or 64 keys
- * that are read together, whichever is more), the sums are f32: results are as near to
- * exact ones as those of f32 products. Any finite sizes do; where they jump by more than
- * 2^3 from some keys to the next a call may take longer. A sequence that sees a NaN or
+ * q, keys, values and softmax weights enter the matrix products as two f16 parts each,
+ * the sums are f32. An element is off by 2^-22 of itself at most, or by the largest of
+ * these where that is more:
+ *   q        2^-39 of the largest of its row
+ *   keys     2^-33 of the largest of the 32 or 64 keys that are read together, and 2^-135
+ *   values   the same, and 2^-81 of the largest value before it in the prefix or own keys
+ *   weights  2^-19 of the largest weight among the 32 keys around it, and 2^-85 of the sum
+ *            of the row's weights
+ * So results are as near to exact ones as those of f32 products, also where one key takes
+ * nearly all of the weight and has small values. Any finite sizes do; where they jump by
+ * more than 2^3 from some keys to the next a call may take longer. A sequence that sees a NaN or
  * an infinity among its keys or values has NaN in the dims that they reach, and may have
  * it in others of the same head.
  * Results are the same bits on every call. ws: flk_decode_shared_ws_bytes of the same arguments, 256-byte

@@ -7,7 +7,7 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_shared import Batch
+from test_gpu_shared import SHAPES as ATTENTION, Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,69 @@ def test_values_that_begin_with_zeros(H, d, tile, rng):
             batch.v[at:at + tile] = 0
             batch.v[at + tile:at + 2 * tile] *= np.float32(2.0 ** (-100 if g % 4 == 1 else 100))
     batch.check()
+
+
+def two_norms(got, o):
+    return np.linalg.norm(got - o, axis=-1), np.linalg.norm(o, axis=-1)
+
+
+@pytest.mark.parametrize("i", range(len(ATTENTION)))
+def test_rows_in_the_2_norm(i, rng):
+    """Ordinary rows are as exact as f32 products make them: a score (some 2 nats, of products
+    that are off by 2^-22 each with either sign) is off by 2^-21 or so, its weight by as much of
+    itself, values by 2^-22; the errors of a row's weights have either sign, so that the row's is
+    theirs. 2^-18 is eight times that, and a thirtieth of what a lost second part (2^-11 to 2^-13)
+    makes of any of the four operands."""
+    prefix, own, H, G, d = ATTENTION[i]
+    batch = Batch(rng, prefix, own, H, G, d, q_scale=2.0)
+    o, _ = batch.want()
+    off, size = two_norms(batch.run(), o)
+    assert (off <= 2.0 ** -18 * size).all(), (off / size).max()
+
+
+def sink(batch, at, gap, rng):
+    """Row `at` of the caches takes `gap` nats more than other keys on average, and has no
+    values."""
+    G, d = batch.G, batch.d
+    u = rng.standard_normal((G, d)).astype(np.float32)
+    u /= np.linalg.norm(u, axis=-1, keepdims=True)
+    batch.k -= (batch.k * u).sum(-1, keepdims=True) * u
+    heads = np.repeat(u, batch.H // G, axis=0)
+    batch.q += 16 * heads
+    batch.k[at] = u * np.float32(gap * math.sqrt(d) / 16)
+    batch.v[at] = 0
+
+
+@pytest.mark.parametrize("gap", [8, 15, 20, 25, 35])
+@pytest.mark.parametrize("P,own,H,G,d,at", [
+    (513, [9, 0], 16, 8, 128, 0), (513, [9, 0], 32, 8, 64, 0),
+    (9000, [3] * 5, 4, 2, 128, 0), (9000, [40], 4, 4, 64, 4321), (200, [70, 900], 16, 8, 128, 150),
+])
+def test_a_key_that_takes_the_weight_and_has_no_values(P, own, H, G, d, at, gap, rng):
+    """What is left of the row is as exact, of its own size, as without that key: as in
+    test_rows_in_the_2_norm, and the score of that key (all others' share hangs on it), a sum
+    of 24 products in f32 whose roundings are 2^-24 of it each, 2^-22 in all where half of
+    them agree."""
+    batch = Batch(rng, [P], [own], H, G, d, q_scale=2.0)
+    sink(batch, batch.prefix_row[0] + at, gap, rng)
+    o, _ = batch.want()
+    off, size = two_norms(batch.run(), o)
+    print(gap, (off / size).max(), flush=True)
+    assert (off <= (2.0 ** -18 + 1.5 * gap * 2.0 ** -22) * size).all(), (off / size).max()
+
+
+def test_many_keys_that_take_the_weight(rng):
+    """The same with such a key in every group's prefix and every sequence's own keys, which lie in
+    few runs (64 kv heads have 8 runs each)."""
+    batch = Batch(rng, [300] * 12, [[200, 33]] * 12, 64, 64, 64, q_scale=2.0)
+    k, q, v = batch.k, batch.q, batch.v
+    u = np.zeros((64, 64), np.float32)
+    u[:, 0] = 1
+    k[..., 0] = np.where(np.isnan(k[..., 0]), k[..., 0], 0)
+    q += 16 * u
+    for i, at in enumerate(batch.prefix_row + batch.own_row):
+        k[at + i % 30, :, 0] += 10 + i % 3 * 4
+        v[at + i % 30] = 0
+    o, _ = batch.want()
+    off, size = two_norms(batch.run(), o)
+    assert (off <= (2.0 ** -18 + 60 * 2.0 ** -22) * size).all(), (off / size).max()

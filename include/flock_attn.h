@@ -284,8 +284,10 @@ int32_t flk_decode_layer_ragged(const float* q_raw, const float* k_raw, const fl
  *   weights  2^-19 of the largest weight among the 32 keys around it, and 2^-85 of the sum
  *            of the row's weights
  * So results are as near to exact ones as those of f32 products, also where one key takes
- * nearly all of the weight and has small values. Any finite sizes do; where they jump by
- * more than 2^3 from some keys to the next a call may take longer. A sequence that sees a NaN or
+ * nearly all of the weight and has small values. Any finite sizes do, as long as scores
+ * are finite: a key whose score overflows to -infinity has no weight, and a row that has no
+ * other key, or one whose score overflows to +infinity, is NaN. Where sizes jump by more than
+ * 2^3 from some keys to the next a call may take longer. A sequence that sees a NaN or
  * an infinity among its keys or values has NaN in the dims that they reach, and may have
  * it in others of the same head.
  * Results are the same bits on every call. ws: flk_decode_shared_ws_bytes of the same arguments, 256-byte

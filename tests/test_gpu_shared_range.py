@@ -111,3 +111,23 @@ def test_many_keys_that_take_the_weight(rng):
     o, _ = batch.want()
     off, size = two_norms(batch.run(), o)
     assert (off <= (2.0 ** -18 + 60 * 2.0 ** -22) * size).all(), (off / size).max()
+
+
+@pytest.mark.parametrize("H,G,d", [(16, 8, 128), (8, 4, 64)])
+def test_scores_past_the_range_of_f32(H, G, d, rng):
+    """Scores of -infinity have no weight beside others (of the prefix or own), and a row with
+    none else is NaN, as one with a score of +infinity is."""
+    batch = Batch(rng, [70, 70], [[40, 3], [5, 90]], H, G, d, q_scale=0.0)
+    batch.q[:] = 1e20
+    for g, size in ((0, -1e20), (1, 1e-21)):
+        at = batch.prefix_row[g]
+        batch.k[at:at + 70] = np.float32(size)
+    for b, size in enumerate((-1e20, 1e-21, -1e20, 1e20)):
+        at = batch.own_row[b]
+        batch.k[at:at + batch.n_keys[b]] = np.float32(size)
+    got = batch.run()
+    assert np.isnan(got[[0, 3]]).all()
+    for b, row, n in ((1, batch.own_row[1], 3), (2, batch.prefix_row[1], 70)):
+        batch.rows = lambda _: list(range(row, row + n))
+        o, tol = batch.want([b])
+        assert (np.abs(got[b] - o[b]) <= tol[b]).all()

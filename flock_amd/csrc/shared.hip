@@ -37,10 +37,12 @@ namespace flk {
 // have fallen behind by kDrop, these are taken first, against a reference of their own. So a
 // key that takes nearly all of the weight and has small values leaves the others as exact as they are
 // without it: with such a key 20 nats above 512 others, 5e-7 off in the 2-norm (f32 5e-7), and 1.4e-4
-// against the largest score so far alone. It falls no farther than l stays below 2^kRoom by. The
-// blocks of ordinary scores (2 nats around their mean) rise and fall as seldom as with the largest
-// score: calls take 0 to 1.5 % longer than with that.
-constexpr float kDrop = 16.f, kFar = 8.f;
+// against the largest score so far alone. A row whose accumulators are kSolid times its sum (of
+// values that are 2^16 at most) does not fall: 2^-25 is little beside what it holds. Nor
+// does one fall farther than l stays below 2^kRoom by. Ordinary scores (2 nats around their mean)
+// rise as often as with the largest score alone, and calls take 0 to 1.5 % longer; with scores 8
+// nats around it -1 to 11 % (32 % without kSolid, whose rows fall and rise in turn).
+constexpr float kDrop = 16.f, kFar = 8.f, kSolid = 256.f;
 constexpr int kRoom = 60;
 
 typedef float floatx16v __attribute__((ext_vector_type(16)));
@@ -312,6 +314,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
 
   floatx16v o[kOT];
   float ref = -INFINITY, l = 0.f;
+  float under = -INFINITY;  // where the reference falls
   floatx16v scores[kBlocks];
   // The scores of the tile in LDS and, among their products, the next tile's way there.
   auto products = [&](int buf) {
@@ -367,6 +370,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     };
     auto move = [&](float to) {
       const float alpha = to == ref ? 1.f : __builtin_amdgcn_exp2f(ref - to);
+      under = to == ref ? under : to - kDrop;
       ref = to;
       if (__ballot(alpha != 1.f && l > 0.f) == 0) return;  // (of accumulators that are 0 as well)
       l *= alpha;
@@ -407,8 +411,14 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
       }
     }
     float to = fmaxf(ref, top);
-    const bool falls = top < ref - kDrop && top > -INFINITY;
+    bool falls = top < under && top > -INFINITY;
     if (__ballot(falls)) {
+      float size = 0.f;
+#pragma unroll
+      for (int x = 0; x < kOT; x++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) size = fmaxf(size, fabsf(o[x][i]));
+      if (max_xor<32>(size) >= max_xor<32>(l) * kSolid) under = -INFINITY, falls = false;
       const float down = fall(top);
       to = falls ? down : to;
     }
@@ -425,8 +435,8 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
 #pragma unroll
     for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
     top *= c_t;
-    const float from = top - ref;
-    if (__ballot(!(fabsf(from - (kSlack - kDrop) / 2) <= (kSlack + kDrop) / 2)))
+    const uint64_t rises = __ballot(top > ref + kSlack), falls = __ballot(top < under);
+    if (rises | (uint32_t)(falls & falls >> 32))  // (a row's lanes are i and i + 32)
       follow(s, buf, kb, c_t, top);
     const float rb = (ref == -INFINITY ? 0.f : ref) - kBias;
 #pragma unroll
@@ -499,7 +509,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
     const uint32_t n_rows = staged.n_rows, part = staged.part;
     const bool busy = wave * 32u < n_rows;
     if (busy && t > 0) load_q(staged.row0, n_rows);
-    ref = -INFINITY, l = 0.f;
+    ref = under = -INFINITY, l = 0.f;
 #pragma unroll
     for (int x = 0; x < kOT; x++) o[x] = floatx16v{};
     v_low = kNoValues;
@@ -549,6 +559,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(SharedArgs a
       // (Neither 0 nor infinite: masked scores are -infinity, others may be 0. The least normal
       // number leaves scores next to 0 too; with the largest those that are not lost beside the
       // tile's largest keys overflow as well.)
+      if (t % 16 == 0) under = ref - kDrop;  // (what is solid is looked at again)
       const float c_t = fminf(fmaxf(c_s * power_of_two(-k_e), 1.17549435e-38f), 3.40282347e38f);
       if (busy) {
 #pragma unroll

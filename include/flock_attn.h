@@ -281,8 +281,9 @@ int32_t flk_decode_layer_ragged(const float* q_raw, const float* k_raw, const fl
  *   q        2^-39 of the largest of its row
  *   keys     2^-33 of the largest of the 32 or 64 keys that are read together, and 2^-135
  *   values   the same, and 2^-81 of the largest value before it in the prefix or own keys
- *   weights  2^-19 of the largest weight among the 32 keys around it, and 2^-85 of the sum
- *            of the row's weights
+ *   weights  2^-19 of the largest weight among the 32 keys around it (or 2^-35 of the sum of
+ *            the row's weights, while its result so far is 2^-8 of the largest value or
+ *            more), and 2^-85 of that sum
  * So results are as near to exact ones as those of f32 products, also where one key takes
  * nearly all of the weight and has small values. Any finite sizes do, as long as scores
  * are finite: a key whose score overflows to -infinity has no weight, and a row that has no

@@ -131,3 +131,20 @@ def test_scores_past_the_range_of_f32(H, G, d, rng):
         batch.rows = lambda _: list(range(row, row + n))
         o, tol = batch.want([b])
         assert (np.abs(got[b] - o[b]) <= tol[b]).all()
+
+
+@pytest.mark.parametrize("size", [0.3, 0.02, 1e-3])
+@pytest.mark.parametrize("spread", [2.0, 8.0])
+@pytest.mark.parametrize("H,G,d", [(16, 8, 128), (32, 8, 64)])
+def test_a_key_that_takes_the_weight_and_has_small_values(H, G, d, spread, size, rng):
+    """The same with values of a part of the others' size, also where scores lie far apart (a sum
+    of more products in turn: scores up to 4 spread, and the gap)."""
+    batch = Batch(rng, [2900], [[40, 200, 0]], H, G, d, q_scale=spread)
+    at = batch.prefix_row[0]
+    v = batch.v[at].copy()
+    sink(batch, at, 20, rng)
+    batch.v[at] = v * np.float32(size)
+    o, _ = batch.want()
+    off, norm = two_norms(batch.run(), o)
+    print(size, (off / norm).max(), flush=True)
+    assert (off <= (2.0 ** -18 + 1.5 * (20 + 4 * spread) * 2.0 ** -22) * norm).all()

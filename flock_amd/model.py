@@ -257,10 +257,12 @@ class Model:
             raise ValueError(f"{n} answers: 1 .. maxPrefill ({self.cfg.maxPrefill}) at a time")
         if not 1 <= top_k <= 64:
             raise ValueError(f"top_k must be 1 .. 64, got {top_k}")
-        if not 0 <= temperature < np.inf:
-            raise ValueError(f"temperature must be finite and >= 0, got {temperature}")
-        if not top_p > 0 or not 0 <= min_p <= 1:
-            raise ValueError(f"top_p must be > 0 and min_p 0 .. 1, got {top_p} and {min_p}")
+        with np.errstate(over="ignore"):  # (what the device gets)
+            settings = np.float32(temperature), np.float32(top_p)
+        if not temperature >= 0 or not settings[0] < np.inf:
+            raise ValueError(f"temperature must be finite and >= 0 in f32, got {temperature}")
+        if not settings[1] > 0 or not 0 <= min_p <= 1:
+            raise ValueError(f"top_p must be > 0 in f32 and min_p 0 .. 1, got {top_p} and {min_p}")
         if maxTokens < 1:
             return [([], []) for _ in range(n)]
         held = self.nKeys + prompt.size - 1

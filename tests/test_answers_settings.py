@@ -1,0 +1,33 @@
+"""What Model.answers refuses before it feeds anything (no GPU needed: nothing is launched)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from flock_amd.decoder import DecoderConfig
+from flock_amd.model import Model
+
+
+class Fed(Exception):
+    pass
+
+
+@pytest.fixture
+def model():
+    """A model that is never run: what would feed or capture raises."""
+    m = Model.__new__(Model)
+    m.cfg, m.vocab, m.nKeys = DecoderConfig(maxKeys=64, maxPrefill=8), 500, 0
+
+    def fed(*_):
+        raise Fed
+    m._feed = m._answers_step = fed
+    return m
+
+
+@pytest.mark.parametrize("settings", [dict(temperature=1e39), dict(temperature=3.5e38),
+                                      dict(top_p=1e-50), dict(top_p=7e-46),
+                                      dict(temperature=-1e-50), dict(temperature=float("nan"))])
+def test_settings_that_f32_does_not_hold(model, settings):
+    """They are f32 on the device: infinite or 0 there, which flk_sample refuses."""
+    with pytest.raises(ValueError):
+        model.answers([1, 2], 2, 2, **settings)

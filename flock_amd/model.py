@@ -253,6 +253,8 @@ class Model:
         prompt = np.ascontiguousarray(prompt, np.uint32).ravel()
         if prompt.size == 0:
             raise ValueError("answers need at least one token id")
+        if prompt.max() >= self.vocab:
+            raise ValueError(f"id {prompt.max()} of a vocabulary of {self.vocab}")
         if n < 1 or n > max(1, self.cfg.maxPrefill):
             raise ValueError(f"{n} answers: 1 .. maxPrefill ({self.cfg.maxPrefill}) at a time")
         if not 1 <= top_k <= 64:

@@ -31,3 +31,12 @@ def test_settings_that_f32_does_not_hold(model, settings):
     """They are f32 on the device: infinite or 0 there, which flk_sample refuses."""
     with pytest.raises(ValueError):
         model.answers([1, 2], 2, 2, **settings)
+
+
+@pytest.mark.parametrize("prompt", [[500], [1, 2, 500], [499, 1 << 31, 3], np.array([-1, 2])])
+def test_ids_outside_the_vocabulary(model, prompt):
+    """The embedding reads them as zeros."""
+    with pytest.raises(ValueError):
+        model.answers(prompt, 2, 2)
+    assert model.nKeys == 0
+

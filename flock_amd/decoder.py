@@ -236,7 +236,7 @@ class DecoderLayer:
         bookkeeping."""
         cfg, b, g = self.cfg, self.buf, self.g
         H, Hkv, d, n = cfg.nHeads, cfg.nKvHeads, cfg.headDim, batch.n_seqs
-        if n > cfg.maxPrefill:
+        if n > max(1, cfg.maxPrefill):
             raise ValueError(f"{n} sequences exceed maxPrefill {cfg.maxPrefill}")
         qkv, row = b["qkv"].ptr, (H + 2 * Hkv) * d
         ops.q8_matvec_ex(self.w_qkv, src, b["qkv"], n, norm_gain=g["attn_norm.weight"],

@@ -239,6 +239,16 @@ class Model:
         ops.set_stream(None)
         return out
 
+    def _answers_step(self, *key) -> "_Answers":
+        """The captured step of ``key`` (answers, ids, stops), kept from call to call."""
+        if self._answers is None or self._answers.key != key:
+            ops.sync()  # (what has been launched, on whichever stream)
+            if self._answers is not None:
+                self._answers.free()
+                self._answers = None
+            self._answers = _Answers(self, *key)
+        return self._answers
+
     def answers(self, prompt, n: int, maxTokens: int, eos=(), temperature: float = 1.0,
                 top_k: int = 64, top_p: float = 1.0, min_p: float = 0.0, seed=None) -> list:
         """n answers to ``prompt`` (fed at positions nKeys..), drawn together: a list of
@@ -271,17 +281,14 @@ class Model:
         if held + n * maxTokens > self.cfg.maxKeys:
             raise CacheFullError(-2, f"KV cache would exceed {self.cfg.maxKeys} keys "
                                      f"({held} + {n} x {maxTokens})")
+        eos = sorted(set(int(e) for e in eos))
+        u32, f32 = np.uint32, np.float32
+        uniform = np.random.default_rng(seed).random((maxTokens, n), f32)
+        # The prompt is fed when nothing is left that could fail.
+        a = self._answers_step(n, maxTokens, len(eos))
         for _ in self._feed(prompt[:-1]):
             pass
         ops.sync()  # (the captured step is on a stream of its own)
-        eos = sorted(set(int(e) for e in eos))
-        key = (n, maxTokens, len(eos))
-        if self._answers is None or self._answers.key != key:
-            if self._answers is not None:
-                self._answers.free()
-                self._answers = None
-            self._answers = _Answers(self, *key)
-        a, u32, f32 = self._answers, np.uint32, np.float32
         a.n_prefix.upload(np.array([held], u32))
         a.seq_row_off.upload(held + maxTokens * np.arange(n, dtype=np.uint64))
         a.n_keys.upload(np.ones(n, u32))
@@ -292,7 +299,6 @@ class Model:
             buf.upload(np.full(n, x, t))
         if eos:
             a.stops.upload(np.array(eos, u32))
-        uniform = np.random.default_rng(seed).random((maxTokens, n), f32)
         a.uniform_log.upload(uniform)
         a.uniform.upload(uniform[0])
         done = 0

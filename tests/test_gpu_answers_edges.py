@@ -1,0 +1,44 @@
+"""Model.answers at the edges of its arguments: a model without prefill, calls that fail."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+from flock_amd import ops  # noqa: E402
+from flock_amd.model import Model  # noqa: E402
+from test_gpu_model import VOCAB, build  # noqa: E402
+
+
+def test_a_model_that_takes_one_id_at_a_time(rng):
+    """maxPrefill 0: one answer at a time, the ids that one of maxPrefill 1 gives."""
+    got = []
+    for P in (0, 1):
+        cfg, layers, embd, gout = build(np.random.default_rng(3), maxPrefill=P)
+        m = Model(cfg, layers, embd, gout, VOCAB)
+        got.append(m.answers([3, 14, 15], 1, 5, seed=4))
+        assert m.nKeys == 2
+        with pytest.raises(ValueError):
+            m.answers([3, 14, 15], 2, 5)
+        m.free()
+    assert got[0] == got[1] and len(got[0][0][0]) == 5
+
+
+def test_a_call_that_fails_feeds_nothing(rng, monkeypatch):
+    cfg, layers, embd, gout = build(rng)
+    m = Model(cfg, layers, embd, gout, VOCAB)
+    first = m.answers([3, 14, 15], 2, 3, seed=4)
+    m.reset()
+    with pytest.raises((ValueError, TypeError)):
+        m.answers([9, 14, 15, 16], 2, 3, seed=-1)
+
+    def failing(*_, **__):
+        raise MemoryError
+    with monkeypatch.context() as patch:
+        patch.setattr(ops, "sample", failing)
+        with pytest.raises(MemoryError):
+            m.answers([9, 14, 15, 16], 2, 4, seed=4)
+    assert m.nKeys == 0 and all(layer.nKeys == 0 for layer in m.layers)
+    assert m.answers([3, 14, 15], 2, 3, seed=4) == first
+    m.free()

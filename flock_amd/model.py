@@ -281,7 +281,7 @@ class Model:
         if held + n * maxTokens > self.cfg.maxKeys:
             raise CacheFullError(-2, f"KV cache would exceed {self.cfg.maxKeys} keys "
                                      f"({held} + {n} x {maxTokens})")
-        eos = sorted(set(int(e) for e in eos))
+        eos = sorted(set(int(e) for e in eos if 0 <= e < self.vocab))
         u32, f32 = np.uint32, np.float32
         uniform = np.random.default_rng(seed).random((maxTokens, n), f32)
         # The prompt is fed when nothing is left that could fail.

@@ -40,3 +40,15 @@ def test_ids_outside_the_vocabulary(model, prompt):
         model.answers(prompt, 2, 2)
     assert model.nKeys == 0
 
+
+
+@pytest.mark.parametrize("eos,stops", [([-1], 0), ([1 << 32], 0), ([3, 1 << 40, 7, 3], 2),
+                                       ([500, 499], 1), (np.array([-5, 4]), 1)])
+def test_stops_outside_the_vocabulary(model, eos, stops):
+    """As for generate, an id that is never drawn ends nothing."""
+    def step(*key):
+        assert key == (2, 2, stops)
+        raise Fed
+    model._answers_step = step
+    with pytest.raises(Fed):
+        model.answers([1, 2], 2, 2, eos=eos)

@@ -42,3 +42,12 @@ def test_a_call_that_fails_feeds_nothing(rng, monkeypatch):
     assert m.nKeys == 0 and all(layer.nKeys == 0 for layer in m.layers)
     assert m.answers([3, 14, 15], 2, 3, seed=4) == first
     m.free()
+
+
+def test_stops_outside_the_vocabulary_end_nothing(rng):
+    cfg, layers, embd, gout = build(rng)
+    m = Model(cfg, layers, embd, gout, VOCAB)
+    first = m.answers([3, 14, 15], 3, 4, seed=4)
+    m.reset()
+    assert m.answers([3, 14, 15], 3, 4, seed=4, eos=[-1, VOCAB, 1 << 32]) == first
+    m.free()

@@ -255,7 +255,8 @@ class Model:
         (ids, their log probabilities), each up to maxTokens long and ending before an id in
         ``eos``. Tokens come from the top_k (up to 64) largest logits as ops.sample draws
         them, temperature 0 takes the largest; log probabilities are the model's own, whatever
-        the settings. ``seed`` fixes the random numbers.
+        the settings. ``seed`` fixes the random numbers. RuntimeError where an answer's logits
+        hold nothing to draw (all NaN or -infinity).
 
         A step is one replay of a captured step of all answers: their queries meet the
         prompt's keys together. The prompt's last id is each answer's first input, so
@@ -319,6 +320,9 @@ class Model:
         for b in range(n):
             stop = np.flatnonzero(np.isin(ids[:, b], eos + [0xffffffff]))
             end = stop[0] if stop.size else done
+            if end < done and ids[end, b] == 0xffffffff:
+                raise RuntimeError(f"answer {b} has no id {end}: none of its logits is above "
+                                   "-infinity")
             out.append(([int(t) for t in ids[:end, b]], [float(x) for x in logprob[:end, b]]))
         return out
 

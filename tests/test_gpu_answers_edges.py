@@ -51,3 +51,19 @@ def test_stops_outside_the_vocabulary_end_nothing(rng):
     m.reset()
     assert m.answers([3, 14, 15], 3, 4, seed=4, eos=[-1, VOCAB, 1 << 32]) == first
     m.free()
+
+
+def test_an_answer_without_a_draw_is_an_error(rng):
+    """Logits that hold nothing but NaN: not the same as answers that stop at once."""
+    cfg, layers, embd, gout = build(rng)
+    m = Model(cfg, layers, embd, gout, VOCAB)
+    first = m.answers([3, 14, 15], 2, 3, seed=4)
+    m.reset()
+    m.g_out.upload(np.full(cfg.hidden, np.nan, np.float32))
+    for eos in ([], [7]):
+        with pytest.raises(RuntimeError, match="no id"):
+            m.answers([3, 14, 15], 2, 3, seed=4, eos=eos)
+        m.reset()
+    m.g_out.upload(gout)
+    assert m.answers([3, 14, 15], 2, 3, seed=4) == first
+    m.free()

@@ -470,7 +470,8 @@ __global__ __launch_bounds__(kTokenThreads) void token_join_kernel(TokenArgs a, 
 }
 
 // Rows are cut where a workgroup each would leave CUs idle, into parts of two chunks a wave at
-// least. Calls, us, cut into 256 / 512 / 1024 workgroups: 64 rows of 151936 18.8 / 17.6 / 24.7,
+// least. (With alternatives two of their workgroups fit a CU: 512 are one round of the GPU, 1024
+// two.) Calls, us, cut into 256 / 512 / 1024 workgroups: 64 rows of 151936 18.8 / 17.6 / 24.7,
 // 100 of 50021 16.1 / 15.2 / 19.2; 256 rows of 151936, uncut / in four 32.4 / 40.7. One row, its
 // parts of one chunk a wave at least / two / four: 14.2 / 13.1 / 13.5.
 constexpr uint32_t kTokenGroups = 512, kTokenLeast = 2;
@@ -519,8 +520,8 @@ hipError_t launch_tokens(const TokenArgs& a, void* ws, hipStream_t st) {
       if (b.uniform) b.uniform += r, b.token += r;
     }
     const dim3 grid(p.splits, b.n_rows), threads(kTokenThreads);
-    // Long segments look again seldom, short ones leave LDS for five workgroups a CU instead of
-    // three. us, segments of 40 / 20: 256 rows of 151936, 50 alternatives 32.4 / 37, 600 of 65000
+    // Long segments look again seldom, short ones leave LDS for four workgroups a CU instead of
+    // two (34880 and 55360 bytes). us, segments of 40 / 20: 256 rows of 151936, 50 alternatives 32.4 / 37, 600 of 65000
     // 44.3 / 35.1, 2048 of 151936 230 / 222.
     const bool entropy = a.entropy != nullptr, few = a.n_rows < 512;
     const auto kernel =

@@ -254,8 +254,9 @@ class Model:
         """n answers to ``prompt`` (fed at positions nKeys..), drawn together: a list of
         (ids, their log probabilities), each up to maxTokens long and ending before an id in
         ``eos``. Tokens come from the top_k (up to 64) largest logits as ops.sample draws
-        them, temperature 0 takes the largest; log probabilities are the model's own, whatever
-        the settings. ``seed`` fixes the random numbers. RuntimeError where an answer's logits
+        them (never from the whole vocabulary), temperature 0 takes the largest; log
+        probabilities are the model's own, whatever the settings: not those of the draw, which is
+        of the alternatives that stay. ``seed`` fixes the random numbers. RuntimeError where an answer's logits
         hold nothing to draw (all NaN or -infinity).
 
         A step is one replay of a captured step of all answers: their queries meet the

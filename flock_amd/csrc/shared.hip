@@ -597,8 +597,12 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a, SharedP
     if (i == 0) return part0 + rows + at_row;
     return part0 + 2 * rows + (size_t)(r.own_run + i) * kSharedRows + head % m;
   };
+  // (The largest weight is below 2: sums reach 2^62, and their product with huge values f32's end.)
   float top = -INFINITY;
-  for (uint32_t i = e; i < n; i += kLanes) top = fmaxf(top, p.ml[at(i)].x);
+  for (uint32_t i = e; i < n; i += kLanes) {
+    const float2 ml = p.ml[at(i)];
+    top = fmaxf(top, ml.x + (float)exponent(ml.y));
+  }
 #pragma unroll
   for (uint32_t x = 1; x < kLanes; x <<= 1) top = fmaxf(top, shfl_xor(top, x));
   float4 f = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -148,3 +148,23 @@ def test_a_key_that_takes_the_weight_and_has_small_values(H, G, d, spread, size,
     off, norm = two_norms(batch.run(), o)
     print(size, (off / norm).max(), flush=True)
     assert (off <= (2.0 ** -18 + 1.5 * (20 + 4 * spread) * 2.0 ** -22) * norm).all()
+
+
+@pytest.mark.parametrize("H,G,d", [(16, 8, 128), (32, 8, 64)])
+@pytest.mark.parametrize("v_scale", [1e-30, 1e30])
+@pytest.mark.parametrize("part", [0.0, 0.01])
+def test_a_key_that_takes_the_weight_of_huge_or_tiny_values(H, G, d, v_scale, part, rng):
+    """References that have fallen leave large sums, beside values near either end of f32. Results
+    below 2^-126 (of 1e-30, and a share of e^-27) are multiples of 2^-149: the partial results of up
+    to 64 runs, their sum's steps and the result itself are off by half of that each."""
+    batch = Batch(rng, [1300], [[40, 700]], H, G, d, q_scale=2.0, v_scale=v_scale)
+    at = batch.prefix_row[0]
+    v = batch.v[at].copy()
+    sink(batch, at, 30, rng)
+    batch.k[batch.own_row[1] + 3] = batch.k[at] * np.float32(0.8)
+    batch.v[batch.own_row[1] + 3] = 0
+    batch.v[at] = v * np.float32(part)
+    o, _ = batch.want()
+    off, size = (x / v_scale for x in two_norms(batch.run().astype(np.float64), o))
+    least = (64 + 2) * 2.0 ** -150 * math.sqrt(d) / v_scale
+    assert (off <= (2.0 ** -18 + 45 * 2.0 ** -22) * size + least).all(), (off / size).max()

@@ -40,7 +40,7 @@ namespace flk {
 // against the largest score so far alone. A row whose accumulators are kSolid times its sum (of
 // values that are 2^16 at most) does not fall: 2^-25 is little beside what it holds. Nor
 // does one fall farther than l stays below 2^kRoom by. Ordinary scores (2 nats around their mean)
-// rise as often as with the largest score alone, and calls take 0 to 1.5 % longer; with scores 8
+// rise as often as with the largest score alone, and calls take 0 to 2 % longer; with scores 8
 // nats around it -1 to 11 % (32 % without kSolid, whose rows fall and rise in turn).
 constexpr float kDrop = 16.f, kFar = 8.f, kSolid = 256.f;
 constexpr int kRoom = 60;
